@@ -77,8 +77,8 @@ int samx_tree_find_prefixsum(const double* sum_tree, int64_t cap, const double* 
  * u: the B unit uniforms the reference draws with random.random() (host generates them with the
  * same generator and copies them in).  idxs_out int64[B]; iws_out float64[B] (and, if not NULL,
  * iws_f32_out float32[B] — what the critic loss is fed).  Requires num_entries >= 2.
- * Indices, tree sums AND the importance weights are bit-exact: the two pows of memory.py:301,308 go through
- * the device routine that follows the host pow bit for bit (samx_pow_device below). */
+ * Indices, tree sums AND the importance weights are bit-exact: the two pows of memory.py:301,308 are the host's,
+ * called by a host function on the stream (samx_pow_device below). */
 int samx_per_sample(const double* sum_tree, const double* min_tree, int64_t cap,
                     int64_t num_entries, const double* u, int64_t B, double beta,
                     int64_t* idxs_out, double* iws_out, float* iws_f32_out, void* stream);
@@ -99,25 +99,28 @@ int samx_per_leaves_from_td_host(const float* td_host, const int64_t* idxs_host,
                                  int64_t num_entries, double alpha, int64_t num_demos, double demos_eps,
                                  double* leaf_out_host, double* max_priority_host);
 
-/* The same refresh ON THE DEVICE (no host round trip between two prioritized update steps): td float32[n]
+/* The same refresh IN STREAM ORDER (the calling thread waits for nothing): td float32[n]
  * and idxs int64[n] in HBM -> leaf_out float64[n]; entries whose index lies outside [0, cap) mean "nothing
  * pending" and are skipped.  per_state: 16 bytes in HBM, {double max_priority; uint64 error bits}: the running
  * max(priority) (memory.py:379) and the reference's two asserts (bit 0: a priority that is not positive,
  * memory.py:371; bit 1: index >= num_entries, memory.py:372) which the host reads when it next needs them.
- * leaf = priority ** alpha with the host pow's bits (samx_pow_device). */
+ * leaf = priority ** alpha with the host's pow (samx_pow_device). */
 int samx_per_leaves_from_td(const float* td, const int64_t* idxs, int64_t n, int64_t cap, int64_t num_entries,
                             double alpha, int64_t num_demos, double demos_eps, double* leaf_out,
                             void* per_state, void* stream);
 
-/* pow(x[i], y) with the bits of the HOST C library's pow (glibc's table-driven routine, FMA build; constants
- * taken from the image's libm by tools/extract_pow_tables.py), computed on the device: what lets
- * `priority ** alpha` (memory.py:341-342,376-377) and the importance weights (memory.py:301,308) stay in HBM.
- * Bit-for-bit domain: x positive and normal, 2^-65 <= |y| < 2^63, |y log x| < 512; outside it the platform pow
- * answers.  tests/test_gpu_pow.py compares >= 2^26 float32-born bases per exponent against libm.
+/* pow(x[i], y) of the HOST C library for numbers in HBM, in stream order: `priority ** alpha`
+ * (memory.py:341-342,376-377) and the importance weights (memory.py:301,308) reach the host's pow in the reference,
+ * and no other implementation has its last bit.  A kernel writes the bases into pinned staging, a host function on
+ * the stream (hipLaunchHostFunc) calls pow on each, a kernel reads the results back; the calling thread only
+ * enqueues.  This call, samx_per_leaves_from_td[_geom], samx_per_sample[_rows] and samx_per_row_prologue[_td[_rows]]
+ * can all be captured; the staging of a captured call belongs to a buffer that the call writes (out, leaf_out,
+ * iws_out; for the pending update of a prologue the sum tree), is the library's and stays until the process ends.  It
+ * comes out of memory that the first eager call of any of them sets aside: make one before the first capture.
  * samx_pow_device_f32_range / samx_pow_host_f32_range: the same for the n float32 values whose bit patterns
  * start at first_bits, widened to double, + bonus (device result in HBM / libm result in host memory).
- * samx_pow_selfcheck(n): HOST — the number of n pseudo-random cases in which the host build of the routine
- * differs from this machine's libm pow (0 expected; non-zero = another libm code path, keep the host refresh). */
+ * samx_pow_selfcheck(n): HOST — the number of n pseudo-random cases in which that host function differs from this
+ * machine's pow (0). */
 int samx_pow_device(const double* x, double y, int64_t n, double* out, void* stream);
 int samx_pow_device_f32_range(uint32_t first_bits, int64_t n, double bonus, double y, double* out, void* stream);
 int samx_pow_host_f32_range(uint32_t first_bits, int64_t n, double bonus, double y, double* out_host);
@@ -508,11 +511,11 @@ int samx_per_row_prologue(double* sum_tree, double* min_tree, int32_t* stamp, in
                           int64_t copy_skip_lo, int64_t copy_skip_n, void* stream);
 
 /* samx_per_row_prologue with the pending update given as TD ERRORS (upd_td float32[n_upd], HBM): workgroup 0
- * first runs the refresh of samx_per_leaves_from_td on them (leaves kept in LDS, per_state updated), then
+ * gets the leaves that the refresh of samx_per_leaves_from_td makes of them (per_state updated), then
  * goes on as above.  No upload words: every input already lives in HBM, so consecutive prioritized rows can
  * sit in one captured graph (sam_agent.py:693-703 of row k feeding memory.py:266-309 of row k + 1).
  * With u != NULL and cap <= 2^30 the work is spread over more of the chip in two launches: 16 subtree
- * workgroups refresh + rebuild the levels below the top 12 (one more adds the D-input sums), then B/32
+ * workgroups rebuild the levels below the top 12 (one more adds the D-input sums), then B/32
  * workgroups each rebuild the top 12 levels in LDS and draw their share of the row's samples.
  * replay_obs0 == NULL: no D-input sums here (the caller computed them at the head of its launch). */
 int samx_per_row_prologue_td(double* sum_tree, double* min_tree, int32_t* stamp, int64_t cap,

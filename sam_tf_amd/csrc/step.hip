@@ -7,6 +7,7 @@
 #include "nets.h"
 #include "fused_wide.h"
 #include "tree_dev.h"
+#include "per_host.h"
 #include "rng.h"
 #include <stdlib.h>
 #include <mutex>
@@ -287,9 +288,8 @@ __global__ __launch_bounds__(1024) void d_input_stats_kernel(
                        addvec, commit, sums, mean_out, std_out, idx_stride, addvec_stride);
 }
 
-// The pending update given as TD errors instead of leaf values: the refresh itself (|td| + 1e-6 ->
-// priority ** alpha with the host pow's bits, max_priority, the reference's asserts) runs at the head of
-// workgroup 0, the leaves stay in LDS.
+// The pending update given as TD errors instead of leaf values: their leaves are made first, in a stage of the host's
+// pow (per_host.h), which upd_leaf then is.
 struct PerRefresh {
     const float* td;          // null: upd_leaf holds the leaf values
     double alpha, demos_eps;
@@ -306,9 +306,8 @@ __global__ __launch_bounds__(1024) void per_row_prologue_kernel(
     const float* __restrict__ replay_obs0, int64_t ring_start, int64_t ring_len,
     const int64_t* __restrict__ p_idx, const float* __restrict__ pool_obs0,
     const int64_t* __restrict__ e_start, int64_t B, int dim, int dimpad, double* __restrict__ addvec,
-    int64_t n_ent, const double* __restrict__ u, double beta, int64_t* __restrict__ idxs_out,
-    double* __restrict__ iws_out, float* __restrict__ iws32_out, const int64_t* __restrict__ copy_src,
-    int64_t* copy_dst, int64_t copy_n, int64_t skip_lo, int64_t skip_n, PerRefresh rf, int fast) {
+    int64_t n_ent, const double* __restrict__ u, int64_t* __restrict__ idxs_out, double* __restrict__ pw,
+    const int64_t* __restrict__ copy_src, int64_t* copy_dst, int64_t copy_n, int64_t skip_lo, int64_t skip_n, int fast) {
     if (copy_src) {
         // the row's host-drawn words (pinned host memory) -> their device home, by BOTH workgroups (same
         // values to the same addresses; each then reads what it wrote itself): no separate upload node.
@@ -319,26 +318,19 @@ __global__ __launch_bounds__(1024) void per_row_prologue_kernel(
         __syncthreads();
     }
     if (blockIdx.x == 0) {
-        // this workgroup's use of the launch's dynamic LDS (n_upd < 1024): the leaves, and with `fast` the
-        // whole working set of the tree update (tree_dev.h: FastLds)
+        // this workgroup's use of the launch's dynamic LDS (n_upd < 1024): with `fast` the whole working set of the
+        // tree update (tree_dev.h: FastLds)
         extern __shared__ double leaf_sh[];
         samx::FastLds& F = *reinterpret_cast<samx::FastLds*>(leaf_sh);
-        double* leaf_lds = fast ? F.cs : leaf_sh;
-        const double* leaf = upd_leaf;
-        if (rf.td) {
-            samx::leaves_from_td_body(rf.td, upd_idx, n_upd, cap, rf.num_entries, rf.alpha, rf.num_demos,
-                                      rf.demos_eps, leaf_lds, rf.state);
-            leaf = leaf_lds;
-        }
-        if (fast) samx::tree_set_fast_body(ts, tm, cap, upd_idx, leaf, n_upd, levels, F);
-        else samx::tree_set_body(ts, tm, stamp, cap, upd_idx, leaf, n_upd, levels);
+        if (fast) samx::tree_set_fast_body(ts, tm, cap, upd_idx, upd_leaf, n_upd, levels, F);
+        else samx::tree_set_body(ts, tm, stamp, cap, upd_idx, upd_leaf, n_upd, levels);
         if (u) {   // ... and, on the updated trees, this row's stratified sample (memory.py:266-309)
             __syncthreads();
             if (fast)
-                samx::per_sample_body(ts, tm, cap, n_ent, u, B, beta, idxs_out, iws_out, iws32_out, 0, B, F.top_s,
+                samx::per_sample_body(ts, tm, cap, n_ent, u, B, idxs_out, pw, 0, B, F.top_s,
                                       2 * cap < samx::kFastTop ? 2 * cap : samx::kFastTop);
             else
-                samx::per_sample_body(ts, tm, cap, n_ent, u, B, beta, idxs_out, iws_out, iws32_out, 0, B);
+                samx::per_sample_body(ts, tm, cap, n_ent, u, B, idxs_out, pw, 0, B);
         }
     } else {
         d_input_stats_body(0, replay_obs0, ring_start, ring_len, p_idx, pool_obs0, e_start, B, dim, dimpad, addvec,
@@ -347,20 +339,19 @@ __global__ __launch_bounds__(1024) void per_row_prologue_kernel(
 }
 
 // The same head of a prioritized row in TWO launches that fill more of the chip (tree_dev.h: "spread over
-// several workgroups").  Launch 1: G subtree workgroups refresh + walk the lower levels, one more workgroup
+// several workgroups").  Launch 1: G subtree workgroups walk the lower levels, one more workgroup
 // adds the row's D-input sums.  Launch 2: S workgroups each rebuild the top in LDS (workgroup 0 stores it)
 // and draw B / S of the row's samples.
-__global__ __launch_bounds__(1024) void per_refresh_walk_kernel(
-    double* __restrict__ ts, double* __restrict__ tm, int64_t cap, const int64_t* __restrict__ upd_idx, int n_upd,
-    int levels, PerRefresh rf, int G, const float* __restrict__ replay_obs0, int64_t ring_start, int64_t ring_len,
+__global__ __launch_bounds__(1024) void per_walk_kernel(
+    double* __restrict__ ts, double* __restrict__ tm, int64_t cap, const int64_t* __restrict__ upd_idx,
+    const double* __restrict__ upd_leaf, int n_upd, int levels, int G, const float* __restrict__ replay_obs0, int64_t ring_start, int64_t ring_len,
     const int64_t* __restrict__ p_idx, const float* __restrict__ pool_obs0, const int64_t* __restrict__ e_start,
     int64_t B, int dim, int dimpad, double* __restrict__ addvec) {
     extern __shared__ double walk_lds[];
     if ((int)blockIdx.x < G) {
         const int64_t sub = cap / G, lo = (int64_t)blockIdx.x * sub;
-        if (rf.geom) rf.num_entries = rf.geom[1];
-        samx::tree_walk_sub_body(ts, tm, cap, upd_idx, rf.td, n_upd, levels, lo, lo + sub, rf.num_entries, rf.alpha,
-                                 rf.num_demos, rf.demos_eps, rf.state, *reinterpret_cast<samx::WalkLds*>(walk_lds));
+        samx::tree_walk_sub_body(ts, tm, cap, upd_idx, upd_leaf, n_upd, levels, lo, lo + sub,
+                                 *reinterpret_cast<samx::WalkLds*>(walk_lds));
     } else {
         d_input_stats_body(0, replay_obs0, ring_start, ring_len, p_idx, pool_obs0, e_start, B, dim, dimpad, addvec,
                            0, nullptr, nullptr, nullptr, 0, 0);
@@ -369,15 +360,14 @@ __global__ __launch_bounds__(1024) void per_refresh_walk_kernel(
 
 __global__ __launch_bounds__(1024) void per_top_sample_kernel(
     double* __restrict__ ts, double* __restrict__ tm, int64_t cap, int levels, int64_t n_ent,
-    const double* __restrict__ u, int64_t B, double beta, int64_t* __restrict__ idxs_out,
-    double* __restrict__ iws_out, float* __restrict__ iws32_out, int64_t per, samx::SampleExt x) {
+    const double* __restrict__ u, int64_t B, int64_t* __restrict__ idxs_out, double* __restrict__ pw, int64_t per,
+    samx::SampleExt x) {
     extern __shared__ double top_lds[];   // [2][kFastTop]
     double* top_s = top_lds;
     double* top_m = top_lds + samx::kFastTop;
     samx::tree_top_body(ts, tm, cap, levels, top_s, top_m, blockIdx.x == 0);
     const int64_t topn = 2 * (cap >> samx::fast_lb(levels));
-    samx::per_sample_body(ts, tm, cap, n_ent, u, B, beta, idxs_out, iws_out, iws32_out, blockIdx.x * per, per, top_s,
-                          topn, top_m, x);
+    samx::per_sample_body(ts, tm, cap, n_ent, u, B, idxs_out, pw, blockIdx.x * per, per, top_s, topn, top_m, x);
 }
 
 // two device arrays -> pinned host memory in one launch (the TD errors and sampled indices a PER row
@@ -631,7 +621,7 @@ static int per_row_prologue_impl(double* sum_tree, double* min_tree, int32_t* st
                      "samx_per_row_prologue_td_rows: needs the TD form, a sample, cap <= 2^30 and ring_len in [1, cap]");
         num_entries = cap;
     }
-    SAMX_REQUIRE(!rf.td || (rf.state && rf.num_entries >= 0 && rf.num_entries <= cap && samx_pow::in_domain(1.0, rf.alpha)),
+    SAMX_REQUIRE(!rf.td || (rf.state && rf.num_entries >= 0 && rf.num_entries <= cap && samx::pow_exponent_ok(rf.alpha)),
                  "samx_per_row_prologue_td: needs the state words, num_entries in [0, cap] and alpha inside the pow domain");
     SAMX_REQUIRE(cap > 0 && (cap & (cap - 1)) == 0, "samx_per_row_prologue: cap %lld is not a power of two",
                  (long long)cap);
@@ -656,37 +646,59 @@ static int per_row_prologue_impl(double* sum_tree, double* min_tree, int32_t* st
     while ((int64_t(1) << levels) < cap) ++levels;
     int dimpad = 1;
     while (dimpad < ob_dim) dimpad *= 2;
-    if (rf.td && u && cap <= (int64_t(1) << 30)) {
-        int G = 16;
-        while (G > 1 && (cap / G) < (int64_t(1) << samx::fast_lb(levels))) G /= 2;
-        while (G > cap) G /= 2;
-        static LdsGrant grant1;
-        if (int rc = grant1.ensure((const void*)per_refresh_walk_kernel, sizeof(samx::WalkLds))) return rc;
-        per_refresh_walk_kernel<<<G + (sums ? 1 : 0), 1024, sizeof(samx::WalkLds), (hipStream_t)stream>>>(
-            sum_tree, min_tree, cap, upd_idx, (int)n_upd, levels, rf, G, replay_obs0, ring_start, ring_len, p_idx,
-            pool_obs0, e_start, B, ob_dim, dimpad, addvec);
-        SAMX_LAUNCH_CHECK();
-        int S = (int)((B + 31) / 32);
-        if (S > 16) S = 16;
-        const int64_t per = (B + S - 1) / S;
-        const size_t lds2 = 2 * samx::kFastTop * sizeof(double);
-        static LdsGrant grant2;
-        if (int rc = grant2.ensure((const void*)per_top_sample_kernel, lds2)) return rc;
-        per_top_sample_kernel<<<S, 1024, lds2, (hipStream_t)stream>>>(sum_tree, min_tree, cap, levels, num_entries, u,
-                                                                     B, beta, idxs_out, iws_out, iws_f32_out, per, sx);
-        SAMX_LAUNCH_CHECK();
-        return SAMX_OK;
+    // the stages of the host's pow: the pending update's leaves (an output of this call is the tree they go into), the
+    // sample's weights
+    samx::PowStage leaves, weights;
+    const hipStream_t st = (hipStream_t)stream;
+    if (rf.td) {
+        if (int rc = samx::host_pow_stage(sum_tree, n_upd, st, &leaves)) return rc;
+        upd_leaf = leaves.x;
     }
-    const int fast = cap <= (int64_t(1) << 30) ? 1 : 0;   // n_upd < 1024 was required above (tree_set_fast_ok)
-    const size_t lds = fast ? sizeof(samx::FastLds) : 2 * 1024 * sizeof(double);
-    static LdsGrant grant;
-    if (int rc = grant.ensure((const void*)per_row_prologue_kernel, lds, 64 * 1024)) return rc;
-    per_row_prologue_kernel<<<2, 1024, lds, (hipStream_t)stream>>>(
-        sum_tree, min_tree, stamp, cap, upd_idx, upd_leaf, (int)n_upd, levels, replay_obs0, ring_start, ring_len,
-        p_idx, pool_obs0, e_start, B, ob_dim, dimpad, addvec, num_entries, u, beta, idxs_out, iws_out, iws_f32_out,
-        copy_src, copy_dst, copy_n, copy_skip_lo, copy_skip_n, rf, fast);
-    SAMX_LAUNCH_CHECK();
-    return SAMX_OK;
+    if (u) {
+        if (int rc = samx::host_pow_stage(iws_out, B + 1, st, &weights)) {
+            if (rf.td) (void)samx::host_pow_done(leaves, st);
+            return rc;
+        }
+    }
+    const int rc = [&]() -> int {
+        if (rf.td)
+            if (int r = samx::per_leaves_enqueue(rf.td, upd_idx, n_upd, cap, rf.num_entries, rf.alpha, rf.num_demos,
+                                                 rf.demos_eps, rf.state, rf.geom, leaves, st)) return r;
+        if (rf.td && u && cap <= (int64_t(1) << 30)) {
+            int G = 16;
+            while (G > 1 && (cap / G) < (int64_t(1) << samx::fast_lb(levels))) G /= 2;
+            while (G > cap) G /= 2;
+            static LdsGrant grant1;
+            if (int r = grant1.ensure((const void*)per_walk_kernel, sizeof(samx::WalkLds))) return r;
+            per_walk_kernel<<<G + (sums ? 1 : 0), 1024, sizeof(samx::WalkLds), st>>>(
+                sum_tree, min_tree, cap, upd_idx, upd_leaf, (int)n_upd, levels, G, replay_obs0, ring_start, ring_len,
+                p_idx, pool_obs0, e_start, B, ob_dim, dimpad, addvec);
+            SAMX_LAUNCH_CHECK();
+            int S = (int)((B + 31) / 32);
+            if (S > 16) S = 16;
+            const int64_t per = (B + S - 1) / S;
+            const size_t lds2 = 2 * samx::kFastTop * sizeof(double);
+            static LdsGrant grant2;
+            if (int r = grant2.ensure((const void*)per_top_sample_kernel, lds2)) return r;
+            per_top_sample_kernel<<<S, 1024, lds2, st>>>(sum_tree, min_tree, cap, levels, num_entries, u, B, idxs_out,
+                                                         weights.x, per, sx);
+            SAMX_LAUNCH_CHECK();
+        } else {
+            const int fast = cap <= (int64_t(1) << 30) ? 1 : 0;   // n_upd < 1024 was required above (tree_set_fast_ok)
+            const size_t lds = fast ? sizeof(samx::FastLds) : 2 * 1024 * sizeof(double);
+            static LdsGrant grant;
+            if (int r = grant.ensure((const void*)per_row_prologue_kernel, lds, 64 * 1024)) return r;
+            per_row_prologue_kernel<<<2, 1024, lds, st>>>(
+                sum_tree, min_tree, stamp, cap, upd_idx, upd_leaf, (int)n_upd, levels, replay_obs0, ring_start, ring_len,
+                p_idx, pool_obs0, e_start, B, ob_dim, dimpad, addvec, num_entries, u, idxs_out, weights.x, copy_src,
+                copy_dst, copy_n, copy_skip_lo, copy_skip_n, fast);
+            SAMX_LAUNCH_CHECK();
+        }
+        return u ? samx::per_weights_enqueue(weights, B, beta, iws_out, iws_f32_out, st) : SAMX_OK;
+    }();
+    const int rd = rf.td ? samx::host_pow_done(leaves, st) : SAMX_OK;
+    const int re = u ? samx::host_pow_done(weights, st) : SAMX_OK;
+    return rc ? rc : rd ? rd : re;
 }
 
 int samx_per_row_prologue(double* sum_tree, double* min_tree, int32_t* stamp, int64_t cap,

@@ -3,6 +3,7 @@
 // HBM/latency-bound pointer chasing over a 2*cap double array (16 MiB at cap 2^20); no MFMA here.
 #include "samx_common.h"
 #include "tree_dev.h"
+#include "per_host.h"
 #include "../../include/samx.h"
 #include <math.h>
 #include <string.h>
@@ -136,34 +137,67 @@ __global__ void tree_find_kernel(const double* v, int64_t cap, const double* pre
 
 __global__ __launch_bounds__(256) void per_sample_kernel(
     const double* __restrict__ sumv, const double* __restrict__ minv, int64_t cap, int64_t n_ent,
-    const double* __restrict__ u, int64_t B, double beta, int64_t* __restrict__ idxs,
-    double* __restrict__ iws, float* __restrict__ iws32, samx::SampleExt x) {
-    samx::per_sample_body(sumv, minv, cap, n_ent, u, B, beta, idxs, iws, iws32,
+    const double* __restrict__ u, int64_t B, int64_t* __restrict__ idxs, double* __restrict__ pw,
+    samx::SampleExt x) {
+    samx::per_sample_body(sumv, minv, cap, n_ent, u, B, idxs, pw,
                           blockIdx.x * (int64_t)256, 256, nullptr, 0, nullptr, x);   // tree_dev.h
 }
 
-// the priority refresh on the device (memory.py:370-379 for the entries of one update)
-__global__ __launch_bounds__(kTreeThreads) void per_leaves_from_td_kernel(
+// the priorities of one update (memory.py:370-375)
+__global__ __launch_bounds__(kTreeThreads) void per_priorities_kernel(
     const float* __restrict__ td, const int64_t* __restrict__ idxs, int n, int64_t cap, int64_t num_entries,
-    double alpha, int64_t num_demos, double demos_eps, double* __restrict__ leaf_out, samx::PerState* state,
+    int64_t num_demos, double demos_eps, double* __restrict__ prio_out, samx::PerState* state,
     const int64_t* __restrict__ geom) {
     if (geom) num_entries = geom[1];   // the ring's entry count as the launch's upload left it (device words)
-    samx::leaves_from_td_body(td, idxs, n, cap, num_entries, alpha, num_demos, demos_eps, leaf_out, state);
+    samx::priorities_from_td_body(td, idxs, n, cap, num_entries, num_demos, demos_eps, prio_out, state);
 }
 
-__global__ void pow_bits_kernel(const double* __restrict__ x, double y, int64_t n, double* __restrict__ out) {
+// stage -> leaf_out; the skipped entries' leaves are zeros
+__global__ void per_leaves_out_kernel(const double* __restrict__ leaf, const int64_t* __restrict__ idxs, int64_t n,
+                                      int64_t cap, double* __restrict__ leaf_out) {
     const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
-    if (i < n) out[i] = samx_pow::pow_bits(x[i], y);
+    if (i < n) leaf_out[i] = idxs[i] >= 0 && idxs[i] < cap ? leaf[i] : 0.0;
 }
 
-// every float32 base from bits lo on, widened (+ bonus): count of results that differ from `expect` is
-// not formed here - the device writes its results, the host compares (tests/test_gpu_pow.py)
-__global__ void pow_bits_f32_range_kernel(uint32_t lo, int64_t n, double bonus, double y, double* __restrict__ out) {
+// pw[i] = (n * prob_i) ** -beta, pw[B] = the largest weight's (memory.py:301-309)
+__global__ void per_weights_kernel(const double* __restrict__ pw, int64_t B, double* __restrict__ iws,
+                                   float* __restrict__ iws32) {
     const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
-    if (i < n) {
-        const float f = __uint_as_float(lo + (uint32_t)i);
-        out[i] = samx_pow::pow_bits(__dadd_rn((double)f, bonus), y);
+    if (i >= B) return;
+    const double w = pw[i] / pw[B];
+    iws[i] = w;
+    if (iws32) iws32[i] = (float)w;
+}
+
+__global__ void pow_in_kernel(const double* __restrict__ x, int64_t n, double* __restrict__ stage) {
+    const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
+    if (i < n) stage[i] = x[i];
+}
+
+// every float32 base from bits lo on, widened (+ bonus)
+__global__ void pow_in_f32_range_kernel(uint32_t lo, int64_t n, double bonus, double* __restrict__ stage) {
+    const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
+    if (i < n) stage[i] = __dadd_rn((double)__uint_as_float(lo + (uint32_t)i), bonus);
+}
+
+// the host's pow of n values in stages of kPowPart; `in` enqueues the kernel that writes count of them from `at` on
+constexpr int64_t kPowPart = int64_t(1) << 20;
+unsigned blocks_of(int64_t n) { return (unsigned)((n + 255) / 256); }
+
+template <typename In>
+int pow_parts(int64_t n, double y, double* out, hipStream_t st, In in) {
+    for (int64_t at = 0; at < n; at += kPowPart) {
+        const int64_t m = n - at < kPowPart ? n - at : kPowPart;
+        samx::PowStage s;
+        if (int rc = samx::host_pow_stage(out + at, m, st, &s)) return rc;
+        in(at, m, s.x);
+        int rc = samx::host_pow_run(s, m, y, st);
+        if (!rc) pow_in_kernel<<<blocks_of(m), 256, 0, st>>>(s.x, m, out + at);
+        if (int rd = samx::host_pow_done(s, st)) return rd;
+        if (rc) return rc;
+        SAMX_LAUNCH_CHECK();
     }
+    return SAMX_OK;
 }
 
 int levels_of(int64_t cap) {
@@ -173,6 +207,51 @@ int levels_of(int64_t cap) {
 }
 
 }  // namespace
+
+namespace samx {
+
+int per_leaves_enqueue(const float* td, const int64_t* idxs, int64_t n, int64_t cap, int64_t num_entries, double alpha,
+                       int64_t num_demos, double demos_eps, PerState* state, const int64_t* geom, const PowStage& s,
+                       hipStream_t st) {
+    per_priorities_kernel<<<1, kTreeThreads, 0, st>>>(td, idxs, (int)n, cap, num_entries, num_demos, demos_eps, s.x,
+                                                      state, geom);
+    SAMX_LAUNCH_CHECK();
+    return host_pow_run(s, n, alpha, st);
+}
+
+int per_weights_enqueue(const PowStage& s, int64_t B, double beta, double* iws, float* iws32, hipStream_t st) {
+    if (int rc = host_pow_run(s, B + 1, -beta, st)) return rc;
+    per_weights_kernel<<<blocks_of(B), 256, 0, st>>>(s.x, B, iws, iws32);
+    SAMX_LAUNCH_CHECK();
+    return SAMX_OK;
+}
+
+}  // namespace samx
+
+static int per_sample_impl(const double* sum_tree, const double* min_tree, int64_t cap, int64_t num_entries,
+                           const double* u, int64_t B, double beta, int64_t* idxs_out, double* iws_out,
+                           float* iws_f32_out, const samx::SampleExt& x, hipStream_t st) {
+    samx::PowStage s;
+    if (int rc = samx::host_pow_stage(iws_out, B + 1, st, &s)) return rc;
+    per_sample_kernel<<<blocks_of(B), 256, 0, st>>>(sum_tree, min_tree, cap, num_entries, u, B, idxs_out, s.x, x);
+    const int rc = samx::per_weights_enqueue(s, B, beta, iws_out, iws_f32_out, st);
+    const int rd = samx::host_pow_done(s, st);
+    return rc ? rc : rd;
+}
+
+static int per_leaves_impl(const float* td, const int64_t* idxs, int64_t n, int64_t cap, int64_t num_entries,
+                           double alpha, int64_t num_demos, double demos_eps, double* leaf_out, void* per_state,
+                           const int64_t* geom, hipStream_t st) {
+    samx::PowStage s;
+    if (int rc = samx::host_pow_stage(leaf_out, n, st, &s)) return rc;
+    const int rc = samx::per_leaves_enqueue(td, idxs, n, cap, num_entries, alpha, num_demos, demos_eps,
+                                            (samx::PerState*)per_state, geom, s, st);
+    if (!rc) per_leaves_out_kernel<<<blocks_of(n), 256, 0, st>>>(s.x, idxs, n, cap, leaf_out);
+    const int rd = samx::host_pow_done(s, st);
+    if (rc || rd) return rc ? rc : rd;
+    SAMX_LAUNCH_CHECK();
+    return SAMX_OK;
+}
 
 extern "C" {
 
@@ -258,10 +337,8 @@ int samx_per_sample(const double* sum_tree, const double* min_tree, int64_t cap,
                  "samx_per_sample: num_entries %lld must be in [2, cap]", (long long)num_entries);
     SAMX_REQUIRE(B > 0, "samx_per_sample: batch must be positive");
     SAMX_REQUIRE(beta > 0, "samx_per_sample: beta must be positive");
-    per_sample_kernel<<<(unsigned)((B + 255) / 256), 256, 0, (hipStream_t)stream>>>(
-        sum_tree, min_tree, cap, num_entries, u, B, beta, idxs_out, iws_out, iws_f32_out, samx::SampleExt());
-    SAMX_LAUNCH_CHECK();
-    return SAMX_OK;
+    return per_sample_impl(sum_tree, min_tree, cap, num_entries, u, B, beta, idxs_out, iws_out, iws_f32_out,
+                           samx::SampleExt(), (hipStream_t)stream);
 }
 
 int samx_per_sample_rows(const double* sum_tree, const double* min_tree, int64_t cap, const int64_t* geom,
@@ -275,10 +352,8 @@ int samx_per_sample_rows(const double* sum_tree, const double* min_tree, int64_t
     SAMX_REQUIRE(B > 0 && beta > 0, "samx_per_sample_rows: batch and beta must be positive");
     samx::SampleExt x;
     x.geom = geom; x.limit = ring_len; x.rows_out = rows_out; x.idx_copy = idx_copy_out;
-    per_sample_kernel<<<(unsigned)((B + 255) / 256), 256, 0, (hipStream_t)stream>>>(
-        sum_tree, min_tree, cap, 0, u, B, beta, idxs_out, iws_out, iws_f32_out, x);
-    SAMX_LAUNCH_CHECK();
-    return SAMX_OK;
+    return per_sample_impl(sum_tree, min_tree, cap, 0, u, B, beta, idxs_out, iws_out, iws_f32_out, x,
+                           (hipStream_t)stream);
 }
 
 int samx_per_leaf_values_host(const int64_t* idxs_host, const double* prios_host, int64_t n,
@@ -306,12 +381,9 @@ int samx_per_leaves_from_td(const float* td, const int64_t* idxs, int64_t n, int
     SAMX_REQUIRE(td && idxs && leaf_out && per_state, "samx_per_leaves_from_td: null pointer");
     SAMX_REQUIRE(n > 0 && n <= (1 << 24), "samx_per_leaves_from_td: batch %lld out of range", (long long)n);
     SAMX_REQUIRE(cap > 0 && num_entries >= 0 && num_entries <= cap, "samx_per_leaves_from_td: bad cap / num_entries");
-    SAMX_REQUIRE(samx_pow::in_domain(1.0, alpha), "samx_per_leaves_from_td: alpha %g outside the pow domain", alpha);
-    per_leaves_from_td_kernel<<<1, kTreeThreads, 0, (hipStream_t)stream>>>(
-        td, idxs, (int)n, cap, num_entries, alpha, num_demos, demos_eps, leaf_out, (samx::PerState*)per_state,
-        nullptr);
-    SAMX_LAUNCH_CHECK();
-    return SAMX_OK;
+    SAMX_REQUIRE(samx::pow_exponent_ok(alpha), "samx_per_leaves_from_td: alpha %g outside the pow domain", alpha);
+    return per_leaves_impl(td, idxs, n, cap, num_entries, alpha, num_demos, demos_eps, leaf_out, per_state, nullptr,
+                           (hipStream_t)stream);
 }
 
 int samx_per_leaves_from_td_geom(const float* td, const int64_t* idxs, int64_t n, int64_t cap, const int64_t* geom,
@@ -320,26 +392,25 @@ int samx_per_leaves_from_td_geom(const float* td, const int64_t* idxs, int64_t n
     SAMX_REQUIRE(td && idxs && leaf_out && per_state && geom, "samx_per_leaves_from_td_geom: null pointer");
     SAMX_REQUIRE(n > 0 && n <= (1 << 24), "samx_per_leaves_from_td_geom: batch %lld out of range", (long long)n);
     SAMX_REQUIRE(cap > 0, "samx_per_leaves_from_td_geom: bad cap");
-    SAMX_REQUIRE(samx_pow::in_domain(1.0, alpha), "samx_per_leaves_from_td_geom: alpha %g outside the pow domain",
-                 alpha);
-    per_leaves_from_td_kernel<<<1, kTreeThreads, 0, (hipStream_t)stream>>>(
-        td, idxs, (int)n, cap, 0, alpha, num_demos, demos_eps, leaf_out, (samx::PerState*)per_state, geom);
-    SAMX_LAUNCH_CHECK();
-    return SAMX_OK;
+    SAMX_REQUIRE(samx::pow_exponent_ok(alpha), "samx_per_leaves_from_td_geom: alpha %g outside the pow domain", alpha);
+    return per_leaves_impl(td, idxs, n, cap, 0, alpha, num_demos, demos_eps, leaf_out, per_state, geom,
+                           (hipStream_t)stream);
 }
 
 int samx_pow_device(const double* x, double y, int64_t n, double* out, void* stream) {
     SAMX_REQUIRE(x && out && n > 0, "samx_pow_device: bad arguments");
-    pow_bits_kernel<<<(unsigned)((n + 255) / 256), 256, 0, (hipStream_t)stream>>>(x, y, n, out);
-    SAMX_LAUNCH_CHECK();
-    return SAMX_OK;
+    const hipStream_t st = (hipStream_t)stream;
+    return pow_parts(n, y, out, st, [&](int64_t at, int64_t m, double* stage) {
+        pow_in_kernel<<<blocks_of(m), 256, 0, st>>>(x + at, m, stage);
+    });
 }
 
 int samx_pow_device_f32_range(uint32_t first_bits, int64_t n, double bonus, double y, double* out, void* stream) {
     SAMX_REQUIRE(out && n > 0 && n <= (int64_t(1) << 31), "samx_pow_device_f32_range: bad arguments");
-    pow_bits_f32_range_kernel<<<(unsigned)((n + 255) / 256), 256, 0, (hipStream_t)stream>>>(first_bits, n, bonus, y, out);
-    SAMX_LAUNCH_CHECK();
-    return SAMX_OK;
+    const hipStream_t st = (hipStream_t)stream;
+    return pow_parts(n, y, out, st, [&](int64_t at, int64_t m, double* stage) {
+        pow_in_f32_range_kernel<<<blocks_of(m), 256, 0, st>>>(first_bits + (uint32_t)at, m, bonus, stage);
+    });
 }
 
 int samx_pow_host_f32_range(uint32_t first_bits, int64_t n, double bonus, double y, double* out_host) {
@@ -360,9 +431,8 @@ int samx_pow_host(const double* x_host, double y, int64_t n, double* out_host) {
 }
 
 int64_t samx_pow_selfcheck(int64_t n) {
-    // the HOST build of pow_bits against this machine's libm pow on n pseudo-random bases and the two usual
-    // exponent signs; a machine whose libm takes another code path (no FMA/AVX2, another glibc) shows up
-    // here as a non-zero count and the callers keep the host round trip
+    // the host function that the device entry points put on the stream against pow called here, on n pseudo-random
+    // bases and the usual exponents
     uint64_t s = 0x9E3779B97F4A7C15ull;
     int64_t bad = 0;
     const double ys[4] = {0.3, 0.6, -0.4, -1.0};
@@ -370,10 +440,11 @@ int64_t samx_pow_selfcheck(int64_t n) {
         s ^= s << 13; s ^= s >> 7; s ^= s << 17;
         const uint64_t ex = 1023 - 30 + (s >> 52) % 61;
         const uint64_t u = (ex << 52) | ((s * 0x2545F4914F6CDD1Dull) & ((1ull << 52) - 1));
-        double x;
+        double x, a;
         memcpy(&x, &u, 8);
-        const double y = ys[i & 3];
-        const double a = samx_pow::pow_bits(x, y), b = pow(x, y);
+        a = x;
+        samx::host_pow_values(&a, 1, ys[i & 3]);
+        const double b = pow(x, ys[i & 3]);
         if (memcmp(&a, &b, 8) != 0) ++bad;
     }
     return bad;

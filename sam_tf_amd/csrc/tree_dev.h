@@ -5,7 +5,6 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <math.h>
-#include "pow_bits.h"
 
 namespace samx {
 
@@ -27,25 +26,23 @@ struct PerState {
     unsigned long long err;
 };
 
-// One entry of the priority refresh (sam_agent.py:702 -> memory.py:370-379): priority = |td| + 1e-6 in
-// float32, widened; the demonstration bonus; leaf = priority ** alpha with the bits of the host pow
-// (pow_bits.h).  Same arithmetic as samx_per_leaves_from_td_host.
-__device__ __forceinline__ double leaf_from_td(float td, int64_t idx, int64_t num_demos, double demos_eps,
-                                               double alpha, double* prio) {
+// One entry's priority in the refresh (sam_agent.py:702 -> memory.py:370-375): |td| + 1e-6 in float32, widened; the
+// demonstration bonus.  The leaf, priority ** alpha, is the host's pow of it (host_pow.h).  Same arithmetic as
+// samx_per_leaves_from_td_host.
+__device__ __forceinline__ double priority_from_td(float td, int64_t idx, int64_t num_demos, double demos_eps) {
     const float p32 = __fadd_rn(fabsf(td), 1e-6f);
     double p = (double)p32;
     if (num_demos > 0 && idx < num_demos) p = __dadd_rn(p, demos_eps);
-    *prio = p;
-    return samx_pow::pow_bits(p, alpha);
+    return p;
 }
 
-// The refresh of n entries by one workgroup (every thread calls this; barrier inside): leaves -> leaf_out
-// (LDS or global), max_priority and the reference's two asserts -> state.  Entries whose index is outside
+// The priorities of n refreshed entries by one workgroup (every thread calls this; barrier inside) -> prio_out (the
+// stage of the host's pow), max_priority and the reference's two asserts -> state.  Entries whose index is outside
 // [0, cap) are the "nothing pending" marker and are skipped.
-__device__ __forceinline__ void leaves_from_td_body(const float* __restrict__ td, const int64_t* __restrict__ idxs,
-                                                    int n, int64_t cap, int64_t num_entries, double alpha,
-                                                    int64_t num_demos, double demos_eps, double* leaf_out,
-                                                    PerState* state) {
+__device__ __forceinline__ void priorities_from_td_body(const float* __restrict__ td, const int64_t* __restrict__ idxs,
+                                                        int n, int64_t cap, int64_t num_entries, int64_t num_demos,
+                                                        double demos_eps, double* __restrict__ prio_out,
+                                                        PerState* state) {
     __shared__ double wmax[kTreeThreads / 64];
     __shared__ unsigned werr[kTreeThreads / 64];
     const int tid = threadIdx.x;
@@ -53,9 +50,9 @@ __device__ __forceinline__ void leaves_from_td_body(const float* __restrict__ td
     unsigned err = 0;
     for (int i = tid; i < n; i += kTreeThreads) {
         const int64_t idx = idxs[i];
-        if (idx < 0 || idx >= cap) { leaf_out[i] = 0.0; continue; }
-        double p;
-        leaf_out[i] = leaf_from_td(td[i], idx, num_demos, demos_eps, alpha, &p);
+        if (idx < 0 || idx >= cap) { prio_out[i] = 0.0; continue; }
+        const double p = priority_from_td(td[i], idx, num_demos, demos_eps);
+        prio_out[i] = p;
         if (!(p > 0.0)) err |= 1u;
         if (idx >= num_entries) err |= 2u;
         if (p > mx) mx = p;
@@ -307,7 +304,7 @@ __device__ __forceinline__ void tree_set_fast_body(double* __restrict__ s, doubl
 // One workgroup's random 8-byte loads (every entry's old sibling at every level below the top: ~18 per
 // entry) are bound by what ONE compute unit can keep in flight, not by latency.  So the lower levels are
 // split by SUBTREE (as tree_set_sub_kernel does for large batches): workgroup g of G takes the entries whose
-// leaf lies in [g cap/G, (g+1) cap/G), refreshes them (leaf_from_td) and walks them up to the lowest level
+// leaf lies in [g cap/G, (g+1) cap/G) and walks them up to the lowest level
 // that fits the top (tree_walk_sub_body); the workgroups of the NEXT launch each load that level (coalesced),
 // recompute the top densely in LDS (tree_top_body; workgroup 0 stores it) and sample on it.
 struct WalkLds {
@@ -321,15 +318,13 @@ __host__ __device__ __forceinline__ int fast_lb(int levels) {
     return levels + 1 > kFastTopLevels ? levels + 1 - kFastTopLevels : 0;
 }
 
-// entries [0, n) with leaf in [lo, hi): refresh from TD errors, duplicates, leaves and `lb` levels of parents.
+// entries [0, n) with leaf in [lo, hi): duplicates, leaves and `lb` levels of parents.
 // The workgroup first compacts its entries onto its first threads; waves left without an entry end at once
 // (s_barrier only waits for the waves still alive), so a subtree with <= 64 entries - the usual case - is
 // walked by ONE wave whose barriers cost nothing.
 __device__ __forceinline__ void tree_walk_sub_body(double* __restrict__ s, double* __restrict__ m, int64_t cap,
-                                                   const int64_t* __restrict__ idxs, const float* __restrict__ td,
-                                                   int n, int levels, int64_t lo, int64_t hi, int64_t num_entries,
-                                                   double alpha, int64_t num_demos, double demos_eps,
-                                                   PerState* state, WalkLds& L) {
+                                                   const int64_t* __restrict__ idxs, const double* __restrict__ leaf,
+                                                   int n, int levels, int64_t lo, int64_t hi, WalkLds& L) {
     __shared__ int mine_cnt;
     const int tid = threadIdx.x;
     const int lb = fast_lb(levels);
@@ -372,17 +367,7 @@ __device__ __forceinline__ void tree_walk_sub_body(double* __restrict__ s, doubl
         }
     }
     SAMX_TREE_STAMP(9)
-    if (active) {   // memory.py:370-379 for this entry; the state words take max / or from every workgroup
-        double p;
-        vs = vm = leaf_from_td(td[entry], node - cap, num_demos, demos_eps, alpha, &p);
-        unsigned long long err = 0;
-        if (!(p > 0.0)) err |= 1ull;
-        if (node - cap >= num_entries) err |= 2ull;
-        if (err) atomicOr(&state->err, err);
-        // positive doubles order like their bit patterns
-        if (p > 0.0) atomicMax(reinterpret_cast<unsigned long long*>(&state->max_priority),
-                               (unsigned long long)__double_as_longlong(p));
-    }
+    if (active) vs = vm = leaf[entry];   // memory.py:376-377
     SAMX_TREE_STAMP(10)
     lds_bar();
     SAMX_TREE_STAMP(11)
@@ -675,15 +660,15 @@ struct SampleExt {
     int64_t* idx_copy = nullptr;     // second copy of the sampled LOGICAL indices (the pending-update buffer)
 };
 
-// PrioritizedRB._sample_w_priorities + the importance weights (memory.py:266-309) for samples
+// PrioritizedRB._sample_w_priorities + the bases of the importance weights (memory.py:266-309; pw[i] = n * prob of
+// sample i, pw[B] = n * the lowest, whose -beta-th power by the host's pow the weights are divided by) for samples
 // first .. first + span of a batch of B, by ONE workgroup in which every thread calls this (barrier
 // inside); the threads with threadIdx.x < 256 work: three waves take the three scalar range reductions,
 // each with one round of loads (range_reduce_wave), meanwhile the top levels of the sum tree are copied
 // into LDS for the descents.
 __device__ __forceinline__ void per_sample_body(const double* __restrict__ sumv, const double* __restrict__ minv,
                                                 int64_t cap, int64_t n_ent, const double* __restrict__ u,
-                                                int64_t B, double beta, int64_t* __restrict__ idxs,
-                                                double* __restrict__ iws, float* __restrict__ iws32,
+                                                int64_t B, int64_t* __restrict__ idxs, double* __restrict__ pw,
                                                 int64_t first, int64_t span, const double* ext_top = nullptr,
                                                 int64_t ext_top_n = 0, const double* ext_top_min = nullptr,
                                                 const SampleExt& x = SampleExt()) {
@@ -721,7 +706,7 @@ __device__ __forceinline__ void per_sample_body(const double* __restrict__ sumv,
     const double piece = p_total / (double)B;
     const double n = (double)n_ent;
     const double lowest = lowest_p / total;
-    const double max_w = samx_pow::pow_bits(__dmul_rn(n, lowest), -beta);
+    if (first == 0 && tid == 0) pw[B] = __dmul_rn(n, lowest);
     for (int64_t i = first + tid; i < B && i < first + span; i += 256) {
         const double s = __dadd_rn(__dmul_rn(u[i], piece), __dmul_rn((double)i, piece));
         double lv = 0.0;
@@ -735,9 +720,7 @@ __device__ __forceinline__ void per_sample_body(const double* __restrict__ sumv,
             x.rows_out[i] = r;
         }
         const double prob = (have ? lv : sumv[cap + idx]) / total;
-        const double w = samx_pow::pow_bits(__dmul_rn(n, prob), -beta) / max_w;
-        iws[i] = w;
-        if (iws32) iws32[i] = (float)w;
+        pw[i] = __dmul_rn(n, prob);
     }
 }
 

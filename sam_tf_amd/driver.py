@@ -102,8 +102,8 @@ class UpdateStepDriver(object):
         self.per = bool(mu.hps.prioritized_replay)
         self.use_graph = bool(use_graph)
         # PER, one process: the priority refresh (|td| + 1e-6 -> priority ** alpha, max_priority, the asserts;
-        # sam_agent.py:693-703 -> memory.py:370-379) stays ON THE DEVICE — its pow carries the host libm's bits
-        # (csrc/pow_bits.h), checked against this machine's libm when the driver is built.  Rows then need no
+        # sam_agent.py:693-703 -> memory.py:370-379) stays ON THE STREAM — its pow is the host's, called by a
+        # host function between two kernels (csrc/host_pow.h), checked when the driver is built.  Rows then need no
         # host between them and are packed K per graph like uniform replay.  per_host_pow=True (or
         # SAMX_PER_HOST_POW=1, or a libm the routine does not reproduce) keeps the host refresh of round 1.
         self.per_dev = bool(self.per and self.comm.Get_size() == 1 and not per_host_pow and

@@ -120,8 +120,8 @@ _POW_OK = None
 
 
 def pow_matches_host(n=200000):
-    """True when the library's pow routine reproduces THIS machine's libm pow bit for bit on n host-side
-    cases (samx_pow_selfcheck) — the condition for keeping the priority refresh on the device."""
+    """True when the host function that the library puts on a stream gives THIS machine's libm pow on n cases
+    (samx_pow_selfcheck)."""
     global _POW_OK
     if _POW_OK is None:
         _POW_OK = int(_L().samx_pow_selfcheck(int(n))) == 0
@@ -177,11 +177,11 @@ _POW_DEV_OK = {}
 
 
 def pow_device_matches_host(alpha, beta, device='cuda', n=4096):
-    """True when the DEVICE build of the pow routine gives this machine's libm bits for the exponents this replay
-    buffer uses: priority ** alpha on float32-born bases (memory.py:341-342,376-377) and (p * N) ** -beta on
-    double ratios (memory.py:301,308).  pow_matches_host checks the host build of the same source on fixed
-    exponents; the device compiler lowers fma / division on its own, so the driver asks this before it keeps the
-    priority refresh on the device (a mismatch falls back to the host refresh: slower, same results)."""
+    """True when pow in stream order (samx_pow_device: pinned staging and a host function) gives this machine's libm
+    bits for the exponents this replay buffer uses: priority ** alpha on float32-born bases
+    (memory.py:341-342,376-377) and (p * N) ** -beta on double ratios (memory.py:301,308).  The driver asks this
+    before it keeps the priority refresh on the stream (a mismatch falls back to the host refresh: slower, same
+    results); the call also sets aside the staging that captured calls take theirs from."""
     dev = torch.device(device)
     key = (float(alpha), float(beta), dev.index if dev.index is not None else torch.cuda.current_device())
     if key not in _POW_DEV_OK:
@@ -199,7 +199,7 @@ def pow_device_matches_host(alpha, beta, device='cuda', n=4096):
 
 
 def pow_device(x, y):
-    """x float64 device tensor -> x ** y with the host pow's bits (samx_pow_device)."""
+    """x float64 device tensor -> x ** y by the host's pow, in stream order (samx_pow_device)."""
     _chk(x, F64, (x.numel(),), 'x')
     out = torch.empty_like(x)
     check(_L().samx_pow_device(ptr(x), float(y), x.numel(), ptr(out), stream_ptr()))
