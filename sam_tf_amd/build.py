@@ -13,7 +13,9 @@ SO = os.path.join(HERE, 'libsamx.so')
 SOURCES = ['core.hip', 'host_pow.hip', 'tree.hip', 'replay.hip', 'optim.hip', 'gemm.hip', 'nets.hip',
            'fused_small.hip', 'fused_ln.hip', 'fused_wide.hip', 'step.hip']
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-ffp-contract=off',
-         '-fno-fast-math', '-Wall', '-Wno-unused-function'] + os.environ.get('SAMX_EXTRA_FLAGS', '').split()
+         '-fno-fast-math', '-Wall', '-Wno-unused-function',
+         # no packed float32 arithmetic: some of its forms have given wrong results on this hardware now and then
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops'] + os.environ.get('SAMX_EXTRA_FLAGS', '').split()
 
 
 def _sources():
