@@ -635,6 +635,54 @@ int samx_step_grads_part(const samx_learner* L, const samx_batch* batch, const s
 int samx_step_apply(const samx_learner* L, int64_t B, int mode, float grad_scale, void* ws,
                     size_t ws_bytes, void* stream);
 
+/* ---- sequence policies --------------------------------------------------------------------------------------------
+ * The parts of a policy that reads a trajectory, each with its gradient: the norms around a block, linear attention with a
+ * decay for each head (the recurrent form when acting), imitation of a teacher's top logits.  No counterpart in the
+ * reference, whose networks are two dense layers (networks.py:222-422).  Element types of the activations: */
+#define SAMX_F32 0
+#define SAMX_BF16 1
+#define SAMX_F16 2
+
+/* The norm behind a block, its gate, the scaled residual and the norm in front of the next block, over N rows of D:
+ *   h = res_scale x + g N(y; post_w, post_b) ;  u = N(h; pre_w, pre_b)
+ * N is LayerNorm (with its bias; helpers/network_util.py:43-56 has it behind a layer) or, without one, the RMS norm.
+ * x, y, h, u: dense [N, D] of the element type; weights and biases float32 [D]; g by gate_kind: none, float32 [D]
+ * (SAMX_GATE_CHANNEL) or the element type [N, D] (SAMX_GATE_FULL).  D at most 16384 (float32: 8192).  Statistics are float32,
+ * of h before it is rounded.  h may be x's own buffer or y's, u the other one. */
+#define SAMX_NORM_RMS 0
+#define SAMX_NORM_LAYER 1
+#define SAMX_GATE_NONE 0
+#define SAMX_GATE_CHANNEL 1
+#define SAMX_GATE_FULL 2
+int samx_block_norm(const void* x, const void* y, int dtype, int64_t N, int64_t D, const float* post_w,
+                    const float* post_b, int gate_kind, const void* gate, const float* pre_w, const float* pre_b,
+                    float res_scale, int kind, float eps, void* h, void* u, void* stream);
+/* Its gradient, from dh (the gradient of h by the residual path) and du (of u); y and h as the forward pass left them,
+ * their statistics are taken again.  dx, dy: [N, D]; dgate: float32 [D] or [N, D] as the gate; dpost_w, dpre_w (and with
+ * LayerNorm dpost_b, dpre_b): float32 [D], sums over the rows in a fixed order.  dx may be dh's own buffer, dy du's. */
+size_t samx_block_norm_grad_ws_bytes(int dtype, int64_t N, int64_t D);
+int samx_block_norm_grad(const void* y, const void* h, const void* dh, const void* du, int dtype, int64_t N, int64_t D,
+                         const float* post_w, const float* post_b, int gate_kind, const void* gate, const float* pre_w,
+                         float res_scale, int kind, float eps, void* dx, void* dy, void* dgate, float* dpost_w,
+                         float* dpost_b, float* dpre_w, float* dpre_b, void* ws, size_t ws_bytes, void* stream);
+
+/* Imitation of a teacher's top logits: for each of N rows of V student logits z (rows ld apart) and the K entries
+ * (idx int32 [N, K], teacher float32 [N, K]) that are known of the teacher's row,
+ *   p_k = e^{t_k / tau - lse}   (lse float32 [N]: the teacher's own log-normaliser at tau; NULL: over the K entries)
+ *   loss = w sum_k p_k (log p_k - log softmax(z / tau)[idx_k])          float32 [N]; w = weight[row], NULL: 1
+ * samx_distill_grad also writes the gradient of scale * sum(loss) to grad (element type, rows ld_grad apart; columns behind
+ * V stay as they were; grad may be the logits' own buffer with their stride).
+ * Entries with an index outside [0, V) do not count (a row may know fewer than K); an index that stands twice counts twice.
+ * A row of weight 0 has loss 0 and gradient 0 whatever its logits hold.  Logits of -inf have probability 0; a row of nothing
+ * else has q = 0 (loss +inf where the teacher has any mass). */
+#define SAMX_DISTILL_MAX_K 1024
+int samx_distill_loss(const void* logits, int64_t ld, int dtype, int64_t N, int64_t V, const int32_t* idx,
+                      const float* teacher, int K, float tau, const float* lse, const float* weight, float* loss,
+                      void* stream);
+int samx_distill_grad(const void* logits, int64_t ld, int dtype, int64_t N, int64_t V, const int32_t* idx,
+                      const float* teacher, int K, float tau, const float* lse, const float* weight, float scale,
+                      float* loss, void* grad, int64_t ld_grad, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -149,6 +149,12 @@ SIGNATURES = {
     'samx_step_grads': (C.c_int, [_LP, _BP, _OP, _P, _SZ, _P]),
     'samx_step_grads_part': (C.c_int, [_LP, _BP, _OP, _P, _SZ, C.c_int, _P]),
     'samx_step_apply': (C.c_int, [_LP, _I64, C.c_int, _F, _P, _SZ, _P]),
+    'samx_block_norm': (C.c_int, [_P, _P, C.c_int, _I64, _I64, _P, _P, C.c_int, _P, _P, _P, _F, C.c_int, _F, _P, _P, _P]),
+    'samx_block_norm_grad_ws_bytes': (_SZ, [C.c_int, _I64, _I64]),
+    'samx_block_norm_grad': (C.c_int, [_P, _P, _P, _P, C.c_int, _I64, _I64, _P, _P, C.c_int, _P, _P, _F, C.c_int, _F,
+                                       _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    'samx_distill_loss': (C.c_int, [_P, _I64, C.c_int, _I64, _I64, _P, _P, C.c_int, _F, _P, _P, _P, _P]),
+    'samx_distill_grad': (C.c_int, [_P, _I64, C.c_int, _I64, _I64, _P, _P, C.c_int, _F, _P, _P, _F, _P, _P, _I64, _P]),
 }
 
 _lib = None

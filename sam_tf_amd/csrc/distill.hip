@@ -1,0 +1,313 @@
+// Imitation of a teacher's top logits: the cross-entropy part of KL(teacher || student) on K entries of a row of V logits,
+// and its gradient.
+//
+//   x_k = t_k / tau - lse ;  p_k = e^{x_k}                lse: the teacher's normaliser, or over the K entries themselves
+//   lse_z = log sum_j e^{z_j / tau}
+//   loss = w sum_k p_k (x_k - (z_{i_k} / tau - lse_z))
+//   grad_j = (scale w / tau) (P q_j - sum_{k: i_k = j} p_k),   q = softmax(z / tau),  P = sum_k p_k
+//
+// Bound: HBM, the logits read once and the gradient written once.  A row therefore stays in the registers of the threads
+// that read it (up to 16 pieces of 16 bytes for each of 1024 threads: 131072 bf16 or 65536 float32 values); only a wider
+// row is read twice.  Sums and statistics are float32, the K terms of the loss float64 (they cancel where student and
+// teacher agree); each gradient value is rounded once.
+#include "seq_dev.h"
+#include "../../include/samx.h"
+
+namespace {
+
+using namespace samx::seq;
+
+struct Args {
+    const void* z; int64_t ld; int64_t N, V;
+    const int32_t* idx; const float* teacher; int K;
+    double inv_tau;
+    const float* lse; const float* weight;
+    double scale;           // of the gradient: scale / tau
+    float* loss; void* grad; int64_t ldg;
+};
+
+// dynamic LDS of a row: {index, p, z} of its K entries
+__host__ __device__ __forceinline__ size_t row_lds(int K) { return (size_t)((K + 3) & ~3) * 12; }
+
+struct RowStat { float m, rs; };   // the row's maximum (0 where there is none) and one over sum e^{(z - m) / tau}
+
+// What a row's threads do with the teacher's K entries once the statistics of the student are known.  Entries outside
+// [0, V) do not count.
+template <typename T, int G>
+struct Teacher {
+    int32_t* si; float* sp; float* sz;
+    int K;
+    __device__ Teacher(char* lds, int K_) : K(K_) {
+        const int n = (K_ + 3) & ~3;
+        si = (int32_t*)lds; sp = (float*)lds + n; sz = (float*)lds + 2 * n;
+    }
+    // indices, the student's logits there (before anything of the row is overwritten) and the largest teacher logit
+    __device__ __forceinline__ float load(const Args& a, int64_t row, int lane, bool on) {
+        const T* z = (const T*)a.z + row * a.ld;
+        float mt = -INFINITY;
+        for (int k = lane; k < ((K + 3) & ~3); k += G) {
+            int32_t i = -1;
+            float t = -INFINITY;
+            if (on && k < K) {
+                i = a.idx[row * K + k];
+                if (i < 0 || i >= a.V) i = -1;
+                else t = a.teacher[row * K + k];
+            }
+            si[k] = i;
+            sp[k] = t;
+            sz[k] = i >= 0 ? to_float(z[i]) : 0.f;
+            mt = OpMax::f(mt, t);
+        }
+        return mt;
+    }
+    // sum of e^{(t - mt) / tau} (this thread's part)
+    __device__ __forceinline__ float sum(float mt, float c2, int lane) const {
+        float s = 0.f;
+        for (int k = lane; k < K; k += G) s += __builtin_amdgcn_exp2f((sp[k] - mt) * c2);
+        return s;
+    }
+    // sp <- p_k; this thread's part of {P, loss}
+    __device__ __forceinline__ void terms(double inv_tau, double lse_t, double lse_z, int lane, double (&v)[2]) {
+        v[0] = v[1] = 0.0;
+        for (int k = lane; k < K; k += G) {
+            const double x = (double)sp[k] * inv_tau - lse_t;
+            const float p = expf((float)x);
+            sp[k] = p;
+            if (p != 0.f) {   // (a NaN comes through)
+                v[0] += (double)p;
+                v[1] += (double)p * (x - ((double)sz[k] * inv_tau - lse_z));
+            }
+        }
+    }
+    // the entries' own gradients, over what the row's stores have left there; an index that stands twice is written by
+    // the first of its entries, with the sum of all
+    __device__ __forceinline__ void write(T* g, float c2, const RowStat& r, float cq, float cp, int lane) const {
+        for (int k = lane; k < K; k += G) {
+            const int32_t i = si[k];
+            if (i < 0) continue;
+            float p = 0.f;
+            bool first = true;
+            for (int j = 0; j < K; j += 4) {
+                const int4 o = *reinterpret_cast<const int4*>(si + j);
+                const int32_t e[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (e[u] == i) {
+                        if (j + u < k) first = false;
+                        p += sp[j + u];
+                    }
+            }
+            if (first) g[i] = from_float<T>(cq * (__builtin_amdgcn_exp2f((sz[k] - r.m) * c2) * r.rs) - cp * p);
+        }
+    }
+};
+
+// log sum e^{z / tau}; of a row of nothing but -inf 0, so that log q stays -inf there
+__device__ __forceinline__ double row_lse(float m, float s, double inv_tau) {
+    return s > 0.f || s != s ? (double)m * inv_tau + log((double)s) : 0.0;
+}
+
+// One row for every G threads, the row in their registers (NV pieces each).
+template <typename T, int G, int NV, bool GRAD>
+__global__ __launch_bounds__(G < 256 ? 256 : G) void row_kernel(Args a) {
+    constexpr int B = G < 256 ? 256 : G, W = B / 64, N = Piece<T>::kN;
+    extern __shared__ char lds[];
+    __shared__ float shf[2 * W * 2];
+    __shared__ double shd[2 * W * 2];
+    int turn = 0, turnd = 0;
+    const int lane = threadIdx.x % G;
+    const int64_t row = (int64_t)blockIdx.x * (B / G) + threadIdx.x / G;
+    const bool live = row < a.N;
+    float w = 0.f;
+    if (live) w = a.weight ? a.weight[row] : 1.f;
+    const bool on = live && w != 0.f;      // a row of weight zero is not looked at
+    const T* z = (const T*)a.z + (live ? row : 0) * a.ld;
+    const T none = from_float<T>(-INFINITY);
+    Piece<T> raw[NV];
+    if (on) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) raw[v] = load_piece(z, ((int64_t)v * G + lane) * N, a.V, none);
+    } else {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int j = 0; j < N; ++j) raw[v].e[j] = none;
+    }
+    Teacher<T, G> te(lds + (threadIdx.x / G) * row_lds(a.K), a.K);
+    const float c2 = (float)(a.inv_tau * 1.4426950408889634);
+    float mx[2] = {-INFINITY, te.load(a, row, lane, on)};
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int j = 0; j < N; ++j) mx[0] = OpMax::f(mx[0], to_float(raw[v].e[j]));
+    row_reduce<OpMax, G>(mx, shf, W, turn);
+    RowStat r;
+    r.m = mx[0] == -INFINITY ? 0.f : mx[0];
+    const float mt = mx[1] == -INFINITY ? 0.f : mx[1];
+    float s[2] = {0.f, a.lse ? 0.f : te.sum(mt, c2, lane)};
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int j = 0; j < N; ++j) s[0] += __builtin_amdgcn_exp2f((to_float(raw[v].e[j]) - r.m) * c2);
+    row_reduce<OpSum, G>(s, shf, W, turn);
+    r.rs = s[0] > 0.f || s[0] != s[0] ? 1.f / s[0] : 0.f;
+    const double lse_z = row_lse(r.m, s[0], a.inv_tau);
+    double lse_t = 0.0;
+    if (on) lse_t = a.lse ? (double)a.lse[row] : row_lse(mt, s[1], a.inv_tau);
+    double tl[2];
+    te.terms(a.inv_tau, lse_t, lse_z, lane, tl);
+    row_reduce<OpSum, G>(tl, shd, W, turnd);
+    if (live && lane == 0) a.loss[row] = on ? (float)((double)w * tl[1]) : 0.f;
+    if constexpr (GRAD) {
+        const float cp = on ? (float)(a.scale * (double)w) : 0.f, cq = on ? (float)(a.scale * (double)w * tl[0]) : 0.f;
+        T* g = (T*)a.grad + (live ? row : 0) * a.ldg;
+        const float f = cq * r.rs;
+        if (live) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                Piece<T> o;
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    o.e[j] = from_float<T>(f * __builtin_amdgcn_exp2f((to_float(raw[v].e[j]) - r.m) * c2));
+                store_piece(g, ((int64_t)v * G + lane) * N, a.V, o);
+            }
+        }
+        __syncthreads();
+        if (on) te.write(g, c2, r, cq, cp, lane);
+    }
+}
+
+// A row that does not fit: 1024 threads read it twice.
+template <typename T, bool GRAD>
+__global__ __launch_bounds__(1024) void wide_kernel(Args a) {
+    constexpr int G = 1024, W = G / 64, N = Piece<T>::kN, U = 4;
+    extern __shared__ char lds[];
+    __shared__ float shf[2 * W * 2];
+    __shared__ double shd[2 * W * 2];
+    int turn = 0, turnd = 0;
+    const int lane = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    const float w = a.weight ? a.weight[row] : 1.f;
+    const bool on = w != 0.f;
+    const T* z = (const T*)a.z + row * a.ld;
+    const T none = from_float<T>(-INFINITY);
+    Teacher<T, G> te(lds, a.K);
+    const float c2 = (float)(a.inv_tau * 1.4426950408889634);
+    float mx[2] = {-INFINITY, te.load(a, row, lane, on)}, part = 0.f;
+    for (int64_t at = (int64_t)lane * N; on && at < a.V; at += (int64_t)U * G * N) {
+        Piece<T> raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = load_piece(z, at + (int64_t)u * G * N, a.V, none);
+        float m = mx[0];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < N; ++j) m = OpMax::f(m, to_float(raw[u].e[j]));
+        const float mm = m == -INFINITY ? 0.f : m;
+        part *= __builtin_amdgcn_exp2f((mx[0] - mm) * c2);      // (0 at first: 0 * e^-inf)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < N; ++j) part += __builtin_amdgcn_exp2f((to_float(raw[u].e[j]) - mm) * c2);
+        mx[0] = m;
+    }
+    const float own = mx[0];
+    row_reduce<OpMax, G>(mx, shf, W, turn);
+    RowStat r;
+    r.m = mx[0] == -INFINITY ? 0.f : mx[0];
+    const float mt = mx[1] == -INFINITY ? 0.f : mx[1];
+    float s[2] = {part * __builtin_amdgcn_exp2f((own - r.m) * c2), a.lse ? 0.f : te.sum(mt, c2, lane)};
+    row_reduce<OpSum, G>(s, shf, W, turn);
+    r.rs = s[0] > 0.f || s[0] != s[0] ? 1.f / s[0] : 0.f;
+    const double lse_z = row_lse(r.m, s[0], a.inv_tau);
+    double lse_t = 0.0;
+    if (on) lse_t = a.lse ? (double)a.lse[row] : row_lse(mt, s[1], a.inv_tau);
+    double tl[2];
+    te.terms(a.inv_tau, lse_t, lse_z, lane, tl);
+    row_reduce<OpSum, G>(tl, shd, W, turnd);
+    if (lane == 0) a.loss[row] = on ? (float)((double)w * tl[1]) : 0.f;
+    if constexpr (GRAD) {
+        const float cp = on ? (float)(a.scale * (double)w) : 0.f, cq = on ? (float)(a.scale * (double)w * tl[0]) : 0.f;
+        T* g = (T*)a.grad + row * a.ldg;
+        const float f = cq * r.rs;
+        for (int64_t at = (int64_t)lane * N; at < a.V; at += (int64_t)U * G * N) {
+            Piece<T> raw[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) raw[u] = load_piece(z, at + (int64_t)u * G * N, on ? a.V : 0, none);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                Piece<T> o;
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    o.e[j] = from_float<T>(f * __builtin_amdgcn_exp2f((to_float(raw[u].e[j]) - r.m) * c2));
+                store_piece(g, at + (int64_t)u * G * N, a.V, o);
+            }
+        }
+        __syncthreads();
+        if (on) te.write(g, c2, r, cq, cp, lane);
+    }
+}
+
+template <typename T, int G, int NV, bool GRAD>
+int launch_row(const Args& a, hipStream_t st) {
+    constexpr int B = G < 256 ? 256 : G, R = B / G;
+    row_kernel<T, G, NV, GRAD><<<(unsigned)((a.N + R - 1) / R), B, R * row_lds(a.K), st>>>(a);
+    SAMX_LAUNCH_CHECK();
+    return SAMX_OK;
+}
+
+template <typename T, bool GRAD>
+int launch(const Args& a, hipStream_t st) {
+    const int64_t n = (a.V + Piece<T>::kN - 1) / Piece<T>::kN;   // pieces of a row
+    if (n <= 64) return launch_row<T, 64, 1, GRAD>(a, st);
+    if (n <= 128) return launch_row<T, 64, 2, GRAD>(a, st);
+    if (n <= 256) return launch_row<T, 64, 4, GRAD>(a, st);
+    if (n <= 512) return launch_row<T, 256, 2, GRAD>(a, st);
+    if (n <= 1024) return launch_row<T, 256, 4, GRAD>(a, st);
+    if (n <= 2048) return launch_row<T, 256, 8, GRAD>(a, st);
+    if (n <= 4096) return launch_row<T, 512, 8, GRAD>(a, st);
+    if (n <= 8192) return launch_row<T, 1024, 8, GRAD>(a, st);
+    if (n <= 16384) return launch_row<T, 1024, 16, GRAD>(a, st);
+    wide_kernel<T, GRAD><<<(unsigned)a.N, 1024, row_lds(a.K), st>>>(a);
+    SAMX_LAUNCH_CHECK();
+    return SAMX_OK;
+}
+
+int distill(const char* who, const void* logits, int64_t ld, int dtype, int64_t N, int64_t V, const int32_t* idx,
+            const float* teacher, int K, float tau, const float* lse, const float* weight, float scale, float* loss,
+            void* grad, int64_t ldg, hipStream_t st) {
+    SAMX_REQUIRE(N >= 0 && N < (int64_t(1) << 31) && V > 0 && V < (int64_t(1) << 31), "%s: N %lld, V %lld out of range", who, (long long)N,
+                 (long long)V);
+    SAMX_REQUIRE(K > 0 && K <= SAMX_DISTILL_MAX_K, "%s: K %d must be in [1, %d]", who, K, SAMX_DISTILL_MAX_K);
+    SAMX_REQUIRE(ld >= V && (!grad || ldg >= V), "%s: a row stride is shorter than V", who);
+    SAMX_REQUIRE(tau >= 1e-6f && tau <= 1e6f && isfinite(scale), "%s: tau must be in [1e-6, 1e6], scale finite", who);
+    SAMX_REQUIRE(dtype >= 0 && dtype <= 2, "%s: unknown element type %d", who, dtype);
+    SAMX_REQUIRE(!grad || grad != logits || ldg == ld, "%s: a gradient in place of the logits has their row stride", who);
+    if (N == 0) return SAMX_OK;
+    SAMX_REQUIRE(logits && idx && teacher && loss, "%s: null pointer", who);
+    const Args a{logits, ld, N, V, idx, teacher, K, 1.0 / (double)tau, lse, weight, (double)scale / (double)tau, loss, grad, ldg};
+    if (dtype == kF32) return grad ? launch<float, true>(a, st) : launch<float, false>(a, st);
+    if (dtype == kBF16) return grad ? launch<bf16, true>(a, st) : launch<bf16, false>(a, st);
+    return grad ? launch<f16, true>(a, st) : launch<f16, false>(a, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+int samx_distill_loss(const void* logits, int64_t ld, int dtype, int64_t N, int64_t V, const int32_t* idx,
+                      const float* teacher, int K, float tau, const float* lse, const float* weight, float* loss,
+                      void* stream) {
+    return distill("samx_distill_loss", logits, ld, dtype, N, V, idx, teacher, K, tau, lse, weight, 1.f, loss, nullptr,
+                   0, (hipStream_t)stream);
+}
+
+int samx_distill_grad(const void* logits, int64_t ld, int dtype, int64_t N, int64_t V, const int32_t* idx,
+                      const float* teacher, int K, float tau, const float* lse, const float* weight, float scale,
+                      float* loss, void* grad, int64_t ld_grad, void* stream) {
+    SAMX_REQUIRE(grad || N == 0, "samx_distill_grad: null pointer");
+    return distill("samx_distill_grad", logits, ld, dtype, N, V, idx, teacher, K, tau, lse, weight, scale, loss, grad,
+                   ld_grad, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -914,3 +914,156 @@ def gemm_f32(A, a_strides, B, b_strides, M, N, R, epi=0, bias=None, aux=None, ad
                              add.stride(0) if add is not None else 0, float(alpha), nsplit, ptr(partials),
                              int(bool(overread_ok)), stream_ptr()))
     return C_
+
+
+# ------------------------------------------------------------------ sequence policies
+
+SEQ_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # SAMX_F32, SAMX_BF16, SAMX_F16
+_NORM = {'rms': 0, 'layer': 1}
+
+
+def _seq_dtype(t, name):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise TypeError('%s must be a CUDA tensor' % name)
+    code = SEQ_DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError('%s must be float32, bfloat16 or float16, got %s' % (name, t.dtype))
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError('%s is on %s, the current device is cuda:%d' % (name, t.device, torch.cuda.current_device()))
+    return code
+
+
+def _on(t, like, dtype, shape, name):
+    """_chk, and on the device of `like`."""
+    _chk(t, dtype, shape, name)
+    if t.device != like.device:
+        raise ValueError('%s is on %s, expected %s' % (name, t.device, like.device))
+    return t
+
+
+def _opt_on(t, like, dtype, shape, name):
+    return None if t is None else _on(t, like, dtype, shape, name)
+
+
+def _apart(named):
+    """Outputs that are given have to be buffers of their own: no two of `named` overlap."""
+    at = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), n) for n, t in named
+                if t is not None and t.numel())
+    for (_, e, a), (b, _, c) in zip(at, at[1:]):
+        if b < e:
+            raise ValueError('%s and %s overlap' % (a, c))
+
+
+def _norm_args(y, gate, post_w, post_b, pre_w, pre_b, kind):
+    code = _seq_dtype(y, 'y')
+    if y.dim() != 2:
+        raise ValueError('y must be [rows, channels], got %s' % (tuple(y.shape),))
+    N, D = y.shape
+    if kind not in _NORM:
+        raise ValueError("kind must be 'rms' or 'layer', got %r" % (kind,))
+    _on(post_w, y, F32, (D,), 'post_w'); _on(pre_w, y, F32, (D,), 'pre_w')
+    if kind == 'layer':
+        _on(post_b, y, F32, (D,), 'post_b'); _on(pre_b, y, F32, (D,), 'pre_b')
+    elif post_b is not None or pre_b is not None:
+        raise ValueError("the RMS norm has no bias")
+    gate_kind = 0
+    if gate is not None:
+        gate_kind = 1 if gate.dim() == 1 else 2
+        _on(gate, y, F32 if gate_kind == 1 else y.dtype, (D,) if gate_kind == 1 else (N, D), 'gate')
+    return code, N, D, gate_kind
+
+
+def block_norm(x, y, post_w, pre_w, post_b=None, pre_b=None, gate=None, res_scale=1.0, kind='rms', eps=1e-8, h=None,
+               u=None):
+    """The norm behind a block, its gate, the scaled residual and the norm in front of the next block in one pass:
+    h = res_scale * x + gate * N(y; post_w, post_b), u = N(h; pre_w, pre_b).  x, y [rows, channels] in float32, bfloat16
+    or float16; weights and biases float32 [channels] (biases with kind 'layer' only); gate None, float32 [channels] or
+    like y.  Returns (h, u); they may be given, x's and y's own buffers among them (samx_block_norm)."""
+    code, N, D, gate_kind = _norm_args(y, gate, post_w, post_b, pre_w, pre_b, kind)
+    _on(x, y, y.dtype, (N, D), 'x')
+    h = torch.empty_like(y) if h is None else _on(h, y, y.dtype, (N, D), 'h')
+    u = torch.empty_like(y) if u is None else _on(u, y, y.dtype, (N, D), 'u')
+    _apart((('h', h), ('u', u)))
+    check(_L().samx_block_norm(ptr(x), ptr(y), code, N, D, ptr(post_w), ptr(post_b), gate_kind, ptr(gate), ptr(pre_w),
+                               ptr(pre_b), float(res_scale), _NORM[kind], float(eps), ptr(h), ptr(u), stream_ptr()))
+    return h, u
+
+
+def block_norm_grad(y, h, dh, du, post_w, pre_w, post_b=None, pre_b=None, gate=None, res_scale=1.0, kind='rms',
+                    eps=1e-8, ws=None):
+    """The gradient of block_norm from dh (the gradient of h by the residual path) and du (of u); y as it went in, h as it
+    came out.  Returns a dict: x, y, gate (None without one), post_w, post_b, pre_w, pre_b (biases None with 'rms')
+    (samx_block_norm_grad)."""
+    code, N, D, gate_kind = _norm_args(y, gate, post_w, post_b, pre_w, pre_b, kind)
+    for t, n in ((h, 'h'), (dh, 'dh'), (du, 'du')):
+        _on(t, y, y.dtype, (N, D), n)
+    L = _L()
+    nb = int(L.samx_block_norm_grad_ws_bytes(code, N, D))
+    if ws is None:
+        ws = torch.empty(max(nb, 1), dtype=torch.uint8, device=y.device)
+    _on(ws, y, torch.uint8, (ws.numel(),), 'ws')
+    layer = kind == 'layer'
+    sums = torch.empty((2 + 2 * layer + (gate_kind == 1), D), dtype=F32, device=y.device)
+    out = dict(x=torch.empty_like(y), y=torch.empty_like(y), gate=None, post_w=sums[0], post_b=None, pre_w=sums[1],
+               pre_b=None)
+    if layer:
+        out['post_b'], out['pre_b'] = sums[2], sums[3]
+    if gate_kind:
+        out['gate'] = sums[-1] if gate_kind == 1 else torch.empty_like(y)
+    check(L.samx_block_norm_grad(
+        ptr(y), ptr(h), ptr(dh), ptr(du), code, N, D, ptr(post_w), ptr(post_b), gate_kind, ptr(gate), ptr(pre_w),
+        float(res_scale), _NORM[kind], float(eps), ptr(out['x']), ptr(out['y']), ptr(out['gate']), ptr(out['post_w']),
+        ptr(out['post_b']), ptr(out['pre_w']), ptr(out['pre_b']), ptr(ws), ws.numel(), stream_ptr()))
+    return out
+
+
+def _rows2(t, name):
+    """[rows, columns] with dense columns -> row stride in elements."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError('%s must be [rows, columns] with dense rows' % name)
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _distill_args(logits, idx, teacher, lse, weight, loss):
+    code = _seq_dtype(logits, 'logits')
+    ld = _rows2(logits, 'logits')
+    N, V = logits.shape
+    if not (isinstance(idx, torch.Tensor) and idx.dim() == 2):
+        raise ValueError('idx must be [rows, K]')
+    K = idx.shape[1]
+    _on(idx, logits, I32, (N, K), 'idx'); _on(teacher, logits, F32, (N, K), 'teacher')
+    _opt_on(lse, logits, F32, (N,), 'lse'); _opt_on(weight, logits, F32, (N,), 'weight')
+    loss = torch.empty(N, dtype=F32, device=logits.device) if loss is None else _on(loss, logits, F32, (N,), 'loss')
+    return code, ld, N, V, K, loss
+
+
+def distill_loss(logits, idx, teacher, tau=1.0, lse=None, weight=None, loss=None):
+    """Imitation of a teacher's top logits: loss float32 [rows], weight * sum_k p_k (log p_k - log softmax(logits /
+    tau)[idx_k]) with p_k = exp(teacher_k / tau - lse) (lse None: normalised over the K entries).  logits [rows, V] in
+    float32, bfloat16 or float16, rows may be apart; idx int32 [rows, K] (entries outside [0, V) do not count), teacher
+    float32 [rows, K]; lse, weight float32 [rows] (samx_distill_loss)."""
+    code, ld, N, V, K, loss = _distill_args(logits, idx, teacher, lse, weight, loss)
+    check(_L().samx_distill_loss(C.c_void_p(logits.data_ptr()), ld, code, N, V, ptr(idx), ptr(teacher), K, float(tau),
+                                 ptr(lse), ptr(weight), ptr(loss), stream_ptr()))
+    return loss
+
+
+def distill_grad(logits, idx, teacher, tau=1.0, lse=None, weight=None, scale=1.0, loss=None, grad=None):
+    """distill_loss and the gradient of scale * its sum: (loss, grad).  grad has the logits' type and shape (and a row
+    stride up to 255 columns wider than V); it may be given, the logits themselves among them; columns behind V stay as
+    they were (samx_distill_grad)."""
+    code, ld, N, V, K, loss = _distill_args(logits, idx, teacher, lse, weight, loss)
+    if grad is None:
+        grad = torch.empty((N, ld if V <= ld < V + 256 else V), dtype=logits.dtype, device=logits.device)[:, :V]
+    elif grad.dtype != logits.dtype or grad.shape != logits.shape or grad.device != logits.device:
+        raise ValueError('grad must be like logits: %s %s on %s' % (logits.dtype, tuple(logits.shape), logits.device))
+    ldg = _rows2(grad, 'grad')
+    if grad.data_ptr() != logits.data_ptr() and N:
+        a, b = logits.data_ptr(), grad.data_ptr()
+        e = logits.element_size()
+        if a < b + ((N - 1) * ldg + V) * e and b < a + ((N - 1) * ld + V) * e:
+            raise ValueError('grad overlaps the logits without being them')
+    check(_L().samx_distill_grad(C.c_void_p(logits.data_ptr()), ld, code, N, V, ptr(idx), ptr(teacher), K, float(tau),
+                                 ptr(lse), ptr(weight), float(scale), ptr(loss), C.c_void_p(grad.data_ptr()), ldg,
+                                 stream_ptr()))
+    return loss, grad
