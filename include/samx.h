@@ -666,6 +666,36 @@ int samx_block_norm_grad(const void* y, const void* h, const void* dh, const voi
                          float res_scale, int kind, float eps, void* dx, void* dy, void* dgate, float* dpost_w,
                          float* dpost_b, float* dpre_w, float* dpre_b, void* ws, size_t ws_bytes, void* stream);
 
+/* Linear attention with a decay for each head, over B sequences of T rows with H query heads of D and HK key heads (H a
+ * multiple of HK: the query heads h of key head h / (H / HK)) of D, their values of DV; D, DV at most 128, B * H at most 65535:
+ *   S_t = e^{decay_h} S_{t-1} + k_t v_t^T ;  out_t = scale q_t^T S_t
+ * q [B, T, H, D], k [B, T, HK, D], v [B, T, HK, DV], dout [B, T, H, DV] of the element type, dense in the last dimension, other
+ * strides (in elements: batch, row, head) as given; decay float32 [H], the logarithm of the factor (<= 0, -inf: no memory);
+ * state float32 [B, H, D, DV] dense, state_in NULL: zero.  lengths int32 [B] (NULL: T): rows of each sequence that are there
+ * (taken into [0, T]); rows behind them are not read, their outputs are zeros, the state behind a sequence is that of its
+ * last row.  out, dq, dk, dv are dense.  Scores and the state are float32; products of 16-bit types take the scores and, for
+ * out, the state in their own type (of float16, both have to be within its range).  A row's inputs have to be finite for the
+ * outputs of the 63 rows before it to be. */
+typedef struct samx_linattn_shape {
+    int32_t dtype, H, HK, D, DV, pad;
+    int64_t B, T;
+    int64_t q[3], k[3], v[3], o[3];
+} samx_linattn_shape;
+size_t samx_linattn_ws_bytes(const samx_linattn_shape* s);
+int samx_linattn(const samx_linattn_shape* s, const void* q, const void* k, const void* v, const float* decay,
+                 float scale, const float* state_in, const int32_t* lengths, void* out, float* state_out, void* ws,
+                 size_t ws_bytes, void* stream);
+/* Its gradient, from dout and dstate (of the state behind the sequence, NULL: zero), decay taken as a constant: dq, dk, dv
+ * (sums over the query heads of a key head, in a fixed order) and dstate_in, the gradient of the state before the first row. */
+size_t samx_linattn_grad_ws_bytes(const samx_linattn_shape* s);
+int samx_linattn_grad(const samx_linattn_shape* s, const void* q, const void* k, const void* v, const float* decay,
+                      const void* dout, float scale, const float* state_in, const float* dstate, const int32_t* lengths,
+                      void* dq, void* dk, void* dv, float* dstate_in, void* ws, size_t ws_bytes, void* stream);
+/* One row of each of B sequences, in float32 throughout: the state is updated in place.  T and the row strides of the shape
+ * are not used. */
+int samx_linattn_step(const samx_linattn_shape* s, const void* q, const void* k, const void* v, const float* decay,
+                      float scale, float* state, void* out, void* stream);
+
 /* Imitation of a teacher's top logits: for each of N rows of V student logits z (rows ld apart) and the K entries
  * (idx int32 [N, K], teacher float32 [N, K]) that are known of the teacher's row,
  *   p_k = e^{t_k / tau - lse}   (lse float32 [N]: the teacher's own log-normaliser at tau; NULL: over the K entries)

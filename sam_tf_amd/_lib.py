@@ -62,6 +62,13 @@ class RetNorm(C.Structure):
     _fields_ = [('mean', C.c_void_p), ('std', C.c_void_p)]
 
 
+class LinattnShape(C.Structure):
+    """Mirror of `struct samx_linattn_shape`."""
+    _fields_ = ([(k, C.c_int32) for k in ('dtype', 'H', 'HK', 'D', 'DV', 'pad')] +
+                [('B', C.c_int64), ('T', C.c_int64)] + [(k, C.c_int64 * 3) for k in ('q', 'k', 'v', 'o')])
+
+
+_SP = C.POINTER(LinattnShape)
 _LP, _BP, _OP, _RP = C.POINTER(Learner), C.POINTER(Batch), C.POINTER(StepOut), C.POINTER(RetNorm)
 
 # name -> (restype, argtypes); must list every symbol include/samx.h declares
@@ -153,6 +160,11 @@ SIGNATURES = {
     'samx_block_norm_grad_ws_bytes': (_SZ, [C.c_int, _I64, _I64]),
     'samx_block_norm_grad': (C.c_int, [_P, _P, _P, _P, C.c_int, _I64, _I64, _P, _P, C.c_int, _P, _P, _F, C.c_int, _F,
                                        _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    'samx_linattn_ws_bytes': (_SZ, [_SP]),
+    'samx_linattn': (C.c_int, [_SP, _P, _P, _P, _P, _F, _P, _P, _P, _P, _P, _SZ, _P]),
+    'samx_linattn_grad_ws_bytes': (_SZ, [_SP]),
+    'samx_linattn_grad': (C.c_int, [_SP, _P, _P, _P, _P, _P, _F, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    'samx_linattn_step': (C.c_int, [_SP, _P, _P, _P, _P, _F, _P, _P, _P]),
     'samx_distill_loss': (C.c_int, [_P, _I64, C.c_int, _I64, _I64, _P, _P, C.c_int, _F, _P, _P, _P, _P]),
     'samx_distill_grad': (C.c_int, [_P, _I64, C.c_int, _I64, _I64, _P, _P, C.c_int, _F, _P, _P, _F, _P, _P, _I64, _P]),
 }

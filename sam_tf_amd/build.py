@@ -11,7 +11,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 SO = os.path.join(HERE, 'libsamx.so')
 SOURCES = ['core.hip', 'host_pow.hip', 'tree.hip', 'replay.hip', 'optim.hip', 'gemm.hip', 'nets.hip',
-           'fused_small.hip', 'fused_ln.hip', 'fused_wide.hip', 'step.hip', 'block_norm.hip', 'distill.hip']
+           'fused_small.hip', 'fused_ln.hip', 'fused_wide.hip', 'step.hip', 'block_norm.hip', 'distill.hip',
+           'linattn.hip']
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-ffp-contract=off',
          '-fno-fast-math', '-Wall', '-Wno-unused-function',
          # no packed float32 arithmetic: some of its forms have given wrong results on this hardware now and then

@@ -1,0 +1,698 @@
+// Linear attention with a decay for each head.  For a head with decay factor l = e^g:
+//
+//   S_t = l S_{t-1} + k_t v_t^T ;  o_t = c q_t^T S_t          (S: [D, Dv], S_{-1} the caller's state or zero)
+//
+// and backward, with G_t the gradient of S_t (G behind the last row: the caller's, without the factor l):
+//
+//   G_t = l G_{t+1} + c q_t do_t^T ;  dq_t = c S_t do_t ;  dk_t = G_t v_t ;  dv_t = G_t^T k_t ;  dS_{-1} = l G_0
+//
+// All four are one recurrence over positions p (rows forwards, or from the last one backwards),
+//
+//   out_p = ps sum_{s <= p} l^{p-s} (a_p . b_s) c_s + l^p so a_p^T X_0 ,
+//
+// with (a, b, c) = (q, k, v), (do, v, k), backwards (k, q, do) and (v, do, q).  X_p is the state a row at p finds,
+// already decayed to it: X_{p+1} = l (X_p + kv b_p c_p^T).
+//
+// A chunk of 64 positions at a time, on the matrix cores: scores P = a b^T masked with l^{p-s}, out = P c + l^p a X,
+// X <- l^64 X + sum_s l^{64-s} b_s c_s^T.  X stays in the registers of the workgroup (float32; each wave owns whole
+// columns).  Operands of 16 bits enter the matrix cores as they are; P and the copy of X that meets a are rounded to
+// their type (an output of that type is rounded again), but l^{64-s} c_s is split into two numbers of the type, so that
+// the state, a float32 output, keeps 16 bits more than the type has.  float32 operands use the float32 matrix
+// instructions throughout.
+//
+// Where batch times heads is less than the device holds, time is cut into segments: kv_kernel makes each segment's own
+// contribution to the state behind it, join_kernel runs the recurrence over the segments, mix_kernel does the rest with
+// a known state at each segment's start.
+#include "seq_dev.h"
+#include "../../include/samx.h"
+
+namespace {
+
+using namespace samx::seq;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kChunk = 64, kThreads = 256, kMaxDim = 128;
+
+// D += A B^T for 16 rows each and the kN * 4 inner values that 64 lanes' pieces hold: lane l has row l % 16, inner values
+// (l / 16) * kN + [0, kN).  D: lane l has column l % 16 (B's row), rows (l / 16) * 4 + [0, 4).
+__device__ __forceinline__ f32x4 mma(const Piece<bf16>& a, const Piece<bf16>& b, f32x4 d) {
+    bf16x8 x, y;
+    __builtin_memcpy(&x, &a, 16);
+    __builtin_memcpy(&y, &b, 16);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, d, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(const Piece<f16>& a, const Piece<f16>& b, f32x4 d) {
+    f16x8 x, y;
+    __builtin_memcpy(&x, &a, 16);
+    __builtin_memcpy(&y, &b, 16);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, d, 0, 0, 0);
+}
+// (four instructions of 4 inner values: each takes the j-th of every lane, an order of the inner values that A and B share)
+__device__ __forceinline__ f32x4 mma(const Piece<float>& a, const Piece<float>& b, f32x4 d) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) d = __builtin_amdgcn_mfma_f32_16x16x4f32(a.e[j], b.e[j], d, 0, 0, 0);
+    return d;
+}
+
+// [B, T, heads, dim], element strides; grp: query heads that share one of its heads
+struct Mat { const void* p; int64_t sb, st, sh; int grp, dim; };
+
+struct Role {
+    Mat a, b, c;
+    void* out; int out_f32;                    // [B, T, H, c.dim] dense, of the type or float32
+    int rev;
+    float kv, ps, so;                          // factors: of b c^T in the state, of the scores, of a X
+    const float* s_in; int64_t in_a, in_c;     // state before the first position, strides of a state's element (a, c)
+    float* s_out;                              // state behind the last, strides as s_in's
+    float* seg; int64_t seg_a, seg_c;          // states at the segments' starts (workspace)
+};
+
+struct Args {
+    Role r[3];
+    int roles, H, B;
+    int64_t T, seg_len;
+    int nseg;
+    int64_t seg_size;                          // floats of a segment's state
+    const float* decay;
+    const int32_t* lengths;
+};
+
+__device__ __forceinline__ float power(float g, int64_t n) { return n == 0 ? 1.f : expf(g * (float)n); }
+
+// where a workgroup works
+struct Place { int role, b, h, seg; int64_t L; float g; };
+
+// 8 workgroups that follow each other run on 8 dies: the roles of one (batch, head, segment) go to the same one
+__device__ __forceinline__ bool place_of(const Args& a, int nseg, Place& p) {
+    const int64_t units = (int64_t)a.B * a.H * nseg, id = blockIdx.x;
+    const int64_t x = id & 7, k = id >> 3, unit = k / a.roles * 8 + x;
+    p.role = (int)(k % a.roles);
+    if (unit >= units) return false;
+    p.seg = (int)(unit % nseg);
+    const int64_t bh = unit / nseg;
+    p.h = (int)(bh % a.H);
+    p.b = (int)(bh / a.H);
+    p.L = a.T;
+    if (a.lengths) {
+        const int64_t n = a.lengths[p.b];
+        p.L = n < 0 ? 0 : n < a.T ? n : a.T;
+    }
+    p.g = a.decay[p.h];
+    return true;
+}
+inline unsigned grid_of(const Args& a, int nseg) {
+    const int64_t units = (int64_t)a.B * a.H * nseg;
+    return (unsigned)((units + 7) / 8 * 8 * a.roles);
+}
+
+// row 0 of a matrix of this place in the order of positions, and the step from one position to the next
+template <typename T>
+struct Rows {
+    const T* p; int64_t step; int dim;
+    __device__ Rows(const Mat& m, const Place& q, int rev) : dim(m.dim) {
+        p = (const T*)m.p + q.b * m.sb + (int64_t)(q.h / m.grp) * m.sh + (rev ? (q.L - 1) * m.st : 0);
+        step = rev ? -m.st : m.st;
+    }
+    // elements [at, at + kN) of position `pos`; zeros behind the row's end and where there is no such position
+    __device__ __forceinline__ Piece<T> piece(int64_t pos, int at, bool there) const {
+        return load_piece(p + (there ? pos * step : 0), (int64_t)at, there ? dim : 0, from_float<T>(0.f));
+    }
+};
+
+// 16 bytes, and 4 values, of LDS: every row and every column that comes here is a multiple of them
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <typename T>
+__device__ __forceinline__ Piece<T> lds_piece(const T* p) {
+    const u32x4 v = *reinterpret_cast<const u32x4*>(p);
+    Piece<T> r;
+    __builtin_memcpy(&r, &v, 16);
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void lds_put(T* p, const Piece<T>& r) {
+    u32x4 v;
+    __builtin_memcpy(&v, &r, 16);
+    *reinterpret_cast<u32x4*>(p) = v;
+}
+__device__ __forceinline__ void lds_put4(float* p, const float (&v)[4]) { *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]}; }
+template <typename T>
+__device__ __forceinline__ void lds_put4(T* p, const float (&v)[4]) {
+    struct { T e[4]; } o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o.e[e] = from_float<T>(v[e]);
+    uint64_t u;
+    __builtin_memcpy(&u, &o, 8);
+    *reinterpret_cast<uint64_t*>(p) = u;
+}
+// what the lanes of a wave have written to LDS is there for the others of the wave
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// LDS rows are 16 bytes longer than their contents: 16 lanes that read 16 rows at one column use all banks
+template <typename T, int DP>
+struct Lds {
+    static constexpr int kN = Piece<T>::kN, kTok = kChunk + kN, kRow = DP + kN;
+    T bt[DP][kTok];          // b, c of the chunk, a row for each of their dimensions
+    T ct[DP][kTok];
+    T p[4][16][kTok];        // each wave's 16 rows of scores
+    T x[DP][kRow];           // X, a row for each column
+    float lam[kChunk + 1];   // l^n
+};
+template <typename T, int DP>
+struct LdsKv {
+    static constexpr int kN = Piece<T>::kN, kTok = kChunk + kN;
+    T bt[DP][kTok];
+    T ct[DP][kTok];
+    float lam[kChunk + 1];
+};
+
+// A chunk's rows of b and c on their way to LDS: blocks of kN positions by kN dimensions, transposed in registers
+template <typename T, int DP>
+struct Staged {
+    static constexpr int kN = Piece<T>::kN, kTb = kChunk / kN, kBlocks = kTb * (DP / kN);   // blocks of one matrix
+    static constexpr int kPer = (2 * kBlocks + kThreads - 1) / kThreads;
+    static constexpr bool kEven = 2 * kBlocks % kThreads == 0;
+    Piece<T> r[kPer][kN];
+    __device__ __forceinline__ void load(const Rows<T>& b, const Rows<T>& c, int64_t base, int n) {
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) {
+            const int id = threadIdx.x + u * kThreads;
+            const bool second = id >= kBlocks;
+            if (!kEven && id >= 2 * kBlocks) continue;
+            const int k = second ? id - kBlocks : id, t0 = k % kTb * kN, d0 = k / kTb * kN;
+            const Rows<T>& m = second ? c : b;
+#pragma unroll
+            for (int i = 0; i < kN; ++i) r[u][i] = m.piece(base + t0 + i, d0, t0 + i < n);
+        }
+    }
+    template <typename L>
+    __device__ __forceinline__ void store(L& l) const {
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) {
+            const int id = threadIdx.x + u * kThreads;
+            const bool second = id >= kBlocks;
+            if (!kEven && id >= 2 * kBlocks) continue;
+            const int k = second ? id - kBlocks : id, t0 = k % kTb * kN, d0 = k / kTb * kN;
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+                Piece<T> o;
+#pragma unroll
+                for (int i = 0; i < kN; ++i) o.e[i] = r[u][i].e[j];
+                lds_put(second ? &l.ct[d0 + j][t0] : &l.bt[d0 + j][t0], o);
+            }
+        }
+    }
+};
+
+// X of a workgroup: wave w owns the tiles of 16 columns w, w + 4, ...; tile (i, j): lane l has column l % 16, rows
+// (l / 16) * 4 + [0, 4) of the a side
+template <int DP> struct State { static constexpr int kJ = DP / 64, kI = DP / 16; f32x4 x[kJ][kI]; };
+
+// X <- l^end X + kv sum_s l^{end - s} b_s c_s^T
+template <typename T, int DP, typename L>
+__device__ __forceinline__ void update(State<DP>& S, const L& l, int end, float kv, int na, int nc) {
+    constexpr int kN = Piece<T>::kN;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
+    const float whole = l.lam[end];
+#pragma unroll
+    for (int j = 0; j < State<DP>::kJ; ++j) {
+        if (w + 4 * j >= nc) continue;
+#pragma unroll
+        for (int i = 0; i < State<DP>::kI; ++i) S.x[j][i] *= whole;
+#pragma unroll
+        for (int k = 0; k < kChunk; k += 4 * kN) {
+            const int s0 = k + q * kN;
+            const Piece<T> c = lds_piece(&l.ct[(w + 4 * j) * 16 + r16][s0]);
+            Piece<T> hi, lo;
+#pragma unroll
+            for (int e = 0; e < kN; ++e) {
+                const int n = end - s0 - e;
+                const float v = to_float(c.e[e]) * (kv * l.lam[n < 0 ? 0 : n]);   // (rows behind the end are zeros)
+                hi.e[e] = from_float<T>(v);
+                if constexpr (sizeof(T) == 2) lo.e[e] = from_float<T>(v - to_float(hi.e[e]));
+            }
+#pragma unroll
+            for (int i = 0; i < State<DP>::kI; ++i) {
+                if (i >= na) continue;
+                const Piece<T> b = lds_piece(&l.bt[i * 16 + r16][s0]);
+                S.x[j][i] = mma(b, hi, S.x[j][i]);
+                if constexpr (sizeof(T) == 2) S.x[j][i] = mma(b, lo, S.x[j][i]);
+            }
+        }
+    }
+}
+
+// a state's elements that exist: X(a, c) <- f(a, c, X(a, c))
+template <int DP, typename F>
+__device__ __forceinline__ void each(State<DP>& S, int da, int dc, F f) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < State<DP>::kJ; ++j)
+#pragma unroll
+        for (int i = 0; i < State<DP>::kI; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int c = (w + 4 * j) * 16 + r16, a = i * 16 + q * 4 + e;
+                if (a < da && c < dc) S.x[j][i][e] = f(a, c, S.x[j][i][e]);
+            }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads) void kv_kernel(Args A) {
+    extern __shared__ __attribute__((aligned(16))) char lds_[];
+    LdsKv<T, DP>& l = *reinterpret_cast<LdsKv<T, DP>*>(lds_);
+    Place p;
+    if (!place_of(A, A.nseg - 1, p)) return;
+    const int64_t at = (int64_t)p.seg * A.seg_len;
+    if (p.L <= at + A.seg_len) return;                  // nobody follows
+    const Role& r = A.r[p.role];
+    const Rows<T> b(r.b, p, r.rev), c(r.c, p, r.rev);
+    const int na = (r.b.dim + 15) / 16, nc = (r.c.dim + 15) / 16;
+    if (threadIdx.x <= kChunk) l.lam[threadIdx.x] = power(p.g, threadIdx.x);
+    State<DP> S;
+#pragma unroll
+    for (int j = 0; j < State<DP>::kJ; ++j)
+#pragma unroll
+        for (int i = 0; i < State<DP>::kI; ++i) S.x[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    Staged<T, DP> st;
+    st.load(b, c, at, kChunk);
+    for (int64_t k = 0; k < A.seg_len; k += kChunk) {
+        __syncthreads();
+        st.store(l);
+        __syncthreads();
+        if (k + kChunk < A.seg_len) st.load(b, c, at + k + kChunk, kChunk);
+        update<T, DP>(S, l, kChunk, r.kv, na, nc);
+    }
+    float* out = r.seg + ((int64_t)(p.b * A.H + p.h) * (A.nseg - 1) + p.seg) * A.seg_size;
+    each<DP>(S, r.b.dim, r.c.dim, [&](int i, int j, float v) { return out[i * r.seg_a + j * r.seg_c] = v; });
+}
+
+// states at the segments' starts: X_{j+1} = l^len X_j + (segment j's own), over the segments that have a follower
+__global__ __launch_bounds__(256) void join_kernel(Args A, int states) {
+    const Role& r = A.r[blockIdx.z];
+    const int64_t bh = blockIdx.y;
+    const int e = blockIdx.x * 256 + threadIdx.x, na = r.b.dim, nc = r.c.dim;
+    if (e >= na * nc) return;
+    const int b = (int)(bh / A.H), h = (int)(bh % A.H);
+    int64_t L = A.T;
+    if (A.lengths) L = A.lengths[b] < A.T ? A.lengths[b] : A.T;
+    // the fast index is the one that lies dense in the workspace
+    const int i = e % na, j = e / na;
+    const float g = A.decay[h], f = power(g, A.seg_len);
+    float x = 0.f;
+    if (r.s_in) x = r.s_in[bh * na * nc + i * r.in_a + j * r.in_c] * (r.rev ? 1.f : power(g, 1));
+    float* s = r.seg + bh * states * A.seg_size + i * r.seg_a + j * r.seg_c;
+    for (int k = 0; k < states && (int64_t)(k + 1) * A.seg_len < L; ++k) {
+        x = f * x + s[k * A.seg_size];
+        s[k * A.seg_size] = x;
+    }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads) void mix_kernel(Args A) {
+    constexpr int kN = Piece<T>::kN, kInner = 4 * kN;      // inner values of one mma
+    extern __shared__ __attribute__((aligned(16))) char lds_[];
+    Lds<T, DP>& l = *reinterpret_cast<Lds<T, DP>*>(lds_);
+    Place p;
+    if (!place_of(A, A.nseg, p)) return;
+    const Role& r = A.r[p.role];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
+    const int64_t at = (int64_t)p.seg * A.seg_len, bh = (int64_t)p.b * A.H + p.h;
+    const int64_t to = at + A.seg_len < p.L ? at + A.seg_len : p.L;         // this segment's positions
+    const int da = r.a.dim, dc = r.c.dim, na = (da + 15) / 16, nc = (dc + 15) / 16;
+    const int64_t out_row = (int64_t)A.H * dc;
+    T* out_t = (T*)r.out + ((int64_t)p.b * A.T * A.H + p.h) * dc;
+    float* out_f = (float*)r.out + ((int64_t)p.b * A.T * A.H + p.h) * dc;
+    {   // rows behind the trajectory's end
+        const int64_t z0 = at > p.L ? at : p.L, z1 = at + A.seg_len < A.T ? at + A.seg_len : A.T;
+        for (int64_t t = z0 + threadIdx.x / 64; t < z1; t += 4)
+            for (int d = lane; d < dc; d += 64) {
+                if (r.out_f32) out_f[t * out_row + d] = 0.f;
+                else out_t[t * out_row + d] = from_float<T>(0.f);
+            }
+    }
+    State<DP> S;
+#pragma unroll
+    for (int j = 0; j < State<DP>::kJ; ++j)
+#pragma unroll
+        for (int i = 0; i < State<DP>::kI; ++i) S.x[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const float* s_in = r.s_in ? r.s_in + bh * da * dc : nullptr;
+    float* s_out = r.s_out ? r.s_out + bh * da * dc : nullptr;
+    if (p.L == 0) {    // nothing to read: the state goes through
+        if (p.seg == 0 && s_out)
+            each<DP>(S, da, dc, [&](int i, int j, float) { return s_out[i * r.in_a + j * r.in_c] = s_in ? s_in[i * r.in_a + j * r.in_c] : 0.f; });
+        return;
+    }
+    if (at >= to) return;
+    const bool last = to == p.L;           // this segment makes the state behind the last position
+    bool have = false;                     // X is not zero
+    if (p.seg > 0) {
+        const float* s = r.seg + (bh * (A.nseg - 1) + p.seg - 1) * A.seg_size;
+        each<DP>(S, da, dc, [&](int i, int j, float) { return s[i * r.seg_a + j * r.seg_c]; });
+        have = true;
+    } else if (s_in) {
+        const float f = r.rev ? 1.f : power(p.g, 1);
+        each<DP>(S, da, dc, [&](int i, int j, float) { return s_in[i * r.in_a + j * r.in_c] * f; });
+        have = true;
+    }
+    const Rows<T> a(r.a, p, r.rev), b(r.b, p, r.rev), c(r.c, p, r.rev);
+    if (threadIdx.x <= kChunk) l.lam[threadIdx.x] = power(p.g, threadIdx.x);
+    auto keep = [&]() {                    // X's copy for the products with a
+#pragma unroll
+        for (int j = 0; j < State<DP>::kJ; ++j)
+#pragma unroll
+            for (int i = 0; i < State<DP>::kI; ++i) {
+                const float v[4] = {S.x[j][i][0], S.x[j][i][1], S.x[j][i][2], S.x[j][i][3]};
+                lds_put4(&l.x[(w + 4 * j) * 16 + r16][i * 16 + q * 4], v);
+            }
+    };
+    if (have) keep();
+    Staged<T, DP> st;
+    st.load(b, c, at, (int)(to - at < kChunk ? to - at : kChunk));
+    for (int64_t base = at; base < to; base += kChunk) {
+        const int n = (int)(to - base < kChunk ? to - base : kChunk);
+        const bool more = base + kChunk < to;
+        __syncthreads();                   // the chunk before is done with
+        st.store(l);
+        // a's rows of this wave, whole
+        const int row = w * 16 + r16;
+        Piece<T> af[DP / kInner];
+#pragma unroll
+        for (int k = 0; k < DP / kInner; ++k)
+            if (k * kInner < da) af[k] = a.piece(base + row, k * kInner + q * kN, row < n);
+        // scores, transposed: column = this wave's row, rows = positions s
+        f32x4 sc[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (t > w) continue;
+            const int s = t * 16 + r16;
+#pragma unroll
+            for (int k = 0; k < DP / kInner; ++k)
+                if (k * kInner < da) sc[t] = mma(b.piece(base + s, k * kInner + q * kN, s < n), af[k], sc[t]);
+        }
+        __syncthreads();                   // bt, ct, lam and X's copy are there
+        if (more) st.load(b, c, base + kChunk, (int)(to - base - kChunk < kChunk ? to - base - kChunk : kChunk));
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int d = row - (t * 16 + q * 4 + e);
+                v[e] = d >= 0 ? r.ps * l.lam[d] * sc[t][e] : 0.f;
+            }
+            lds_put4(&l.p[w][r16][t * 16 + q * 4], v);
+        }
+        wave_sync();
+        // out, transposed: column = this wave's row, rows = columns of c
+        const float decayed = r.so * l.lam[row];
+#pragma unroll
+        for (int j = 0; j < DP / 16; ++j) {
+            if (j >= nc) continue;
+            f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (have) {
+#pragma unroll
+                for (int k = 0; k < DP / kInner; ++k)
+                    if (k * kInner < da) o = mma(lds_piece(&l.x[j * 16 + r16][k * kInner + q * kN]), af[k], o);
+                o *= decayed;
+            }
+#pragma unroll
+            for (int k = 0; k < kChunk; k += kInner)
+                if (k <= w * 16 + 15) o = mma(lds_piece(&l.ct[j * 16 + r16][k + q * kN]), lds_piece(&l.p[w][r16][k + q * kN]), o);
+            if (row < n) {
+                const int64_t tok = r.rev ? p.L - 1 - (base + row) : base + row;
+                const int d = j * 16 + q * 4;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (d + e < dc) {
+                        if (r.out_f32) out_f[tok * out_row + d + e] = o[e];
+                        else out_t[tok * out_row + d + e] = from_float<T>(o[e]);
+                    }
+            }
+        }
+        if (more || (last && s_out)) {
+            // behind the last row the state of the forward recurrence has not been decayed once more
+            update<T, DP>(S, l, more ? kChunk : r.rev ? n : n - 1, r.kv, na, nc);
+            have = true;
+            if (more) {
+                __syncthreads();           // everybody has read X's copy
+                keep();
+            }
+        }
+    }
+    if (last && s_out) each<DP>(S, da, dc, [&](int i, int j, float v) { return s_out[i * r.in_a + j * r.in_c] = v; });
+}
+
+// sums of the query heads that share a key head: float32 [rows, HK, grp, dim] -> [rows, HK, dim] of the type
+template <typename T>
+__global__ __launch_bounds__(256) void group_kernel(const float* __restrict__ in, T* __restrict__ out, int64_t n, int grp, int dim) {
+    const int64_t e = blockIdx.x * (int64_t)256 + threadIdx.x;
+    if (e >= n) return;
+    const int64_t row = e / dim, d = e % dim;
+    const float* p = in + row * grp * dim + d;
+    float v = 0.f;
+    for (int k = 0; k < grp; ++k) v += p[(int64_t)k * dim];
+    out[e] = from_float<T>(v);
+}
+
+// One row: S <- l S + k v^T, out = c q^T S, in place.  A workgroup has C columns of a state (16 bytes for each of C / 4
+// lanes); its other lanes take the rows by turns.
+template <typename T>
+__global__ __launch_bounds__(256) void step_kernel(Mat Q, Mat K, Mat V, const float* __restrict__ decay, float* __restrict__ state,
+                                                   T* __restrict__ out, int H, int D, int DV, float scale, int cols, int per_head) {
+    __shared__ float sq[kMaxDim], sk[kMaxDim];
+    __shared__ float part[256 * 4];
+    const int64_t unit = blockIdx.x / per_head;
+    const int h = (int)(unit % H), c0 = (int)(blockIdx.x % per_head) * cols;
+    const int64_t b = unit / H;
+    const T* q = (const T*)Q.p + b * Q.sb + h * Q.sh;
+    const T* k = (const T*)K.p + b * K.sb + (int64_t)(h / K.grp) * K.sh;
+    const T* v = (const T*)V.p + b * V.sb + (int64_t)(h / V.grp) * V.sh;
+    for (int i = threadIdx.x; i < D; i += 256) { sq[i] = to_float(q[i]); sk[i] = to_float(k[i]); }
+    const int lanes = cols / 4, c = c0 + threadIdx.x % lanes * 4, rows = 256 / lanes;
+    float ve[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ve[e] = c + e < DV ? to_float(v[c + e]) : 0.f;
+    const float l = power(decay[h], 1);
+    float* s = state + unit * D * DV;
+    __syncthreads();
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = threadIdx.x / lanes; i < D; i += rows) {
+        Piece<float> x = load_piece(s + (int64_t)i * DV, (int64_t)c, (int64_t)DV, 0.f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x.e[e] = l * x.e[e] + sk[i] * ve[e];
+            acc[e] += sq[i] * x.e[e];
+        }
+        store_piece(s + (int64_t)i * DV, (int64_t)c, (int64_t)DV, x);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[threadIdx.x * 4 + e] = acc[e];
+    __syncthreads();
+    const int col = threadIdx.x;
+    if (col < cols && c0 + col < DV) {
+        float o = 0.f;
+        for (int i = 0; i < rows; ++i) o += part[i * cols + col];
+        out[(b * H + h) * DV + c0 + col] = from_float<T>(o * scale);
+    }
+}
+
+// ---------------------------------------------------------------- host
+
+// Workgroups that a device keeps busy: two for each of its units.
+int segments(int64_t B, int H, int roles, int64_t T) {
+    const int64_t units = B * H * roles, want = 2 * (int64_t)cu_count();
+    int64_t n = (want + units - 1) / (units > 0 ? units : 1);
+    const int64_t most = T / 256;          // four chunks at least
+    n = n < most ? n : most;
+    return (int)(n < 1 ? 1 : n);
+}
+int64_t seg_len_of(int64_t T, int nseg) {
+    const int64_t s = (T + nseg - 1) / nseg;
+    return (s + kChunk - 1) / kChunk * kChunk;
+}
+void cut(Args& a) {
+    a.nseg = segments(a.B, a.H, a.roles, a.T);
+    a.seg_len = seg_len_of(a.T, a.nseg);
+    if (a.seg_len < kChunk) a.seg_len = kChunk;
+    a.nseg = (int)((a.T + a.seg_len - 1) / a.seg_len);
+    if (a.nseg < 1) a.nseg = 1;
+}
+
+template <typename T, int DP>
+int launch(Args& a, const int (&joined)[2], int joins, hipStream_t st) {
+    if (a.nseg > 1) {
+        Args k = a;
+        k.roles = joins;
+        for (int i = 0; i < joins; ++i) k.r[i] = a.r[joined[i]];
+        static samx::LdsGrant grant;
+        if (int rc = grant.ensure((const void*)kv_kernel<T, DP>, sizeof(LdsKv<T, DP>))) return rc;
+        kv_kernel<T, DP><<<grid_of(k, a.nseg - 1), kThreads, sizeof(LdsKv<T, DP>), st>>>(k);
+        SAMX_LAUNCH_CHECK();
+        const int most = a.r[0].b.dim * a.r[0].c.dim;    // (the same product for every role)
+        join_kernel<<<dim3((unsigned)((most + 255) / 256), (unsigned)(a.B * a.H), (unsigned)joins), 256, 0, st>>>(k, a.nseg - 1);
+        SAMX_LAUNCH_CHECK();
+    }
+    static samx::LdsGrant grant;
+    if (int rc = grant.ensure((const void*)mix_kernel<T, DP>, sizeof(Lds<T, DP>))) return rc;
+    mix_kernel<T, DP><<<grid_of(a, a.nseg), kThreads, sizeof(Lds<T, DP>), st>>>(a);
+    SAMX_LAUNCH_CHECK();
+    return SAMX_OK;
+}
+
+template <typename T>
+int launch_dim(Args& a, int most, const int (&joined)[2], int joins, hipStream_t st) {
+    return most <= 64 ? launch<T, 64>(a, joined, joins, st) : launch<T, 128>(a, joined, joins, st);
+}
+
+int launch_type(int dtype, Args& a, int most, const int (&joined)[2], int joins, hipStream_t st) {
+    if (dtype == kF32) return launch_dim<float>(a, most, joined, joins, st);
+    if (dtype == kBF16) return launch_dim<bf16>(a, most, joined, joins, st);
+    return launch_dim<f16>(a, most, joined, joins, st);
+}
+
+int64_t up4(int64_t n) { return (n + 3) / 4 * 4; }
+
+int check(const char* who, const samx_linattn_shape* s) {
+    SAMX_REQUIRE(s, "%s: null shape", who);
+    SAMX_REQUIRE(s->dtype >= 0 && s->dtype <= 2, "%s: unknown element type %d", who, s->dtype);
+    SAMX_REQUIRE(s->B >= 0 && s->T >= 0 && s->T < (int64_t(1) << 31) && s->H > 0 && s->HK > 0 && s->H % s->HK == 0,
+                 "%s: bad sizes (B %lld, T %lld, H %d, HK %d; H has to be a multiple of HK)", who, (long long)s->B,
+                 (long long)s->T, s->H, s->HK);
+    SAMX_REQUIRE(s->D > 0 && s->D <= kMaxDim && s->DV > 0 && s->DV <= kMaxDim, "%s: head dimensions %d, %d must be in [1, %d]", who,
+                 s->D, s->DV, kMaxDim);
+    SAMX_REQUIRE(s->B * s->H <= 65535, "%s: B * H %lld is more than 65535", who, (long long)(s->B * s->H));
+    return SAMX_OK;
+}
+
+Mat mat(const void* p, const int64_t (&st)[3], int grp, int dim) { return Mat{p, st[0], st[1], st[2], grp, dim}; }
+
+size_t seg_bytes(const Args& a, int D, int DV) {
+    return a.nseg > 1 ? (size_t)a.B * a.H * (a.nseg - 1) * up4(D) * up4(DV) * sizeof(float) : 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t samx_linattn_ws_bytes(const samx_linattn_shape* s) {
+    if (check("samx_linattn_ws_bytes", s)) return 0;
+    Args a{};
+    a.roles = 1; a.B = (int)s->B; a.H = s->H; a.T = s->T;
+    cut(a);
+    return seg_bytes(a, s->D, s->DV) + 256;
+}
+
+int samx_linattn(const samx_linattn_shape* s, const void* q, const void* k, const void* v, const float* decay, float scale,
+                 const float* state_in, const int32_t* lengths, void* out, float* state_out, void* ws, size_t ws_bytes,
+                 void* stream) {
+    if (int rc = check("samx_linattn", s)) return rc;
+    SAMX_REQUIRE(isfinite(scale), "samx_linattn: scale must be finite");
+    if (s->B == 0) return SAMX_OK;
+    SAMX_REQUIRE(((q && k && v && out) || s->T == 0) && decay && state_out, "samx_linattn: null pointer");
+    Args a{};
+    a.roles = 1; a.B = (int)s->B; a.H = s->H; a.T = s->T; a.decay = decay; a.lengths = lengths;
+    cut(a);
+    const size_t need = seg_bytes(a, s->D, s->DV);
+    if (need && (!ws || ws_bytes < need)) return samx::fail(SAMX_ERR_WORKSPACE, "samx_linattn: workspace %zu < %zu", ws_bytes, need);
+    const int rep = s->H / s->HK;
+    a.seg_size = up4(s->D) * up4(s->DV);
+    Role& r = a.r[0];
+    r.a = mat(q, s->q, 1, s->D); r.b = mat(k, s->k, rep, s->D); r.c = mat(v, s->v, rep, s->DV);
+    r.out = out; r.kv = 1.f; r.ps = scale; r.so = scale;
+    r.s_in = state_in; r.in_a = s->DV; r.in_c = 1; r.s_out = state_out;
+    r.seg = (float*)ws; r.seg_a = 1; r.seg_c = up4(s->D);
+    const int joined[2] = {0, 0};
+    return launch_type(s->dtype, a, s->D > s->DV ? s->D : s->DV, joined, 1, (hipStream_t)stream);
+}
+
+size_t samx_linattn_grad_ws_bytes(const samx_linattn_shape* s) {
+    if (check("samx_linattn_grad_ws_bytes", s)) return 0;
+    Args a{};
+    a.roles = 3; a.B = (int)s->B; a.H = s->H; a.T = s->T;
+    cut(a);
+    const size_t rows = s->H == s->HK ? 0 : (size_t)s->B * s->T * s->H;
+    return 2 * seg_bytes(a, s->D, s->DV) + rows * (s->D + s->DV) * sizeof(float) + 256;
+}
+
+int samx_linattn_grad(const samx_linattn_shape* s, const void* q, const void* k, const void* v, const float* decay,
+                      const void* dout, float scale, const float* state_in, const float* dstate, const int32_t* lengths,
+                      void* dq, void* dk, void* dv, float* dstate_in, void* ws, size_t ws_bytes, void* stream) {
+    if (int rc = check("samx_linattn_grad", s)) return rc;
+    SAMX_REQUIRE(isfinite(scale), "samx_linattn_grad: scale must be finite");
+    if (s->B == 0) return SAMX_OK;
+    SAMX_REQUIRE(((q && k && v && dout && dq && dk && dv) || s->T == 0) && decay && dstate_in, "samx_linattn_grad: null pointer");
+    const size_t need = samx_linattn_grad_ws_bytes(s) - 256;
+    if (need && (!ws || ws_bytes < need)) return samx::fail(SAMX_ERR_WORKSPACE, "samx_linattn_grad: workspace %zu < %zu", ws_bytes, need);
+    Args a{};
+    a.roles = 3; a.B = (int)s->B; a.H = s->H; a.T = s->T; a.decay = decay; a.lengths = lengths;
+    cut(a);
+    const int rep = s->H / s->HK, D = s->D, DV = s->DV;
+    const Mat Q = mat(q, s->q, 1, D), K = mat(k, s->k, rep, D), V = mat(v, s->v, rep, DV), O = mat(dout, s->o, 1, DV);
+    a.seg_size = up4(D) * up4(DV);
+    float* seg0 = (float*)ws;
+    float* seg1 = seg0 + seg_bytes(a, D, DV) / sizeof(float);
+    float* heads = seg1 + seg_bytes(a, D, DV) / sizeof(float);
+    const int64_t rows = s->B * s->T;
+    float* dk_h = heads;
+    float* dv_h = heads + rows * s->H * D;
+    // dq: the forward states, transposed
+    Role& x = a.r[0];
+    x.a = O; x.b = V; x.c = K; x.out = dq; x.kv = 1.f; x.ps = scale; x.so = scale;
+    x.s_in = state_in; x.in_a = 1; x.in_c = DV; x.seg = seg0; x.seg_a = 1; x.seg_c = up4(DV);
+    // dv: the gradient's states; the last of them, decayed, is the gradient of the state before the first row
+    Role& y = a.r[1];
+    y.a = K; y.b = Q; y.c = O; y.out = rep > 1 ? (void*)dv_h : dv; y.out_f32 = rep > 1; y.rev = 1;
+    y.kv = scale; y.ps = scale; y.so = 1.f;
+    y.s_in = dstate; y.in_a = DV; y.in_c = 1; y.s_out = dstate_in; y.seg = seg1; y.seg_a = 1; y.seg_c = up4(D);
+    // dk: the same states, transposed
+    Role& z = a.r[2];
+    z = y;
+    z.a = V; z.b = O; z.c = Q; z.out = rep > 1 ? (void*)dk_h : dk; z.s_out = nullptr;
+    z.in_a = 1; z.in_c = DV; z.seg_a = up4(D); z.seg_c = 1;
+    const hipStream_t st = (hipStream_t)stream;
+    const int joined[2] = {0, 1};
+    if (int rc = launch_type(s->dtype, a, D > DV ? D : DV, joined, 2, st)) return rc;
+    if (rep > 1 && rows > 0) {
+        for (int i = 0; i < 2; ++i) {
+            const int dim = i ? DV : D;
+            const int64_t n = rows * s->HK * dim;
+            const float* in = i ? dv_h : dk_h;
+            void* out = i ? dv : dk;
+            const unsigned g = (unsigned)((n + 255) / 256);
+            if (s->dtype == kF32) group_kernel<float><<<g, 256, 0, st>>>(in, (float*)out, n, rep, dim);
+            else if (s->dtype == kBF16) group_kernel<bf16><<<g, 256, 0, st>>>(in, (bf16*)out, n, rep, dim);
+            else group_kernel<f16><<<g, 256, 0, st>>>(in, (f16*)out, n, rep, dim);
+            SAMX_LAUNCH_CHECK();
+        }
+    }
+    return SAMX_OK;
+}
+
+int samx_linattn_step(const samx_linattn_shape* s, const void* q, const void* k, const void* v, const float* decay, float scale,
+                      float* state, void* out, void* stream) {
+    if (int rc = check("samx_linattn_step", s)) return rc;
+    SAMX_REQUIRE(isfinite(scale), "samx_linattn_step: scale must be finite");
+    if (s->B == 0) return SAMX_OK;
+    SAMX_REQUIRE(q && k && v && decay && state && out, "samx_linattn_step: null pointer");
+    const int rep = s->H / s->HK;
+    const Mat Q = mat(q, s->q, 1, s->D), K = mat(k, s->k, rep, s->D), V = mat(v, s->v, rep, s->DV);
+    int cols = 16;
+    while (cols < s->DV && cols < 128) cols *= 2;
+    const int per = (s->DV + cols - 1) / cols;
+    const unsigned g = (unsigned)(s->B * s->H * per);
+    const hipStream_t st = (hipStream_t)stream;
+    if (s->dtype == kF32) step_kernel<float><<<g, 256, 0, st>>>(Q, K, V, decay, state, (float*)out, s->H, s->D, s->DV, scale, cols, per);
+    else if (s->dtype == kBF16) step_kernel<bf16><<<g, 256, 0, st>>>(Q, K, V, decay, state, (bf16*)out, s->H, s->D, s->DV, scale, cols, per);
+    else step_kernel<f16><<<g, 256, 0, st>>>(Q, K, V, decay, state, (f16*)out, s->H, s->D, s->DV, scale, cols, per);
+    SAMX_LAUNCH_CHECK();
+    return SAMX_OK;
+}
+
+}  // extern "C"

@@ -1017,6 +1017,94 @@ def block_norm_grad(y, h, dh, du, post_w, pre_w, post_b=None, pre_b=None, gate=N
     return out
 
 
+def _heads(t, like, shape, name):
+    """[B, T, heads, dim] dense in the last dimension -> its strides (batch, row, head)."""
+    if not (isinstance(t, torch.Tensor) and t.device == like.device and t.dtype == like.dtype):
+        raise TypeError('%s must be %s on %s' % (name, like.dtype, like.device))
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError('%s has shape %s, expected %s' % (name, tuple(t.shape), tuple(shape)))
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError('%s must be dense in its last dimension' % name)
+    return t.stride()[:-1]
+
+
+def _linattn_args(q, k, v, decay, dout=None):
+    code = _seq_dtype(q, 'q')
+    if q.dim() != 4 or not isinstance(k, torch.Tensor) or k.dim() != 4 or not isinstance(v, torch.Tensor) or v.dim() != 4:
+        raise ValueError('q, k and v must be [batch, rows, heads, dim]')
+    B, T, H, D = q.shape
+    HK, DV = k.shape[2], v.shape[3]
+    s = _lib.LinattnShape(code, H, HK, D, DV, 0, B, T)
+    s.q[:] = _heads(q, q, (B, T, H, D), 'q')
+    s.k[:] = _heads(k, q, (B, T, HK, D), 'k')
+    s.v[:] = _heads(v, q, (B, T, HK, DV), 'v')
+    if dout is not None:
+        s.o[:] = _heads(dout, q, (B, T, H, DV), 'dout')
+    _on(decay, q, F32, (H,), 'decay')
+    return s
+
+
+def _linattn_ws(s, ws, nbytes, like):
+    if ws is None:
+        return torch.empty(max(1, nbytes), dtype=torch.uint8, device=like.device)
+    return _on(ws, like, torch.uint8, (ws.numel(),), 'ws')
+
+
+def linattn(q, k, v, decay, scale=1.0, state=None, lengths=None, out=None, state_out=None, ws=None):
+    """Linear attention with a decay for each head, S_t = exp(decay) S_{t-1} + k_t v_t^T, out_t = scale q_t^T S_t, over
+    whole sequences: q [B, T, H, D], k [B, T, HK, D], v [B, T, HK, DV] in float32, bfloat16 or float16 (views of a joint
+    projection may be given), decay float32 [H], state float32 [B, H, D, DV] before the first row (None: zero), lengths
+    int32 [B] (None: T).  Returns (out [B, T, H, DV], the state behind the last row) (samx_linattn)."""
+    s = _linattn_args(q, k, v, decay)
+    shape = (s.B, s.H, s.D, s.DV)
+    _opt_on(state, q, F32, shape, 'state'); _opt_on(lengths, q, I32, (s.B,), 'lengths')
+    made = out is None or state_out is None
+    out = torch.empty((s.B, s.T, s.H, s.DV), dtype=q.dtype, device=q.device) if out is None else \
+        _on(out, q, q.dtype, (s.B, s.T, s.H, s.DV), 'out')
+    state_out = torch.empty(shape, dtype=F32, device=q.device) if state_out is None else \
+        _on(state_out, q, F32, shape, 'state_out')
+    if not made:
+        _apart((('out', out), ('state_out', state_out)))
+    if state is not None and state.data_ptr() == state_out.data_ptr() and state.numel():
+        raise ValueError('state_out is state: the segments of a sequence read it while others write')
+    L = _L()
+    ws = _linattn_ws(s, ws, L.samx_linattn_ws_bytes(C.byref(s)), q)
+    check(L.samx_linattn(C.byref(s), q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr(decay), float(scale), ptr(state),
+                         ptr(lengths), ptr(out), ptr(state_out), ptr(ws), ws.numel(), stream_ptr()))
+    return out, state_out
+
+
+def linattn_grad(q, k, v, decay, dout, scale=1.0, state=None, dstate=None, lengths=None, ws=None):
+    """The gradient of linattn from dout and dstate (of the state behind the last row, None: zero); decay counts as a
+    constant.  Returns (dq, dk, dv, the gradient of the state before the first row) (samx_linattn_grad)."""
+    s = _linattn_args(q, k, v, decay, dout)
+    shape = (s.B, s.H, s.D, s.DV)
+    _opt_on(state, q, F32, shape, 'state'); _opt_on(dstate, q, F32, shape, 'dstate')
+    _opt_on(lengths, q, I32, (s.B,), 'lengths')
+    L = _L()
+    ws = _linattn_ws(s, ws, L.samx_linattn_grad_ws_bytes(C.byref(s)), q)
+    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
+    ds = torch.empty(shape, dtype=F32, device=q.device)
+    check(L.samx_linattn_grad(C.byref(s), q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr(decay), dout.data_ptr(),
+                              float(scale), ptr(state), ptr(dstate), ptr(lengths), ptr(dq), ptr(dk), ptr(dv), ptr(ds),
+                              ptr(ws), ws.numel(), stream_ptr()))
+    return dq, dk, dv, ds
+
+
+def linattn_step(q, k, v, decay, state, scale=1.0, out=None):
+    """One row of each sequence (acting): q [B, H, D], k [B, HK, D], v [B, HK, DV], state float32 [B, H, D, DV], updated in
+    place.  Returns out [B, H, DV] (samx_linattn_step)."""
+    if not all(isinstance(t, torch.Tensor) and t.dim() == 3 for t in (q, k, v)):
+        raise ValueError('q, k and v must be [batch, heads, dim]')
+    s = _linattn_args(q[:, None], k[:, None], v[:, None], decay)
+    _on(state, q, F32, (s.B, s.H, s.D, s.DV), 'state')
+    out = torch.empty((s.B, s.H, s.DV), dtype=q.dtype, device=q.device) if out is None else \
+        _on(out, q, q.dtype, (s.B, s.H, s.DV), 'out')
+    check(_L().samx_linattn_step(C.byref(s), q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr(decay), float(scale),
+                                 ptr(state), ptr(out), stream_ptr()))
+    return out
+
+
 def _rows2(t, name):
     """[rows, columns] with dense columns -> row stride in elements."""
     if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):

@@ -94,3 +94,45 @@ def distill(z, idx, t, tau, lse, weight, scale):
         loss[i] = w * total
         grad[i] = scale / tau * w * (mass[i] * logq.exp() - dense)
     return loss, grad, mass
+
+
+# ------------------------------------------------------------------ linear attention
+
+def _spans(lengths, B, T):
+    return [T if lengths is None else max(0, min(T, int(lengths[b]))) for b in range(B)]
+
+
+def linattn(q, k, v, decay, scale, state, lengths):
+    """The recurrence: (out, state behind the last row)."""
+    B, T, H, D = q.shape
+    HK, DV = k.shape[2], v.shape[3]
+    out = torch.zeros(B, T, H, DV, dtype=torch.float64)
+    S = torch.zeros(B, H, D, DV, dtype=torch.float64) if state is None else state.clone()
+    lam = torch.exp(decay)[:, None, None]
+    head = torch.arange(H) // (H // HK)
+    for b, n in enumerate(_spans(lengths, B, T)):
+        for t in range(n):
+            S[b] = lam * S[b] + k[b, t, head][:, :, None] * v[b, t, head][:, None, :]
+            out[b, t] = scale * (q[b, t][:, None, :] @ S[b])[:, 0]
+    return out, S
+
+
+def linattn_grad(q, k, v, decay, dout, scale, state, dstate, lengths):
+    """By the formulas: (dq, dk, dv, gradient of the state before the first row)."""
+    B, T, H, D = q.shape
+    HK, DV = k.shape[2], v.shape[3]
+    dq, dk, dv = (torch.zeros(t.shape, dtype=torch.float64) for t in (q, k, v))
+    S = torch.zeros(B, H, D, DV, dtype=torch.float64) if state is None else state.clone()
+    G = torch.zeros(B, H, D, DV, dtype=torch.float64) if dstate is None else dstate.clone()
+    lam = torch.exp(decay)[:, None, None]
+    head, rep = torch.arange(H) // (H // HK), H // HK
+    for b, n in enumerate(_spans(lengths, B, T)):
+        for t in range(n):
+            S[b] = lam * S[b] + k[b, t, head][:, :, None] * v[b, t, head][:, None, :]
+            dq[b, t] = scale * (S[b] @ dout[b, t][:, :, None])[:, :, 0]
+        for t in reversed(range(n)):
+            g = G[b] + scale * q[b, t][:, :, None] * dout[b, t][:, None, :]
+            dk[b, t] = (g @ v[b, t, head][:, :, None])[:, :, 0].reshape(HK, rep, D).sum(1)
+            dv[b, t] = (k[b, t, head][:, None, :] @ g)[:, 0].reshape(HK, rep, DV).sum(1)
+            G[b] = lam * g
+    return dq, dk, dv, G
