@@ -32,91 +32,123 @@ struct Args {
     float res, eps;
 };
 
-// E float32 channel values of this thread; a lane's elements are P pieces of kN, piece p at (p * G + lane) * kN
+// This thread's elements of a row: P pieces, piece p the kN elements from at[p] on.  The row's last piece starts kN before
+// its end, however few of its elements are not its neighbour's: those come as zeros (keep), so that every load is a whole
+// one.  Rows of less than a piece are read by elements.
 template <typename T, int G, int P>
-__device__ __forceinline__ void load_channels(const float* w, int D, int lane, float other, float (&out)[P * Piece<T>::kN]) {
-    constexpr int N = Piece<T>::kN;
+struct Cols {
+    static constexpr int N = Piece<T>::kN, E = P * N;
+    int D, at[P], first[P];               // first: elements that are the neighbour's (kN: all, no piece)
+    uint32_t keep[P][4];
+    __device__ Cols(int D_, int lane) : D(D_) {
 #pragma unroll
-    for (int p = 0; p < P; ++p)
+        for (int p = 0; p < P; ++p) {
+            const int want = (p * G + lane) * N, last = D >= N ? D - N : 0;
+            at[p] = want < last ? want : last;
+            first[p] = want >= D ? N : want - at[p];
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int at = (p * G + lane) * N + j;
-            out[p * N + j] = w && at < D ? w[at] : other;
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (sizeof(T) == 4) keep[p][j] = j >= first[p] ? ~0u : 0u;
+                else keep[p][j] = (2 * j >= first[p] ? 0xffffu : 0u) | (2 * j + 1 >= first[p] ? 0xffff0000u : 0u);
+            }
         }
-}
-
-template <typename T, int G, int P>
-__device__ __forceinline__ void load_row(const void* base, int64_t row, int64_t rows, int D, int lane, Piece<T> (&r)[P]) {
-    const T* at = (const T*)base + (row < rows ? row : 0) * (int64_t)D;
-#pragma unroll
-    for (int p = 0; p < P; ++p) r[p] = load_piece(at, (int64_t)(p * G + lane) * Piece<T>::kN, row < rows ? D : 0, from_float<T>(0.f));
-}
-
-template <typename T, int G, int P>
-__device__ __forceinline__ void store_row(void* base, int64_t row, int D, int lane, const float (&v)[P * Piece<T>::kN]) {
-    constexpr int N = Piece<T>::kN;
-    T* at = (T*)base + row * (int64_t)D;
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-        Piece<T> o;
-#pragma unroll
-        for (int j = 0; j < N; ++j) o.e[j] = from_float<T>(v[p * N + j]);
-        store_piece(at, (int64_t)(p * G + lane) * N, (int64_t)D, o);
     }
-}
-
-// the lanes' elements that are channels at all (the others hold zeros and stay out of a variance)
-template <typename T, int G, int P>
-__device__ __forceinline__ bool in_row(int D, int lane, int i) {
-    constexpr int N = Piece<T>::kN;
-    return (i / N * G + lane) * N + i % N < D;
-}
+    // whether element i of the thread is its own
+    __device__ __forceinline__ bool own(int i) const {
+        return i % N >= first[i / N] && at[i / N] + i % N < D;
+    }
+    __device__ __forceinline__ void channels(const float* w, float (&out)[E]) const {
+#pragma unroll
+        for (int i = 0; i < E; ++i) out[i] = own(i) ? w[at[i / N] + i % N] : 0.f;
+    }
+    __device__ __forceinline__ void load(const void* base, int64_t row, int64_t rows, Piece<T> (&r)[P]) const {
+        const T* x = (const T*)base + (row < rows ? row : 0) * (int64_t)D;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            if (D >= N) {
+                const Raw16 v = *reinterpret_cast<const Raw16*>(x + at[p]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) r[p].w[j] = row < rows ? v.w[j] & keep[p][j] : 0u;
+            } else {
+                r[p] = load_piece(x, 0, row < rows && first[p] == 0 ? D : 0, 0u);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(void* base, int64_t row, const float (&v)[E]) const {
+        T* x = (T*)base + row * (int64_t)D;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const Piece<T> o = pack<T>(v + p * N);
+            if (first[p] == 0 && D >= N) {
+                Raw16 r;
+                __builtin_memcpy(&r, &o, 16);
+                *reinterpret_cast<Raw16*>(x + at[p]) = r;
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (own(p * N + j)) {
+                        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(x + at[p] + j) = o.w[j];
+                        else *reinterpret_cast<uint16_t*>(x + at[p] + j) = (uint16_t)o.bits(j);
+                    }
+            }
+        }
+    }
+};
 
 template <typename T, int G, int P, bool LAYER, int GATE>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void forward_kernel(Args a) {
     constexpr int B = G < 256 ? 256 : G, W = B / 64, N = Piece<T>::kN, E = P * N, R = B / G;
     __shared__ float sh[2 * W];
     int turn = 0;
-    const int lane = threadIdx.x % G, D = a.D;
+    const int D = a.D;
+    const Cols<T, G, P> cols(D, threadIdx.x % G);
     const float inv = 1.f / (float)D;
-    float w1[E], w2[E], b1[E], b2[E], gc[E];
-    load_channels<T, G, P>(a.w1, D, lane, 0.f, w1);
-    load_channels<T, G, P>(a.w2, D, lane, 0.f, w2);
+    float w1[E], w2[E], b1[E], b2[E];
+    cols.channels(a.w1, w1);
+    cols.channels(a.w2, w2);
     if constexpr (LAYER) {
-        load_channels<T, G, P>(a.b1, D, lane, 0.f, b1);
-        load_channels<T, G, P>(a.b2, D, lane, 0.f, b2);
+        cols.channels(a.b1, b1);
+        cols.channels(a.b2, b2);
     }
-    if constexpr (GATE == kChannel) load_channels<T, G, P>((const float*)a.gate, D, lane, 0.f, gc);
+    if constexpr (GATE == kChannel) {   // a channel's gate is a factor of its weight and its bias
+        float gc[E];
+        cols.channels((const float*)a.gate, gc);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            w1[i] *= gc[i];
+            if constexpr (LAYER) b1[i] *= gc[i];
+        }
+    }
     const int64_t step = (int64_t)gridDim.x * R;
     int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / G;
     Piece<T> ry[P], rx[P], rg[P];
-    load_row<T, G, P>(a.y, row, a.N, D, lane, ry);
-    load_row<T, G, P>(a.x, row, a.N, D, lane, rx);
-    if constexpr (GATE == kFull) load_row<T, G, P>(a.gate, row, a.N, D, lane, rg);
+    cols.load(a.y, row, a.N, ry);
+    cols.load(a.x, row, a.N, rx);
+    if constexpr (GATE == kFull) cols.load(a.gate, row, a.N, rg);
     for (int64_t base = (int64_t)blockIdx.x * R; base < a.N; base += step, row += step) {
         float h[E];
         float v[1] = {0.f};
         if constexpr (LAYER) {
 #pragma unroll
-            for (int i = 0; i < E; ++i) { h[i] = to_float(ry[i / N].e[i % N]); v[0] += h[i]; }
+            for (int i = 0; i < E; ++i) { h[i] = ry[i / N].f(i % N); v[0] += h[i]; }
             row_reduce<OpSum, G>(v, sh, W, turn);
             const float m = v[0] * inv;
             v[0] = 0.f;
 #pragma unroll
-            for (int i = 0; i < E; ++i) { h[i] = in_row<T, G, P>(D, lane, i) ? h[i] - m : 0.f; v[0] += h[i] * h[i]; }
+            for (int i = 0; i < E; ++i) { h[i] = cols.own(i) ? h[i] - m : 0.f; v[0] += h[i] * h[i]; }
         } else {
 #pragma unroll
-            for (int i = 0; i < E; ++i) { h[i] = to_float(ry[i / N].e[i % N]); v[0] += h[i] * h[i]; }
+            for (int i = 0; i < E; ++i) { h[i] = ry[i / N].f(i % N); v[0] += h[i] * h[i]; }
         }
         float x[E], g[E];
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = to_float(rx[i / N].e[i % N]);
+        for (int i = 0; i < E; ++i) x[i] = rx[i / N].f(i % N);
         if constexpr (GATE == kFull)
 #pragma unroll
-            for (int i = 0; i < E; ++i) g[i] = to_float(rg[i / N].e[i % N]);
-        load_row<T, G, P>(a.y, row + step, a.N, D, lane, ry);
-        load_row<T, G, P>(a.x, row + step, a.N, D, lane, rx);
-        if constexpr (GATE == kFull) load_row<T, G, P>(a.gate, row + step, a.N, D, lane, rg);
+            for (int i = 0; i < E; ++i) g[i] = rg[i / N].f(i % N);
+        cols.load(a.y, row + step, a.N, ry);
+        cols.load(a.x, row + step, a.N, rx);
+        if constexpr (GATE == kFull) cols.load(a.gate, row + step, a.N, rg);
         row_reduce<OpSum, G>(v, sh, W, turn);
         const float sy = 1.f / sqrtf(v[0] * inv + a.eps);
         v[0] = 0.f;
@@ -124,18 +156,17 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void forward_kernel(Args a) {
         for (int i = 0; i < E; ++i) {
             float n = h[i] * sy * w1[i];
             if constexpr (LAYER) n += b1[i];
-            if constexpr (GATE == kChannel) n *= gc[i];
             if constexpr (GATE == kFull) n *= g[i];
             h[i] = a.res * x[i] + n;
             v[0] += LAYER ? h[i] : h[i] * h[i];
         }
-        if (row < a.N) store_row<T, G, P>(a.o1, row, D, lane, h);
+        if (row < a.N) cols.store(a.o1, row, h);
         row_reduce<OpSum, G>(v, sh, W, turn);
         if constexpr (LAYER) {
             const float m = v[0] * inv;
             v[0] = 0.f;
 #pragma unroll
-            for (int i = 0; i < E; ++i) { h[i] = in_row<T, G, P>(D, lane, i) ? h[i] - m : 0.f; v[0] += h[i] * h[i]; }
+            for (int i = 0; i < E; ++i) { h[i] = cols.own(i) ? h[i] - m : 0.f; v[0] += h[i] * h[i]; }
             row_reduce<OpSum, G>(v, sh, W, turn);
         }
         const float su = 1.f / sqrtf(v[0] * inv + a.eps);
@@ -144,51 +175,58 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void forward_kernel(Args a) {
             h[i] = h[i] * su * w2[i];
             if constexpr (LAYER) h[i] += b2[i];
         }
-        if (row < a.N) store_row<T, G, P>(a.o2, row, D, lane, h);
+        if (row < a.N) cols.store(a.o2, row, h);
     }
 }
 
-// sums over the rows, in this order: dw1, dw2, [db1, db2 (LAYER)], [dgate (kChannel)]
-template <bool LAYER, int GATE> constexpr int kSums = 2 + (LAYER ? 2 : 0) + (GATE == kChannel ? 1 : 0);
+// sums over the rows: A = sum g dh' yh (g: kFull, else without it), dw2, and for LayerNorm B = sum g dh', db2.  A channel's
+// gate is a factor of its sums: dw1 = g A, db1 = g B, dgate = w1 A + b1 B.
+template <bool LAYER> constexpr int kSums = LAYER ? 4 : 2;
 
 template <typename T, int G, int P, bool LAYER, int GATE>
-__global__ __launch_bounds__(G < 256 ? 256 : G) void backward_kernel(Args a) {
+__global__ __launch_bounds__(G < 256 ? 256 : G, 4) void backward_kernel(Args a) {
     constexpr int B = G < 256 ? 256 : G, W = B / 64, N = Piece<T>::kN, E = P * N, R = B / G;
     __shared__ float sh[2 * W * 4];
     int turn = 0;
-    const int lane = threadIdx.x % G, D = a.D;
+    const int D = a.D;
+    const Cols<T, G, P> cols(D, threadIdx.x % G);
     const float inv = 1.f / (float)D;
-    float w1[E], w2[E], b1[E], gc[E];
-    load_channels<T, G, P>(a.w1, D, lane, 0.f, w1);
-    load_channels<T, G, P>(a.w2, D, lane, 0.f, w2);
-    if constexpr (LAYER && GATE != kNone) load_channels<T, G, P>(a.b1, D, lane, 0.f, b1);
-    if constexpr (GATE == kChannel) load_channels<T, G, P>((const float*)a.gate, D, lane, 0.f, gc);
-    float dw1[E], dw2[E], db1[E], db2[E], dgc[E];
+    float w1[E], w2[E], b1[E];
+    cols.channels(a.w1, w1);
+    cols.channels(a.w2, w2);
+    if constexpr (LAYER && GATE == kFull) cols.channels(a.b1, b1);
+    if constexpr (GATE == kChannel) {
+        float gc[E];
+        cols.channels((const float*)a.gate, gc);
 #pragma unroll
-    for (int i = 0; i < E; ++i) dw1[i] = dw2[i] = db1[i] = db2[i] = dgc[i] = 0.f;
+        for (int i = 0; i < E; ++i) w1[i] *= gc[i];
+    }
+    float sa[E], sw[E], sb[E], sv[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) sa[i] = sw[i] = sb[i] = sv[i] = 0.f;
     const int64_t step = (int64_t)gridDim.x * R;
     int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / G;
     Piece<T> ry[P], rh[P], rdu[P], rdh[P], rg[P];
-    load_row<T, G, P>(a.y, row, a.N, D, lane, ry);
-    load_row<T, G, P>(a.h, row, a.N, D, lane, rh);
-    load_row<T, G, P>(a.du, row, a.N, D, lane, rdu);
-    load_row<T, G, P>(a.dh, row, a.N, D, lane, rdh);
-    if constexpr (GATE == kFull) load_row<T, G, P>(a.gate, row, a.N, D, lane, rg);
+    cols.load(a.y, row, a.N, ry);
+    cols.load(a.h, row, a.N, rh);
+    cols.load(a.du, row, a.N, rdu);
+    cols.load(a.dh, row, a.N, rdh);
+    if constexpr (GATE == kFull) cols.load(a.gate, row, a.N, rg);
     for (int64_t base = (int64_t)blockIdx.x * R; base < a.N; base += step, row += step) {
         float y[E], h[E], du[E], dh[E], g[E];
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            y[i] = to_float(ry[i / N].e[i % N]);
-            h[i] = to_float(rh[i / N].e[i % N]);
-            du[i] = to_float(rdu[i / N].e[i % N]);
-            dh[i] = to_float(rdh[i / N].e[i % N]);
-            if constexpr (GATE == kFull) g[i] = to_float(rg[i / N].e[i % N]);
+            y[i] = ry[i / N].f(i % N);
+            h[i] = rh[i / N].f(i % N);
+            du[i] = rdu[i / N].f(i % N);
+            dh[i] = rdh[i / N].f(i % N);
+            if constexpr (GATE == kFull) g[i] = rg[i / N].f(i % N);
         }
-        load_row<T, G, P>(a.y, row + step, a.N, D, lane, ry);
-        load_row<T, G, P>(a.h, row + step, a.N, D, lane, rh);
-        load_row<T, G, P>(a.du, row + step, a.N, D, lane, rdu);
-        load_row<T, G, P>(a.dh, row + step, a.N, D, lane, rdh);
-        if constexpr (GATE == kFull) load_row<T, G, P>(a.gate, row + step, a.N, D, lane, rg);
+        cols.load(a.y, row + step, a.N, ry);
+        cols.load(a.h, row + step, a.N, rh);
+        cols.load(a.du, row + step, a.N, rdu);
+        cols.load(a.dh, row + step, a.N, rdh);
+        if constexpr (GATE == kFull) cols.load(a.gate, row + step, a.N, rg);
         if constexpr (LAYER) {
             float v[2] = {0.f, 0.f};
 #pragma unroll
@@ -197,7 +235,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void backward_kernel(Args a) {
             const float my = v[0] * inv, mh = v[1] * inv;
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                const bool in = in_row<T, G, P>(D, lane, i);
+                const bool in = cols.own(i);
                 y[i] = in ? y[i] - my : 0.f;
                 h[i] = in ? h[i] - mh : 0.f;
             }
@@ -217,82 +255,83 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void backward_kernel(Args a) {
         const float sy = row < a.N ? 1.f / sqrtf(v[0] * inv + a.eps) : 0.f;
         const float s = row < a.N ? 1.f / sqrtf(v[1] * inv + a.eps) : 0.f;
         const float kh = v[2] * s * inv, km = LAYER ? v[3] * inv : 0.f;
-        // dh becomes the whole gradient of h, y the normalised y
+        // dh becomes the whole gradient of h, y the normalised y, h k', du the gate's gradient
         float t[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             const float hh = h[i] * s;
             dh[i] += s * (du[i] * w2[i] - hh * kh - km);
-            dw2[i] += du[i] * hh;
-            if constexpr (LAYER) db2[i] += du[i];
+            sw[i] += du[i] * hh;
+            if constexpr (LAYER) sv[i] += du[i];
             y[i] *= sy;
             float dn = dh[i];
-            if constexpr (GATE == kChannel) dn *= gc[i];
             if constexpr (GATE == kFull) dn *= g[i];
-            dw1[i] += dn * y[i];
-            if constexpr (LAYER) db1[i] += dn;
-            const float k = dn * w1[i];
-            t[0] += k * y[i];
-            if constexpr (LAYER) t[1] += k;
-            // du: the gate's gradient, h: k'
-            if constexpr (GATE != kNone) {
-                const float n = LAYER ? y[i] * w1[i] + b1[i] : y[i] * w1[i];
-                if constexpr (GATE == kChannel) dgc[i] += dh[i] * n;
-                else du[i] = dh[i] * n;
-            }
-            h[i] = k;
+            sa[i] += dn * y[i];
+            if constexpr (LAYER) sb[i] += dn;
+            h[i] = dn * w1[i];
+            t[0] += h[i] * y[i];
+            if constexpr (LAYER) t[1] += h[i];
+            if constexpr (GATE == kFull) du[i] = dh[i] * (LAYER ? y[i] * w1[i] + b1[i] : y[i] * w1[i]);
             dh[i] *= a.res;
         }
         if (row < a.N) {
-            store_row<T, G, P>(a.o1, row, D, lane, dh);
-            if constexpr (GATE == kFull) store_row<T, G, P>(a.og, row, D, lane, du);
+            cols.store(a.o1, row, dh);
+            if constexpr (GATE == kFull) cols.store(a.og, row, du);
         }
         row_reduce<OpSum, G>(t, sh, W, turn);
         const float ky = t[0] * inv, kn = LAYER ? t[1] * inv : 0.f;
 #pragma unroll
         for (int i = 0; i < E; ++i) h[i] = sy * (h[i] - y[i] * ky - kn);
-        if (row < a.N) store_row<T, G, P>(a.o2, row, D, lane, h);
+        if (row < a.N) cols.store(a.o2, row, h);
     }
     // this row group's sums; the groups of a wave are added first
-    constexpr int S = kSums<LAYER, GATE>, GW = G < 64 ? 64 : G;
+    constexpr int S = kSums<LAYER>, GW = G < 64 ? 64 : G;
     float* part = a.part + ((int64_t)blockIdx.x * (B / GW) + threadIdx.x / GW) * S * D;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        float v[5] = {dw1[i], dw2[i], db1[i], db2[i], dgc[i]};
+        float v[4] = {sa[i], sw[i], sb[i], sv[i]};
 #pragma unroll
         for (int o = G; o < 64; o <<= 1)
 #pragma unroll
-            for (int c = 0; c < 5; ++c) v[c] += __shfl_xor(v[c], o, 64);
-        dw1[i] = v[0]; dw2[i] = v[1]; db1[i] = v[2]; db2[i] = v[3]; dgc[i] = v[4];
-    }
+            for (int c = 0; c < S; ++c) v[c] += __shfl_xor(v[c], o, 64);
+        if (cols.own(i) && threadIdx.x % GW < G)
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        const int at = (i / N * G + lane) * N + i % N;
-        if (at < D && threadIdx.x % GW < G) {
-            part[at] = dw1[i];
-            part[D + at] = dw2[i];
-            if constexpr (LAYER) { part[2 * D + at] = db1[i]; part[3 * D + at] = db2[i]; }
-            if constexpr (GATE == kChannel) part[(S - 1) * D + at] = dgc[i];
-        }
+            for (int c = 0; c < S; ++c) part[c * D + cols.at[i / N] + i % N] = v[c];
     }
 }
 
-struct Columns { float* out[5]; };
+struct Columns { const float *w1, *b1, *gate; float *dw1, *dw2, *db1, *db2, *dgate; };
 
-// out[s][d] = sum over the parts: 64 columns a workgroup, 16 threads a column that take every 16th part
-__global__ __launch_bounds__(1024) void column_kernel(const float* __restrict__ part, int parts, int D, int sums, Columns c) {
-    __shared__ float sh[16][64];
-    const int64_t col = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63), all = (int64_t)sums * D;
-    const int g = threadIdx.x >> 6;
-    float v = 0.f;
-    if (col < all)
-        for (int p = g; p < parts; p += 16) v += part[p * all + col];
-    sh[g][threadIdx.x & 63] = v;
+// the sums of all parts and what follows from them: 16 columns a workgroup, 64 threads a column that take every 64th part
+template <bool LAYER>
+__global__ __launch_bounds__(1024) void column_kernel(const float* __restrict__ part, int parts, int D, Columns c) {
+    constexpr int S = kSums<LAYER>;
+    __shared__ float sh[16][S][16];
+    const int d = blockIdx.x * 16 + (threadIdx.x & 15), g = threadIdx.x >> 4;
+    float v[S];
+#pragma unroll
+    for (int k = 0; k < S; ++k) v[k] = 0.f;
+    if (d < D)
+        for (int p = g; p < parts; p += 64)
+#pragma unroll
+            for (int k = 0; k < S; ++k) v[k] += part[((int64_t)p * S + k) * D + d];
+#pragma unroll
+    for (int o = 16; o < 64; o <<= 1)
+#pragma unroll
+        for (int k = 0; k < S; ++k) v[k] += __shfl_xor(v[k], o, 64);
+    if ((threadIdx.x & 63) < 16)
+#pragma unroll
+        for (int k = 0; k < S; ++k) sh[threadIdx.x >> 6][k][threadIdx.x & 15] = v[k];
     __syncthreads();
-    if (g == 0 && col < all) {
-        for (int i = 1; i < 16; ++i) v += sh[i][threadIdx.x & 63];
-        c.out[col / D][col % D] = v;
-    }
+    if (threadIdx.x >= 16 || d >= D) return;
+    for (int w = 1; w < 16; ++w)
+#pragma unroll
+        for (int k = 0; k < S; ++k) v[k] += sh[w][k][threadIdx.x];
+    const float gate = c.gate ? c.gate[d] : 1.f;
+    c.dw1[d] = gate * v[0];
+    c.dw2[d] = v[1];
+    if constexpr (LAYER) { c.db1[d] = gate * v[2]; c.db2[d] = v[3]; }
+    if (c.dgate) c.dgate[d] = LAYER ? c.w1[d] * v[0] + c.b1[d] * v[2] : c.w1[d] * v[0];
 }
 
 // rows of a workgroup, pieces of a thread: a thread holds 8 elements (bf16, f16) or 4 of float32 until a row needs more
@@ -369,7 +408,8 @@ int samx_block_norm(const void* x, const void* y, int dtype, int64_t N, int64_t 
                     float eps, void* h, void* u, void* stream) {
     if (int rc = check("samx_block_norm", N, D, dtype, kind, gate_kind, res_scale, eps)) return rc;
     if (N == 0) return SAMX_OK;
-    SAMX_REQUIRE(x && y && post_w && pre_w && h && u && (gate_kind == kNone || gate), "samx_block_norm: null pointer");
+    SAMX_REQUIRE(x && y && post_w && pre_w && h && u && (gate_kind == kNone || gate) &&
+                     (kind == SAMX_NORM_RMS || (post_b && pre_b)), "samx_block_norm: null pointer");
     SAMX_REQUIRE(h != u, "samx_block_norm: h and u are two outputs");
     Args a{};
     a.x = x; a.y = y; a.gate = gate; a.w1 = post_w; a.b1 = post_b; a.w2 = pre_w; a.b2 = pre_b;
@@ -384,7 +424,7 @@ int samx_block_norm(const void* x, const void* y, int dtype, int64_t N, int64_t 
 size_t samx_block_norm_grad_ws_bytes(int dtype, int64_t N, int64_t D) {
     if (dtype < 0 || dtype > 2 || N < 0 || D <= 0 || D > most_dim(dtype)) return 0;
     const int G = threads_of(dtype, (int)D);
-    return (size_t)grid_of(N, G) * parts_of(G) * 5 * D * sizeof(float) + 256;
+    return (size_t)grid_of(N, G) * parts_of(G) * 4 * D * sizeof(float) + 256;
 }
 
 int samx_block_norm_grad(const void* y, const void* h, const void* dh, const void* du, int dtype, int64_t N, int64_t D,
@@ -397,7 +437,7 @@ int samx_block_norm_grad(const void* y, const void* h, const void* dh, const voi
                  "samx_block_norm_grad: null pointer");
     SAMX_REQUIRE(gate_kind == kNone || ((gate || (gate_kind == kFull && N == 0)) && (dgate || (gate_kind == kFull && N == 0))),
                  "samx_block_norm_grad: a gate needs its gradient's buffer");
-    SAMX_REQUIRE(kind == SAMX_NORM_RMS || (dpost_b && dpre_b), "samx_block_norm_grad: LayerNorm needs dpost_b and dpre_b");
+    SAMX_REQUIRE(kind == SAMX_NORM_RMS || (post_b && dpost_b && dpre_b), "samx_block_norm_grad: LayerNorm needs its biases");
     if (ws_bytes < samx_block_norm_grad_ws_bytes(dtype, N, D))
         return samx::fail(SAMX_ERR_WORKSPACE, "samx_block_norm_grad: workspace %zu < %zu", ws_bytes,
                           samx_block_norm_grad_ws_bytes(dtype, N, D));
@@ -412,13 +452,12 @@ int samx_block_norm_grad(const void* y, const void* h, const void* dh, const voi
                                       : pick<f16, true>(a, G, grid, kind, gate_kind, st);
         if (rc) return rc;
     }
-    Columns c{};
-    int sums = 0;
-    c.out[sums++] = dpost_w;
-    c.out[sums++] = dpre_w;
-    if (kind == SAMX_NORM_LAYER) { c.out[sums++] = dpost_b; c.out[sums++] = dpre_b; }
-    if (gate_kind == kChannel) c.out[sums++] = (float*)dgate;
-    column_kernel<<<(unsigned)(((int64_t)sums * D + 63) / 64), 1024, 0, st>>>((const float*)ws, grid * parts_of(G), (int)D, sums, c);
+    const bool channel = gate_kind == kChannel;
+    const Columns c{post_w, post_b, channel ? (const float*)gate : nullptr, dpost_w, dpre_w, dpost_b, dpre_b,
+                    channel ? (float*)dgate : nullptr};
+    const unsigned blocks = (unsigned)((D + 15) / 16);
+    if (kind == SAMX_NORM_LAYER) column_kernel<true><<<blocks, 1024, 0, st>>>((const float*)ws, grid * parts_of(G), (int)D, c);
+    else column_kernel<false><<<blocks, 1024, 0, st>>>((const float*)ws, grid * parts_of(G), (int)D, c);
     SAMX_LAUNCH_CHECK();
     return SAMX_OK;
 }

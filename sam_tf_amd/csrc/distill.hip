@@ -107,7 +107,7 @@ __device__ __forceinline__ double row_lse(float m, float s, double inv_tau) {
     return s > 0.f || s != s ? (double)m * inv_tau + log((double)s) : 0.0;
 }
 
-// One row for every G threads, the row in their registers (NV pieces each).
+// One row for every G threads, the row in their registers: NV whole pieces each, and of the last V % kN values one.
 template <typename T, int G, int NV, bool GRAD>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void row_kernel(Args a) {
     constexpr int B = G < 256 ? 256 : G, W = B / 64, N = Piece<T>::kN;
@@ -115,40 +115,44 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void row_kernel(Args a) {
     __shared__ float shf[2 * W * 2];
     __shared__ double shd[2 * W * 2];
     int turn = 0, turnd = 0;
-    const int lane = threadIdx.x % G;
-    const int64_t row = (int64_t)blockIdx.x * (B / G) + threadIdx.x / G;
+    const int lane = threadIdx.x % G, slot = __builtin_amdgcn_readfirstlane(threadIdx.x / G);
+    const int V = (int)a.V, whole = V / N * N, tail = V - whole;
+    const int64_t row = (int64_t)blockIdx.x * (B / G) + slot;
     const bool live = row < a.N;
-    float w = 0.f;
-    if (live) w = a.weight ? a.weight[row] : 1.f;
+    const float w = live ? a.weight ? a.weight[row] : 1.f : 0.f;
     const bool on = live && w != 0.f;      // a row of weight zero is not looked at
     const T* z = (const T*)a.z + (live ? row : 0) * a.ld;
-    const T none = from_float<T>(-INFINITY);
     Piece<T> raw[NV];
-    if (on) {
+    const int here = on ? whole : 0;
 #pragma unroll
-        for (int v = 0; v < NV; ++v) raw[v] = load_piece(z, ((int64_t)v * G + lane) * N, a.V, none);
-    } else {
+    for (int v = 0; v < NV; ++v) {
+        const int at = (v * G + lane) * N;
+        if (at < here) {
+            const Raw16 x = *reinterpret_cast<const Raw16*>(z + at);
+            __builtin_memcpy(&raw[v], &x, 16);
+        } else {
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int j = 0; j < N; ++j) raw[v].e[j] = none;
+            for (int j = 0; j < 4; ++j) raw[v].w[j] = sizeof(T) == 4 ? kNegInf<T> : kNegInf<T> * 0x10001u;
+        }
     }
-    Teacher<T, G> te(lds + (threadIdx.x / G) * row_lds(a.K), a.K);
+    const float zt = on && lane < tail ? to_float(z[whole + lane]) : -INFINITY;
+    Teacher<T, G> te(lds + slot * row_lds(a.K), a.K);
     const float c2 = (float)(a.inv_tau * 1.4426950408889634);
-    float mx[2] = {-INFINITY, te.load(a, row, lane, on)};
+    float mx[2] = {zt, te.load(a, row, lane, on)};
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int j = 0; j < N; ++j) mx[0] = OpMax::f(mx[0], to_float(raw[v].e[j]));
+        for (int j = 0; j < N; ++j) mx[0] = OpMax::f(mx[0], raw[v].f(j));
     row_reduce<OpMax, G>(mx, shf, W, turn);
+    forget(raw);
     RowStat r;
     r.m = mx[0] == -INFINITY ? 0.f : mx[0];
     const float mt = mx[1] == -INFINITY ? 0.f : mx[1];
-    float s[2] = {0.f, a.lse ? 0.f : te.sum(mt, c2, lane)};
+    float s[2] = {__builtin_amdgcn_exp2f((zt - r.m) * c2), a.lse ? 0.f : te.sum(mt, c2, lane)};
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int j = 0; j < N; ++j) s[0] += __builtin_amdgcn_exp2f((to_float(raw[v].e[j]) - r.m) * c2);
+        for (int j = 0; j < N; ++j) s[0] += __builtin_amdgcn_exp2f((raw[v].f(j) - r.m) * c2);
     row_reduce<OpSum, G>(s, shf, W, turn);
     r.rs = s[0] > 0.f || s[0] != s[0] ? 1.f / s[0] : 0.f;
     const double lse_z = row_lse(r.m, s[0], a.inv_tau);
@@ -162,15 +166,22 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void row_kernel(Args a) {
         const float cp = on ? (float)(a.scale * (double)w) : 0.f, cq = on ? (float)(a.scale * (double)w * tl[0]) : 0.f;
         T* g = (T*)a.grad + (live ? row : 0) * a.ldg;
         const float f = cq * r.rs;
+        forget(raw);
         if (live) {
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                Piece<T> o;
+                const int at = (v * G + lane) * N;
+                float o[N];
 #pragma unroll
-                for (int j = 0; j < N; ++j)
-                    o.e[j] = from_float<T>(f * __builtin_amdgcn_exp2f((to_float(raw[v].e[j]) - r.m) * c2));
-                store_piece(g, ((int64_t)v * G + lane) * N, a.V, o);
+                for (int j = 0; j < N; ++j) o[j] = f * __builtin_amdgcn_exp2f((raw[v].f(j) - r.m) * c2);
+                const Piece<T> p = pack<T>(o);
+                if (at < whole) {
+                    Raw16 x;
+                    __builtin_memcpy(&x, &p, 16);
+                    *reinterpret_cast<Raw16*>(g + at) = x;
+                }
             }
+            if (lane < tail) g[whole + lane] = from_float<T>(f * __builtin_amdgcn_exp2f((zt - r.m) * c2));
         }
         __syncthreads();
         if (on) te.write(g, c2, r, cq, cp, lane);
@@ -190,25 +201,24 @@ __global__ __launch_bounds__(1024) void wide_kernel(Args a) {
     const float w = a.weight ? a.weight[row] : 1.f;
     const bool on = w != 0.f;
     const T* z = (const T*)a.z + row * a.ld;
-    const T none = from_float<T>(-INFINITY);
     Teacher<T, G> te(lds, a.K);
     const float c2 = (float)(a.inv_tau * 1.4426950408889634);
     float mx[2] = {-INFINITY, te.load(a, row, lane, on)}, part = 0.f;
     for (int64_t at = (int64_t)lane * N; on && at < a.V; at += (int64_t)U * G * N) {
         Piece<T> raw[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) raw[u] = load_piece(z, at + (int64_t)u * G * N, a.V, none);
+        for (int u = 0; u < U; ++u) raw[u] = load_piece(z, at + (int64_t)u * G * N, a.V, kNegInf<T>);
         float m = mx[0];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int j = 0; j < N; ++j) m = OpMax::f(m, to_float(raw[u].e[j]));
+            for (int j = 0; j < N; ++j) m = OpMax::f(m, raw[u].f(j));
         const float mm = m == -INFINITY ? 0.f : m;
         part *= __builtin_amdgcn_exp2f((mx[0] - mm) * c2);      // (0 at first: 0 * e^-inf)
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int j = 0; j < N; ++j) part += __builtin_amdgcn_exp2f((to_float(raw[u].e[j]) - mm) * c2);
+            for (int j = 0; j < N; ++j) part += __builtin_amdgcn_exp2f((raw[u].f(j) - mm) * c2);
         mx[0] = m;
     }
     const float own = mx[0];
@@ -233,14 +243,13 @@ __global__ __launch_bounds__(1024) void wide_kernel(Args a) {
         for (int64_t at = (int64_t)lane * N; at < a.V; at += (int64_t)U * G * N) {
             Piece<T> raw[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) raw[u] = load_piece(z, at + (int64_t)u * G * N, on ? a.V : 0, none);
+            for (int u = 0; u < U; ++u) raw[u] = load_piece(z, at + (int64_t)u * G * N, on ? a.V : 0, kNegInf<T>);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                Piece<T> o;
+                float o[N];
 #pragma unroll
-                for (int j = 0; j < N; ++j)
-                    o.e[j] = from_float<T>(f * __builtin_amdgcn_exp2f((to_float(raw[u].e[j]) - r.m) * c2));
-                store_piece(g, at + (int64_t)u * G * N, a.V, o);
+                for (int j = 0; j < N; ++j) o[j] = f * __builtin_amdgcn_exp2f((raw[u].f(j) - r.m) * c2);
+                store_piece(g, at + (int64_t)u * G * N, a.V, pack<T>(o));
             }
         }
         __syncthreads();
@@ -258,7 +267,7 @@ int launch_row(const Args& a, hipStream_t st) {
 
 template <typename T, bool GRAD>
 int launch(const Args& a, hipStream_t st) {
-    const int64_t n = (a.V + Piece<T>::kN - 1) / Piece<T>::kN;   // pieces of a row
+    const int64_t n = a.V / Piece<T>::kN;   // whole pieces of a row
     if (n <= 64) return launch_row<T, 64, 1, GRAD>(a, st);
     if (n <= 128) return launch_row<T, 64, 2, GRAD>(a, st);
     if (n <= 256) return launch_row<T, 64, 4, GRAD>(a, st);
@@ -276,7 +285,7 @@ int launch(const Args& a, hipStream_t st) {
 int distill(const char* who, const void* logits, int64_t ld, int dtype, int64_t N, int64_t V, const int32_t* idx,
             const float* teacher, int K, float tau, const float* lse, const float* weight, float scale, float* loss,
             void* grad, int64_t ldg, hipStream_t st) {
-    SAMX_REQUIRE(N >= 0 && N < (int64_t(1) << 31) && V > 0 && V < (int64_t(1) << 31), "%s: N %lld, V %lld out of range", who, (long long)N,
+    SAMX_REQUIRE(N >= 0 && N < (int64_t(1) << 31) && V > 0 && V < (int64_t(1) << 31) - 64, "%s: N %lld, V %lld out of range", who, (long long)N,
                  (long long)V);
     SAMX_REQUIRE(K > 0 && K <= SAMX_DISTILL_MAX_K, "%s: K %d must be in [1, %d]", who, K, SAMX_DISTILL_MAX_K);
     SAMX_REQUIRE(ld >= V && (!grad || ldg >= V), "%s: a row stride is shorter than V", who);

@@ -16,9 +16,8 @@
 // A chunk of 64 positions at a time, on the matrix cores: scores P = a b^T masked with l^{p-s}, out = P c + l^p a X,
 // X <- l^64 X + sum_s l^{64-s} b_s c_s^T.  X stays in the registers of the workgroup (float32; each wave owns whole
 // columns).  Operands of 16 bits enter the matrix cores as they are; P and the copy of X that meets a are rounded to
-// their type (an output of that type is rounded again), but l^{64-s} c_s is split into two numbers of the type, so that
-// the state, a float32 output, keeps 16 bits more than the type has.  float32 operands use the float32 matrix
-// instructions throughout.
+// their type (an output of that type is rounded again), but l^{64-s} c_s is split into numbers of the type whose sum it is,
+// so that the state, a float32 output, is one.  float32 operands use the float32 matrix instructions throughout.
 //
 // Where batch times heads is less than the device holds, time is cut into segments: kv_kernel makes each segment's own
 // contribution to the state behind it, join_kernel runs the recurrence over the segments, mix_kernel does the rest with
@@ -53,7 +52,7 @@ __device__ __forceinline__ f32x4 mma(const Piece<f16>& a, const Piece<f16>& b, f
 // (four instructions of 4 inner values: each takes the j-th of every lane, an order of the inner values that A and B share)
 __device__ __forceinline__ f32x4 mma(const Piece<float>& a, const Piece<float>& b, f32x4 d) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) d = __builtin_amdgcn_mfma_f32_16x16x4f32(a.e[j], b.e[j], d, 0, 0, 0);
+    for (int j = 0; j < 4; ++j) d = __builtin_amdgcn_mfma_f32_16x16x4f32(a.f(j), b.f(j), d, 0, 0, 0);
     return d;
 }
 
@@ -108,22 +107,53 @@ inline unsigned grid_of(const Args& a, int nseg) {
     return (unsigned)((units + 7) / 8 * 8 * a.roles);
 }
 
-// row 0 of a matrix of this place in the order of positions, and the step from one position to the next
-template <typename T>
+#define SAMX_GLOBAL __attribute__((address_space(1)))
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+
+// a matrix of this place in the order of positions: its row 0, the step from one position to the next.  EVEN: its rows
+// are whole pieces.  (The pointer says that it is one to global memory, which the compiler cannot see behind the choice
+// of a role: it would use the instructions that may also mean LDS.)
+template <typename T, bool EVEN>
 struct Rows {
-    const T* p; int64_t step; int dim;
-    __device__ Rows(const Mat& m, const Place& q, int rev) : dim(m.dim) {
-        p = (const T*)m.p + q.b * m.sb + (int64_t)(q.h / m.grp) * m.sh + (rev ? (q.L - 1) * m.st : 0);
-        step = rev ? -m.st : m.st;
+    static constexpr int kN = Piece<T>::kN;
+    const SAMX_GLOBAL char* p; int64_t step; int dim;
+    __device__ Rows(Mat m, Place q, int rev) : dim(m.dim) {
+        p = (const SAMX_GLOBAL char*)m.p + (int64_t)sizeof(T) * (q.b * m.sb + (int64_t)(q.h / m.grp) * m.sh + (rev ? (q.L - 1) * m.st : 0));
+        step = (int64_t)sizeof(T) * (rev ? -m.st : m.st);
     }
     // elements [at, at + kN) of position `pos`; zeros behind the row's end and where there is no such position
     __device__ __forceinline__ Piece<T> piece(int64_t pos, int at, bool there) const {
-        return load_piece(p + (there ? pos * step : 0), (int64_t)at, there ? dim : 0, from_float<T>(0.f));
+        Piece<T> r;
+        if constexpr (EVEN) {
+            there = there && at < dim;
+            const u32x4 v = *(const SAMX_GLOBAL u32x4_any*)(there ? p + pos * step + at * (int)sizeof(T) : p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r.w[j] = there ? v[j] : 0u;
+        } else {
+            const SAMX_GLOBAL char* e = p + (there ? pos * step : 0) + at * (int)sizeof(T);
+            const int n = there ? dim - at : 0;
+            if (n >= kN) {
+                const u32x4 v = *(const SAMX_GLOBAL u32x4_any*)e;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) r.w[j] = v[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if constexpr (sizeof(T) == 4) r.w[j] = j < n ? *(const SAMX_GLOBAL uint32_t*)(e + 4 * j) : 0u;
+                    else r.w[j] = (2 * j < n ? (uint32_t)*(const SAMX_GLOBAL uint16_t*)(e + 4 * j) : 0u) |
+                                  (2 * j + 1 < n ? (uint32_t)*(const SAMX_GLOBAL uint16_t*)(e + 4 * j + 2) : 0u) << 16;
+                }
+            }
+        }
+        return r;
     }
 };
 
 // 16 bytes, and 4 values, of LDS: every row and every column that comes here is a multiple of them
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 template <typename T>
 __device__ __forceinline__ Piece<T> lds_piece(const T* p) {
     const u32x4 v = *reinterpret_cast<const u32x4*>(p);
@@ -179,14 +209,16 @@ struct Staged {
     static constexpr int kPer = (2 * kBlocks + kThreads - 1) / kThreads;
     static constexpr bool kEven = 2 * kBlocks % kThreads == 0;
     Piece<T> r[kPer][kN];
-    __device__ __forceinline__ void load(const Rows<T>& b, const Rows<T>& c, int64_t base, int n) {
+    template <bool EVEN>
+    __device__ __forceinline__ void load(const Rows<T, EVEN>& b, const Rows<T, EVEN>& c, int64_t base, int n) {
 #pragma unroll
         for (int u = 0; u < kPer; ++u) {
             const int id = threadIdx.x + u * kThreads;
-            const bool second = id >= kBlocks;
+            const bool second = __builtin_amdgcn_readfirstlane(id) >= kBlocks;
             if (!kEven && id >= 2 * kBlocks) continue;
             const int k = second ? id - kBlocks : id, t0 = k % kTb * kN, d0 = k / kTb * kN;
-            const Rows<T>& m = second ? c : b;
+            Rows<T, EVEN> m = b;       // (kBlocks is a multiple of 64: the same for a whole wave)
+            if (second) m = c;
 #pragma unroll
             for (int i = 0; i < kN; ++i) r[u][i] = m.piece(base + t0 + i, d0, t0 + i < n);
         }
@@ -196,14 +228,17 @@ struct Staged {
 #pragma unroll
         for (int u = 0; u < kPer; ++u) {
             const int id = threadIdx.x + u * kThreads;
-            const bool second = id >= kBlocks;
+            const bool second = __builtin_amdgcn_readfirstlane(id) >= kBlocks;
             if (!kEven && id >= 2 * kBlocks) continue;
             const int k = second ? id - kBlocks : id, t0 = k % kTb * kN, d0 = k / kTb * kN;
 #pragma unroll
             for (int j = 0; j < kN; ++j) {
                 Piece<T> o;
 #pragma unroll
-                for (int i = 0; i < kN; ++i) o.e[i] = r[u][i].e[j];
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (sizeof(T) == 4) o.w[i] = r[u][i].w[j];
+                    else o.w[i] = __builtin_amdgcn_perm(r[u][2 * i + 1].w[j / 2], r[u][2 * i].w[j / 2], j & 1 ? 0x07060302u : 0x05040100u);
+                }
                 lds_put(second ? &l.ct[d0 + j][t0] : &l.bt[d0 + j][t0], o);
             }
         }
@@ -213,6 +248,10 @@ struct Staged {
 // X of a workgroup: wave w owns the tiles of 16 columns w, w + 4, ...; tile (i, j): lane l has column l % 16, rows
 // (l / 16) * 4 + [0, 4) of the a side
 template <int DP> struct State { static constexpr int kJ = DP / 64, kI = DP / 16; f32x4 x[kJ][kI]; };
+
+template <typename T> constexpr int kParts = 1;
+template <> inline constexpr int kParts<f16> = 2;
+template <> inline constexpr int kParts<bf16> = 3;
 
 // X <- l^end X + kv sum_s l^{end - s} b_s c_s^T
 template <typename T, int DP, typename L>
@@ -229,20 +268,26 @@ __device__ __forceinline__ void update(State<DP>& S, const L& l, int end, float 
         for (int k = 0; k < kChunk; k += 4 * kN) {
             const int s0 = k + q * kN;
             const Piece<T> c = lds_piece(&l.ct[(w + 4 * j) * 16 + r16][s0]);
-            Piece<T> hi, lo;
+            // l^{end - s} c_s in numbers of the type: one of float32, two of float16 (22 bits), three of bfloat16 (24)
+            float v[kN];
 #pragma unroll
             for (int e = 0; e < kN; ++e) {
                 const int n = end - s0 - e;
-                const float v = to_float(c.e[e]) * (kv * l.lam[n < 0 ? 0 : n]);   // (rows behind the end are zeros)
-                hi.e[e] = from_float<T>(v);
-                if constexpr (sizeof(T) == 2) lo.e[e] = from_float<T>(v - to_float(hi.e[e]));
+                v[e] = c.f(e) * (kv * l.lam[n < 0 ? 0 : n]);   // (rows behind the end are zeros)
+            }
+            Piece<T> part[kParts<T>];
+#pragma unroll
+            for (int u = 0; u < kParts<T>; ++u) {
+                part[u] = pack<T>(v);
+#pragma unroll
+                for (int e = 0; e < kN; ++e) v[e] -= part[u].f(e);
             }
 #pragma unroll
             for (int i = 0; i < State<DP>::kI; ++i) {
                 if (i >= na) continue;
                 const Piece<T> b = lds_piece(&l.bt[i * 16 + r16][s0]);
-                S.x[j][i] = mma(b, hi, S.x[j][i]);
-                if constexpr (sizeof(T) == 2) S.x[j][i] = mma(b, lo, S.x[j][i]);
+#pragma unroll
+                for (int u = 0; u < kParts<T>; ++u) S.x[j][i] = mma(b, part[u], S.x[j][i]);
             }
         }
     }
@@ -263,7 +308,7 @@ __device__ __forceinline__ void each(State<DP>& S, int da, int dc, F f) {
             }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool EVEN>
 __global__ __launch_bounds__(kThreads) void kv_kernel(Args A) {
     extern __shared__ __attribute__((aligned(16))) char lds_[];
     LdsKv<T, DP>& l = *reinterpret_cast<LdsKv<T, DP>*>(lds_);
@@ -271,8 +316,9 @@ __global__ __launch_bounds__(kThreads) void kv_kernel(Args A) {
     if (!place_of(A, A.nseg - 1, p)) return;
     const int64_t at = (int64_t)p.seg * A.seg_len;
     if (p.L <= at + A.seg_len) return;                  // nobody follows
-    const Role& r = A.r[p.role];
-    const Rows<T> b(r.b, p, r.rev), c(r.c, p, r.rev);
+    const Role r = A.r[p.role];
+    const int64_t seg_a = r.seg_a, seg_c = r.seg_c;
+    const Rows<T, EVEN> b(r.b, p, r.rev), c(r.c, p, r.rev);
     const int na = (r.b.dim + 15) / 16, nc = (r.c.dim + 15) / 16;
     if (threadIdx.x <= kChunk) l.lam[threadIdx.x] = power(p.g, threadIdx.x);
     State<DP> S;
@@ -289,8 +335,8 @@ __global__ __launch_bounds__(kThreads) void kv_kernel(Args A) {
         if (k + kChunk < A.seg_len) st.load(b, c, at + k + kChunk, kChunk);
         update<T, DP>(S, l, kChunk, r.kv, na, nc);
     }
-    float* out = r.seg + ((int64_t)(p.b * A.H + p.h) * (A.nseg - 1) + p.seg) * A.seg_size;
-    each<DP>(S, r.b.dim, r.c.dim, [&](int i, int j, float v) { return out[i * r.seg_a + j * r.seg_c] = v; });
+    SAMX_GLOBAL float* out = (SAMX_GLOBAL float*)r.seg + ((int64_t)(p.b * A.H + p.h) * (A.nseg - 1) + p.seg) * A.seg_size;
+    each<DP>(S, r.b.dim, r.c.dim, [=](int i, int j, float v) { return out[i * seg_a + j * seg_c] = v; });
 }
 
 // states at the segments' starts: X_{j+1} = l^len X_j + (segment j's own), over the segments that have a follower
@@ -314,54 +360,71 @@ __global__ __launch_bounds__(256) void join_kernel(Args A, int states) {
     }
 }
 
-template <typename T, int DP>
-__global__ __launch_bounds__(kThreads) void mix_kernel(Args A) {
+template <typename T, int DP, bool EVEN>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void mix_kernel(Args A) {
     constexpr int kN = Piece<T>::kN, kInner = 4 * kN;      // inner values of one mma
     extern __shared__ __attribute__((aligned(16))) char lds_[];
     Lds<T, DP>& l = *reinterpret_cast<Lds<T, DP>*>(lds_);
     Place p;
     if (!place_of(A, A.nseg, p)) return;
-    const Role& r = A.r[p.role];
+    // (by value: a reference into the arguments makes the compiler keep a copy of all of them in scratch memory)
+    const Role r = A.r[p.role];
+    const int64_t in_a = r.in_a, in_c = r.in_c, seg_a = r.seg_a, seg_c = r.seg_c;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
     const int64_t at = (int64_t)p.seg * A.seg_len, bh = (int64_t)p.b * A.H + p.h;
     const int64_t to = at + A.seg_len < p.L ? at + A.seg_len : p.L;         // this segment's positions
     const int da = r.a.dim, dc = r.c.dim, na = (da + 15) / 16, nc = (dc + 15) / 16;
     const int64_t out_row = (int64_t)A.H * dc;
-    T* out_t = (T*)r.out + ((int64_t)p.b * A.T * A.H + p.h) * dc;
-    float* out_f = (float*)r.out + ((int64_t)p.b * A.T * A.H + p.h) * dc;
+    const int64_t out_at = ((int64_t)p.b * A.T * A.H + p.h) * dc;
+    SAMX_GLOBAL char* const outp = (SAMX_GLOBAL char*)r.out + out_at * (r.out_f32 ? 4 : (int)sizeof(T));
+    // four of a row's outputs from d on, those that exist
+    auto put4 = [=](int64_t row, int d, f32x4 v) {
+        if (sizeof(T) == 4 || r.out_f32) {
+            SAMX_GLOBAL float* o = (SAMX_GLOBAL float*)outp + row * out_row + d;
+            if (EVEN) { if (d < dc) *(SAMX_GLOBAL f32x4_any*)o = v; return; }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (d + e < dc) o[e] = v[e];
+        } else if constexpr (sizeof(T) == 2) {
+            SAMX_GLOBAL uint16_t* o = (SAMX_GLOBAL uint16_t*)outp + row * out_row + d;
+            const uint32_t lo = pack2<T>(v[0], v[1]), hi = pack2<T>(v[2], v[3]);
+            if (EVEN) { if (d < dc) *(SAMX_GLOBAL u32x2_any*)o = u32x2{lo, hi}; return; }
+            if (d < dc) o[0] = (uint16_t)lo;
+            if (d + 1 < dc) o[1] = (uint16_t)(lo >> 16);
+            if (d + 2 < dc) o[2] = (uint16_t)hi;
+            if (d + 3 < dc) o[3] = (uint16_t)(hi >> 16);
+        }
+    };
     {   // rows behind the trajectory's end
         const int64_t z0 = at > p.L ? at : p.L, z1 = at + A.seg_len < A.T ? at + A.seg_len : A.T;
         for (int64_t t = z0 + threadIdx.x / 64; t < z1; t += 4)
-            for (int d = lane; d < dc; d += 64) {
-                if (r.out_f32) out_f[t * out_row + d] = 0.f;
-                else out_t[t * out_row + d] = from_float<T>(0.f);
-            }
+            for (int d = lane * 4; d < dc; d += 256) put4(t, d, f32x4{0.f, 0.f, 0.f, 0.f});
     }
     State<DP> S;
 #pragma unroll
     for (int j = 0; j < State<DP>::kJ; ++j)
 #pragma unroll
         for (int i = 0; i < State<DP>::kI; ++i) S.x[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const float* s_in = r.s_in ? r.s_in + bh * da * dc : nullptr;
-    float* s_out = r.s_out ? r.s_out + bh * da * dc : nullptr;
+    const SAMX_GLOBAL float* s_in = r.s_in ? (const SAMX_GLOBAL float*)r.s_in + bh * da * dc : nullptr;
+    SAMX_GLOBAL float* s_out = r.s_out ? (SAMX_GLOBAL float*)r.s_out + bh * da * dc : nullptr;
     if (p.L == 0) {    // nothing to read: the state goes through
         if (p.seg == 0 && s_out)
-            each<DP>(S, da, dc, [&](int i, int j, float) { return s_out[i * r.in_a + j * r.in_c] = s_in ? s_in[i * r.in_a + j * r.in_c] : 0.f; });
+            each<DP>(S, da, dc, [=](int i, int j, float) { return s_out[i * in_a + j * in_c] = s_in ? s_in[i * in_a + j * in_c] : 0.f; });
         return;
     }
     if (at >= to) return;
     const bool last = to == p.L;           // this segment makes the state behind the last position
     bool have = false;                     // X is not zero
     if (p.seg > 0) {
-        const float* s = r.seg + (bh * (A.nseg - 1) + p.seg - 1) * A.seg_size;
-        each<DP>(S, da, dc, [&](int i, int j, float) { return s[i * r.seg_a + j * r.seg_c]; });
+        const SAMX_GLOBAL float* s = (const SAMX_GLOBAL float*)r.seg + (bh * (A.nseg - 1) + p.seg - 1) * A.seg_size;
+        each<DP>(S, da, dc, [=](int i, int j, float) { return s[i * seg_a + j * seg_c]; });
         have = true;
     } else if (s_in) {
         const float f = r.rev ? 1.f : power(p.g, 1);
-        each<DP>(S, da, dc, [&](int i, int j, float) { return s_in[i * r.in_a + j * r.in_c] * f; });
+        each<DP>(S, da, dc, [=](int i, int j, float) { return s_in[i * in_a + j * in_c] * f; });
         have = true;
     }
-    const Rows<T> a(r.a, p, r.rev), b(r.b, p, r.rev), c(r.c, p, r.rev);
+    const Rows<T, EVEN> a(r.a, p, r.rev), b(r.b, p, r.rev), c(r.c, p, r.rev);
     if (threadIdx.x <= kChunk) l.lam[threadIdx.x] = power(p.g, threadIdx.x);
     auto keep = [&]() {                    // X's copy for the products with a
 #pragma unroll
@@ -427,13 +490,7 @@ __global__ __launch_bounds__(kThreads) void mix_kernel(Args A) {
                 if (k <= w * 16 + 15) o = mma(lds_piece(&l.ct[j * 16 + r16][k + q * kN]), lds_piece(&l.p[w][r16][k + q * kN]), o);
             if (row < n) {
                 const int64_t tok = r.rev ? p.L - 1 - (base + row) : base + row;
-                const int d = j * 16 + q * 4;
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (d + e < dc) {
-                        if (r.out_f32) out_f[tok * out_row + d + e] = o[e];
-                        else out_t[tok * out_row + d + e] = from_float<T>(o[e]);
-                    }
+                put4(tok, j * 16 + q * 4, o);
             }
         }
         if (more || (last && s_out)) {
@@ -446,7 +503,7 @@ __global__ __launch_bounds__(kThreads) void mix_kernel(Args A) {
             }
         }
     }
-    if (last && s_out) each<DP>(S, da, dc, [&](int i, int j, float v) { return s_out[i * r.in_a + j * r.in_c] = v; });
+    if (last && s_out) each<DP>(S, da, dc, [=](int i, int j, float v) { return s_out[i * in_a + j * in_c] = v; });
 }
 
 // sums of the query heads that share a key head: float32 [rows, HK, grp, dim] -> [rows, HK, dim] of the type
@@ -484,13 +541,14 @@ __global__ __launch_bounds__(256) void step_kernel(Mat Q, Mat K, Mat V, const fl
     __syncthreads();
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
     for (int i = threadIdx.x / lanes; i < D; i += rows) {
-        Piece<float> x = load_piece(s + (int64_t)i * DV, (int64_t)c, (int64_t)DV, 0.f);
+        const Piece<float> x = load_piece(s + (int64_t)i * DV, (int64_t)c, (int64_t)DV, 0u);
+        float y[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            x.e[e] = l * x.e[e] + sk[i] * ve[e];
-            acc[e] += sq[i] * x.e[e];
+            y[e] = l * x.f(e) + sk[i] * ve[e];
+            acc[e] += sq[i] * y[e];
         }
-        store_piece(s + (int64_t)i * DV, (int64_t)c, (int64_t)DV, x);
+        store_piece(s + (int64_t)i * DV, (int64_t)c, (int64_t)DV, pack<float>(y));
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) part[threadIdx.x * 4 + e] = acc[e];
@@ -525,30 +583,33 @@ void cut(Args& a) {
     if (a.nseg < 1) a.nseg = 1;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool EVEN>
 int launch(Args& a, const int (&joined)[2], int joins, hipStream_t st) {
     if (a.nseg > 1) {
         Args k = a;
         k.roles = joins;
         for (int i = 0; i < joins; ++i) k.r[i] = a.r[joined[i]];
         static samx::LdsGrant grant;
-        if (int rc = grant.ensure((const void*)kv_kernel<T, DP>, sizeof(LdsKv<T, DP>))) return rc;
-        kv_kernel<T, DP><<<grid_of(k, a.nseg - 1), kThreads, sizeof(LdsKv<T, DP>), st>>>(k);
+        if (int rc = grant.ensure((const void*)kv_kernel<T, DP, EVEN>, sizeof(LdsKv<T, DP>))) return rc;
+        kv_kernel<T, DP, EVEN><<<grid_of(k, a.nseg - 1), kThreads, sizeof(LdsKv<T, DP>), st>>>(k);
         SAMX_LAUNCH_CHECK();
         const int most = a.r[0].b.dim * a.r[0].c.dim;    // (the same product for every role)
         join_kernel<<<dim3((unsigned)((most + 255) / 256), (unsigned)(a.B * a.H), (unsigned)joins), 256, 0, st>>>(k, a.nseg - 1);
         SAMX_LAUNCH_CHECK();
     }
     static samx::LdsGrant grant;
-    if (int rc = grant.ensure((const void*)mix_kernel<T, DP>, sizeof(Lds<T, DP>))) return rc;
-    mix_kernel<T, DP><<<grid_of(a, a.nseg), kThreads, sizeof(Lds<T, DP>), st>>>(a);
+    if (int rc = grant.ensure((const void*)mix_kernel<T, DP, EVEN>, sizeof(Lds<T, DP>))) return rc;
+    mix_kernel<T, DP, EVEN><<<grid_of(a, a.nseg), kThreads, sizeof(Lds<T, DP>), st>>>(a);
     SAMX_LAUNCH_CHECK();
     return SAMX_OK;
 }
 
 template <typename T>
 int launch_dim(Args& a, int most, const int (&joined)[2], int joins, hipStream_t st) {
-    return most <= 64 ? launch<T, 64>(a, joined, joins, st) : launch<T, 128>(a, joined, joins, st);
+    const int n = Piece<T>::kN;
+    if (a.r[0].b.dim % n == 0 && a.r[0].c.dim % n == 0)
+        return most <= 64 ? launch<T, 64, true>(a, joined, joins, st) : launch<T, 128, true>(a, joined, joins, st);
+    return most <= 64 ? launch<T, 64, false>(a, joined, joins, st) : launch<T, 128, false>(a, joined, joins, st);
 }
 
 int launch_type(int dtype, Args& a, int most, const int (&joined)[2], int joins, hipStream_t st) {

@@ -31,21 +31,85 @@ template <> __device__ __forceinline__ bf16 from_float<bf16>(float x) {
 }
 template <> __device__ __forceinline__ f16 from_float<f16>(float x) { f16 r; r.v = (_Float16)x; return r; }
 
-// 16 bytes of a row.  gfx950 loads and stores them at any address, so a piece starts at a multiple of kN elements of
-// its row whatever the row's own alignment is.
-template <typename T> struct Piece { static constexpr int kN = 16 / (int)sizeof(T); T e[kN]; };
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// two values rounded to 16 bits each, the first in the low half
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<bf16>(float a, float b) {
+    const bf16x2 v = __builtin_convertvector((f32x2){a, b}, bf16x2);
+    uint32_t r;
+    __builtin_memcpy(&r, &v, 4);
+    return r;
+}
+template <> __device__ __forceinline__ uint32_t pack2<f16>(float a, float b) {
+    const f16x2 v = __builtin_convertvector((f32x2){a, b}, f16x2);
+    uint32_t r;
+    __builtin_memcpy(&r, &v, 4);
+    return r;
+}
+
+// 16 bytes of a row, packed as they lie there.  gfx950 loads and stores them at any address, so a piece starts at a
+// multiple of kN elements of its row whatever the row's own alignment is.
+template <typename T>
+struct Piece {
+    static constexpr int kN = 16 / (int)sizeof(T);
+    uint32_t w[4];
+    __device__ __forceinline__ uint32_t bits(int j) const {
+        if constexpr (sizeof(T) == 4) return w[j];
+        else return j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu;
+    }
+    __device__ __forceinline__ float f(int j) const;
+};
+template <> __device__ __forceinline__ float Piece<float>::f(int j) const { return __uint_as_float(w[j]); }
+template <> __device__ __forceinline__ float Piece<bf16>::f(int j) const {
+    return __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+}
+template <> __device__ __forceinline__ float Piece<f16>::f(int j) const {
+    const uint16_t u = (uint16_t)bits(j);
+    _Float16 h;
+    __builtin_memcpy(&h, &u, 2);
+    return (float)h;
+}
 struct Raw16 { uint32_t w[4]; } __attribute__((packed, aligned(2)));
 
-// elements [at, at + kN) of a row of n, `fill` where there are none
+// kN values, each rounded once (two of 16 bits by one instruction)
 template <typename T>
-__device__ __forceinline__ Piece<T> load_piece(const T* row, int64_t at, int64_t n, T fill) {
+__device__ __forceinline__ Piece<T> pack(const float* v) {
+    Piece<T> p;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p.w[j] = __float_as_uint(v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p.w[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
+    }
+    return p;
+}
+
+template <typename T> __device__ __forceinline__ uint32_t element_bits(const T* p) {
+    if constexpr (sizeof(T) == 4) return *reinterpret_cast<const uint32_t*>(p);
+    else return *reinterpret_cast<const uint16_t*>(p);
+}
+
+// elements [at, at + kN) of a row of n; where there are none the element whose bits are `fill`
+template <typename T>
+__device__ __forceinline__ Piece<T> load_piece(const T* row, int64_t at, int64_t n, uint32_t fill) {
     Piece<T> p;
     if (at + Piece<T>::kN <= n) {
         const Raw16 r = *reinterpret_cast<const Raw16*>(row + at);
         __builtin_memcpy(&p, &r, 16);
     } else {
 #pragma unroll
-        for (int j = 0; j < Piece<T>::kN; ++j) p.e[j] = at + j < n ? row[at + j] : fill;
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (sizeof(T) == 4) {
+                p.w[j] = at + j < n ? element_bits(row + at + j) : fill;
+            } else {
+                const int64_t i = at + 2 * j;
+                p.w[j] = (i < n ? element_bits(row + i) : fill) | (i + 1 < n ? element_bits(row + i + 1) : fill) << 16;
+            }
+        }
     }
     return p;
 }
@@ -59,9 +123,26 @@ __device__ __forceinline__ void store_piece(T* row, int64_t at, int64_t n, const
     } else {
 #pragma unroll
         for (int j = 0; j < Piece<T>::kN; ++j)
-            if (at + j < n) row[at + j] = p.e[j];
+            if (at + j < n) {
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(row + at + j) = p.w[j];
+                else *reinterpret_cast<uint16_t*>(row + at + j) = (uint16_t)p.bits(j);
+            }
     }
 }
+
+// The compiler is not to keep what it has computed from the pieces so far: they are unpacked again where they are used
+// next, which costs an instruction a value instead of a register.
+template <typename T, int N>
+__device__ __forceinline__ void forget(Piece<T> (&p)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(p[i].w[j]));
+}
+
+// minus infinity of a type
+template <typename T> constexpr uint32_t kNegInf = sizeof(T) == 4 ? 0xff800000u : 0xff80u;
+template <> inline constexpr uint32_t kNegInf<f16> = 0xfc00u;
 
 struct OpSum { template <typename V> static __device__ __forceinline__ V f(V a, V b) { return a + b; } };
 struct OpMax { template <typename V> static __device__ __forceinline__ V f(V a, V b) { return a > b ? a : b; } };
@@ -90,13 +171,23 @@ __device__ __forceinline__ void row_reduce(V (&v)[C], V* sh, int waves, int& tur
 #pragma unroll
             for (int c = 0; c < C; ++c) mine[wave * C + c] = v[c];
         __syncthreads();
-        const int first = wave / (G / 64) * (G / 64);
+        constexpr int K = G / 64;
+        const int first = wave / K * K;
+        if constexpr (sizeof(V) == 4 && (C & (C - 1)) == 0 && K * C <= 64) {
+            // one value a lane, reduced over the waves by lanes: the row's results come out of one register
+            V t = mine[first * C + (threadIdx.x & (K * C - 1))];
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            V t = mine[first * C + c];
+            for (int o = C; o < K * C; o <<= 1) t = Op::f(t, __shfl_xor(t, o, 64));
 #pragma unroll
-            for (int w = 1; w < G / 64; ++w) t = Op::f(t, mine[(first + w) * C + c]);
-            v[c] = t;
+            for (int c = 0; c < C; ++c) v[c] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(t), c));
+        } else {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                V t = mine[first * C + c];
+#pragma unroll
+                for (int w = 1; w < K; ++w) t = Op::f(t, mine[(first + w) * C + c]);
+                v[c] = t;
+            }
         }
     }
 }
