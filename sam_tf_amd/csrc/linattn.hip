@@ -64,9 +64,9 @@ struct Role {
     void* out; int out_f32;                    // [B, T, H, c.dim] dense, of the type or float32
     int rev;
     float kv, ps, so;                          // factors: of b c^T in the state, of the scores, of a X
-    const float* s_in; int64_t in_a, in_c;     // state before the first position, strides of a state's element (a, c)
+    const float* s_in; int in_a, in_c;     // state before the first position, strides of a state's element (a, c)
     float* s_out;                              // state behind the last, strides as s_in's
-    float* seg; int64_t seg_a, seg_c;          // states at the segments' starts (workspace)
+    float* seg; int turned;                    // states at the segments' starts (workspace); turned: another role's, transposed
 };
 
 struct Args {
@@ -170,12 +170,26 @@ __device__ __forceinline__ void lds_put(T* p, const Piece<T>& r) {
 __device__ __forceinline__ void lds_put4(float* p, const float (&v)[4]) { *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]}; }
 template <typename T>
 __device__ __forceinline__ void lds_put4(T* p, const float (&v)[4]) {
-    struct { T e[4]; } o;
+    *reinterpret_cast<u32x2*>(p) = u32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+}
+// A piece down a column: elements [0, kN) are rows[e][lane % 16].  16 bits: two transposing reads, in each of which 16
+// lanes read 4 rows of 16 values and get a column each; with 4-byte values a read for each row.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+template <typename T>
+__device__ __forceinline__ Piece<T> lds_column(const T* rows, int stride) {
+    const int r16 = threadIdx.x & 15;
+    Piece<T> r;
+    if constexpr (sizeof(T) == 2) {
+        const T* p = rows + (r16 >> 2) * stride + (r16 & 3) * 4;
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * stride));
+        __builtin_memcpy(&r.w[0], &a, 8);
+        __builtin_memcpy(&r.w[2], &b, 8);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o.e[e] = from_float<T>(v[e]);
-    uint64_t u;
-    __builtin_memcpy(&u, &o, 8);
-    *reinterpret_cast<uint64_t*>(p) = u;
+        for (int e = 0; e < 4; ++e) r.w[e] = __float_as_uint(rows[e * stride + r16]);
+    }
+    return r;
 }
 // what the lanes of a wave have written to LDS is there for the others of the wave
 __device__ __forceinline__ void wave_sync() {
@@ -186,116 +200,108 @@ __device__ __forceinline__ void wave_sync() {
 
 // LDS rows are 16 bytes longer than their contents: 16 lanes that read 16 rows at one column use all banks
 template <typename T, int DP>
-struct Lds {
-    static constexpr int kN = Piece<T>::kN, kTok = kChunk + kN, kRow = DP + kN;
-    T bt[DP][kTok];          // b, c of the chunk, a row for each of their dimensions
-    T ct[DP][kTok];
-    T p[4][16][kTok];        // each wave's 16 rows of scores
-    T x[DP][kRow];           // X, a row for each column
-    float lam[kChunk + 1];   // l^n
+struct LdsKv {
+    static constexpr int kRow = DP + Piece<T>::kN;
+    T b[kChunk][kRow], c[kChunk][kRow];                  // the chunk's rows
+    float lam[kChunk + 4];                               // l^n
 };
 template <typename T, int DP>
-struct LdsKv {
-    static constexpr int kN = Piece<T>::kN, kTok = kChunk + kN;
-    T bt[DP][kTok];
-    T ct[DP][kTok];
-    float lam[kChunk + 1];
+struct Lds : LdsKv<T, DP> {
+    static constexpr int kTok = kChunk + Piece<T>::kN;
+    T p[4][16][kTok];                                    // each wave's 16 rows of scores
+    T x[DP][LdsKv<T, DP>::kRow];                         // X, a row for each column
 };
 
-// A chunk's rows of b and c on their way to LDS: blocks of kN positions by kN dimensions, transposed in registers
+// A chunk's rows of b and c on their way to LDS
 template <typename T, int DP>
 struct Staged {
-    static constexpr int kN = Piece<T>::kN, kTb = kChunk / kN, kBlocks = kTb * (DP / kN);   // blocks of one matrix
-    static constexpr int kPer = (2 * kBlocks + kThreads - 1) / kThreads;
-    static constexpr bool kEven = 2 * kBlocks % kThreads == 0;
-    Piece<T> r[kPer][kN];
+    static constexpr int kN = Piece<T>::kN, kAcross = DP / kN, kDown = kThreads / kAcross, kPer = kChunk / kDown;
+    Piece<T> b[kPer], c[kPer];
     template <bool EVEN>
-    __device__ __forceinline__ void load(const Rows<T, EVEN>& b, const Rows<T, EVEN>& c, int64_t base, int n) {
+    __device__ __forceinline__ void load(const Rows<T, EVEN>& mb, const Rows<T, EVEN>& mc, int64_t base, int n) {
+        const int t = threadIdx.x / kAcross, d = threadIdx.x % kAcross * kN;
 #pragma unroll
-        for (int u = 0; u < kPer; ++u) {
-            const int id = threadIdx.x + u * kThreads;
-            const bool second = __builtin_amdgcn_readfirstlane(id) >= kBlocks;
-            if (!kEven && id >= 2 * kBlocks) continue;
-            const int k = second ? id - kBlocks : id, t0 = k % kTb * kN, d0 = k / kTb * kN;
-            Rows<T, EVEN> m = b;       // (kBlocks is a multiple of 64: the same for a whole wave)
-            if (second) m = c;
+        for (int u = 0; u < kPer; ++u) b[u] = mb.piece(base + t + u * kDown, d, t + u * kDown < n);
 #pragma unroll
-            for (int i = 0; i < kN; ++i) r[u][i] = m.piece(base + t0 + i, d0, t0 + i < n);
-        }
+        for (int u = 0; u < kPer; ++u) c[u] = mc.piece(base + t + u * kDown, d, t + u * kDown < n);
     }
     template <typename L>
     __device__ __forceinline__ void store(L& l) const {
+        const int t = threadIdx.x / kAcross, d = threadIdx.x % kAcross * kN;
 #pragma unroll
         for (int u = 0; u < kPer; ++u) {
-            const int id = threadIdx.x + u * kThreads;
-            const bool second = __builtin_amdgcn_readfirstlane(id) >= kBlocks;
-            if (!kEven && id >= 2 * kBlocks) continue;
-            const int k = second ? id - kBlocks : id, t0 = k % kTb * kN, d0 = k / kTb * kN;
-#pragma unroll
-            for (int j = 0; j < kN; ++j) {
-                Piece<T> o;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (sizeof(T) == 4) o.w[i] = r[u][i].w[j];
-                    else o.w[i] = __builtin_amdgcn_perm(r[u][2 * i + 1].w[j / 2], r[u][2 * i].w[j / 2], j & 1 ? 0x07060302u : 0x05040100u);
-                }
-                lds_put(second ? &l.ct[d0 + j][t0] : &l.bt[d0 + j][t0], o);
-            }
+            lds_put(&l.b[t + u * kDown][d], b[u]);
+            lds_put(&l.c[t + u * kDown][d], c[u]);
         }
     }
 };
 
-// X of a workgroup: wave w owns the tiles of 16 columns w, w + 4, ...; tile (i, j): lane l has column l % 16, rows
+// X of a workgroup: wave w owns the tiles of 16 columns w, w + 4, ...; tile (j, i): lane l has column l % 16, rows
 // (l / 16) * 4 + [0, 4) of the a side
-template <int DP> struct State { static constexpr int kJ = DP / 64, kI = DP / 16; f32x4 x[kJ][kI]; };
+template <int DP>
+struct State {
+    static constexpr int kJ = DP / 64, kI = DP / 16;
+    f32x4 x[kJ][kI];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int j = 0; j < kJ; ++j)
+#pragma unroll
+            for (int i = 0; i < kI; ++i) x[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+};
 
+// numbers of the type whose sum a float32 is
 template <typename T> constexpr int kParts = 1;
 template <> inline constexpr int kParts<f16> = 2;
 template <> inline constexpr int kParts<bf16> = 3;
 
-// X <- l^end X + kv sum_s l^{end - s} b_s c_s^T
+// X <- l^end X + kv sum_s l^{end - s} b_s c_s^T, with l^{end - s} c_s in as many numbers of the type as it has
 template <typename T, int DP, typename L>
-__device__ __forceinline__ void update(State<DP>& S, const L& l, int end, float kv, int na, int nc) {
-    constexpr int kN = Piece<T>::kN;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
+__device__ __forceinline__ void update(State<DP>& S, const L& l, int end, float kv) {
+    constexpr int kN = Piece<T>::kN, kJ = State<DP>::kJ, kI = State<DP>::kI, kP = kParts<T>;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane >> 4;
     const float whole = l.lam[end];
 #pragma unroll
-    for (int j = 0; j < State<DP>::kJ; ++j) {
-        if (w + 4 * j >= nc) continue;
+    for (int j = 0; j < kJ; ++j)
 #pragma unroll
-        for (int i = 0; i < State<DP>::kI; ++i) S.x[j][i] *= whole;
+        for (int i = 0; i < kI; ++i) S.x[j][i] *= whole;
 #pragma unroll
-        for (int k = 0; k < kChunk; k += 4 * kN) {
-            const int s0 = k + q * kN;
-            const Piece<T> c = lds_piece(&l.ct[(w + 4 * j) * 16 + r16][s0]);
-            // l^{end - s} c_s in numbers of the type: one of float32, two of float16 (22 bits), three of bfloat16 (24)
+    for (int k = 0; k < kChunk; k += 4 * kN) {
+        const int s0 = k + q * kN;
+        float f[kN];
+#pragma unroll
+        for (int e = 0; e < kN; ++e) {
+            const int n = end - s0 - e;
+            f[e] = kv * l.lam[n < 0 ? 0 : n];   // (rows behind the end are zeros)
+        }
+        Piece<T> part[kJ][kP];
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) {
+            const Piece<T> c = lds_column(&l.c[s0][(w + 4 * j) * 16], L::kRow);
             float v[kN];
 #pragma unroll
-            for (int e = 0; e < kN; ++e) {
-                const int n = end - s0 - e;
-                v[e] = c.f(e) * (kv * l.lam[n < 0 ? 0 : n]);   // (rows behind the end are zeros)
+            for (int e = 0; e < kN; ++e) v[e] = c.f(e) * f[e];
+#pragma unroll
+            for (int u = 0; u < kP; ++u) {
+                part[j][u] = pack<T>(v);
+#pragma unroll
+                for (int e = 0; e < kN; ++e) v[e] -= part[j][u].f(e);
             }
-            Piece<T> part[kParts<T>];
+        }
 #pragma unroll
-            for (int u = 0; u < kParts<T>; ++u) {
-                part[u] = pack<T>(v);
+        for (int i = 0; i < kI; ++i) {
+            const Piece<T> b = lds_column(&l.b[s0][i * 16], L::kRow);
 #pragma unroll
-                for (int e = 0; e < kN; ++e) v[e] -= part[u].f(e);
-            }
+            for (int j = 0; j < kJ; ++j)
 #pragma unroll
-            for (int i = 0; i < State<DP>::kI; ++i) {
-                if (i >= na) continue;
-                const Piece<T> b = lds_piece(&l.bt[i * 16 + r16][s0]);
-#pragma unroll
-                for (int u = 0; u < kParts<T>; ++u) S.x[j][i] = mma(b, part[u], S.x[j][i]);
-            }
+                for (int u = 0; u < kP; ++u) S.x[j][i] = mma(b, part[j][u], S.x[j][i]);
         }
     }
 }
 
-// a state's elements that exist: X(a, c) <- f(a, c, X(a, c))
-template <int DP, typename F>
-__device__ __forceinline__ void each(State<DP>& S, int da, int dc, F f) {
+// A caller's state, [da, dc] values with the strides sa, sc: to and from a workgroup's registers.
+template <int DP>
+__device__ __forceinline__ void state_load(State<DP>& S, const SAMX_GLOBAL float* m, int da, int dc, int sa, int sc, float f) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
 #pragma unroll
     for (int j = 0; j < State<DP>::kJ; ++j)
@@ -304,12 +310,53 @@ __device__ __forceinline__ void each(State<DP>& S, int da, int dc, F f) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int c = (w + 4 * j) * 16 + r16, a = i * 16 + q * 4 + e;
-                if (a < da && c < dc) S.x[j][i][e] = f(a, c, S.x[j][i][e]);
+                const bool there = a < da && c < dc;
+                const float v = m[(uint32_t)(there ? a * sa + c * sc : 0)];      // (no branch: the loads go out together)
+                S.x[j][i][e] = there ? v * f : 0.f;
             }
+}
+template <int DP>
+__device__ __forceinline__ void state_store(const State<DP>& S, SAMX_GLOBAL float* m, int da, int dc, int sa, int sc) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < State<DP>::kJ; ++j)
+#pragma unroll
+        for (int i = 0; i < State<DP>::kI; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int c = (w + 4 * j) * 16 + r16, a = i * 16 + q * 4 + e;
+                if (a < da && c < dc) m[(uint32_t)(a * sa + c * sc)] = S.x[j][i][e];
+            }
+}
+// A segment's state in the workspace: all tiles, [columns][rows] dense; `turned`: the matrix that is wanted is its transpose.
+template <int DP>
+__device__ __forceinline__ void seg_load(State<DP>& S, const SAMX_GLOBAL float* m, bool turned) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < State<DP>::kJ; ++j)
+#pragma unroll
+        for (int i = 0; i < State<DP>::kI; ++i) {
+            const uint32_t c = (w + 4 * j) * 16 + r16, a = i * 16 + q * 4;
+            if (!turned) {
+                S.x[j][i] = *(const SAMX_GLOBAL f32x4*)(m + c * DP + a);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) S.x[j][i][e] = m[(a + e) * DP + c];
+            }
+        }
+}
+template <int DP>
+__device__ __forceinline__ void seg_store(const State<DP>& S, SAMX_GLOBAL float* m) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < State<DP>::kJ; ++j)
+#pragma unroll
+        for (int i = 0; i < State<DP>::kI; ++i)
+            *(SAMX_GLOBAL f32x4*)(m + (uint32_t)(((w + 4 * j) * 16 + r16) * DP + i * 16 + q * 4)) = S.x[j][i];
 }
 
 template <typename T, int DP, bool EVEN>
-__global__ __launch_bounds__(kThreads) void kv_kernel(Args A) {
+__global__ __launch_bounds__(kThreads, 2) void kv_kernel(Args A) {
     extern __shared__ __attribute__((aligned(16))) char lds_[];
     LdsKv<T, DP>& l = *reinterpret_cast<LdsKv<T, DP>*>(lds_);
     Place p;
@@ -317,15 +364,10 @@ __global__ __launch_bounds__(kThreads) void kv_kernel(Args A) {
     const int64_t at = (int64_t)p.seg * A.seg_len;
     if (p.L <= at + A.seg_len) return;                  // nobody follows
     const Role r = A.r[p.role];
-    const int64_t seg_a = r.seg_a, seg_c = r.seg_c;
     const Rows<T, EVEN> b(r.b, p, r.rev), c(r.c, p, r.rev);
-    const int na = (r.b.dim + 15) / 16, nc = (r.c.dim + 15) / 16;
     if (threadIdx.x <= kChunk) l.lam[threadIdx.x] = power(p.g, threadIdx.x);
     State<DP> S;
-#pragma unroll
-    for (int j = 0; j < State<DP>::kJ; ++j)
-#pragma unroll
-        for (int i = 0; i < State<DP>::kI; ++i) S.x[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    S.zero();
     Staged<T, DP> st;
     st.load(b, c, at, kChunk);
     for (int64_t k = 0; k < A.seg_len; k += kChunk) {
@@ -333,47 +375,55 @@ __global__ __launch_bounds__(kThreads) void kv_kernel(Args A) {
         st.store(l);
         __syncthreads();
         if (k + kChunk < A.seg_len) st.load(b, c, at + k + kChunk, kChunk);
-        update<T, DP>(S, l, kChunk, r.kv, na, nc);
+        update<T, DP>(S, l, kChunk, r.kv);
     }
-    SAMX_GLOBAL float* out = (SAMX_GLOBAL float*)r.seg + ((int64_t)(p.b * A.H + p.h) * (A.nseg - 1) + p.seg) * A.seg_size;
-    each<DP>(S, r.b.dim, r.c.dim, [=](int i, int j, float v) { return out[i * seg_a + j * seg_c] = v; });
+    seg_store<DP>(S, (SAMX_GLOBAL float*)r.seg + ((int64_t)(p.b * A.H + p.h) * (A.nseg - 1) + p.seg) * A.seg_size);
 }
 
 // states at the segments' starts: X_{j+1} = l^len X_j + (segment j's own), over the segments that have a follower
-__global__ __launch_bounds__(256) void join_kernel(Args A, int states) {
+template <int DP>
+__global__ __launch_bounds__(256) void join_kernel(Args A) {
+    constexpr int U = 8;
     const Role& r = A.r[blockIdx.z];
     const int64_t bh = blockIdx.y;
-    const int e = blockIdx.x * 256 + threadIdx.x, na = r.b.dim, nc = r.c.dim;
-    if (e >= na * nc) return;
+    const int e = blockIdx.x * 256 + threadIdx.x, na = r.b.dim, nc = r.c.dim, states = A.nseg - 1;
     const int b = (int)(bh / A.H), h = (int)(bh % A.H);
     int64_t L = A.T;
     if (A.lengths) L = A.lengths[b] < A.T ? A.lengths[b] : A.T;
-    // the fast index is the one that lies dense in the workspace
-    const int i = e % na, j = e / na;
+    const int i = e % DP, j = e / DP;
+    if (i >= na || j >= nc) return;       // (kv_kernel has left zeros there)
     const float g = A.decay[h], f = power(g, A.seg_len);
     float x = 0.f;
     if (r.s_in) x = r.s_in[bh * na * nc + i * r.in_a + j * r.in_c] * (r.rev ? 1.f : power(g, 1));
-    float* s = r.seg + bh * states * A.seg_size + i * r.seg_a + j * r.seg_c;
-    for (int k = 0; k < states && (int64_t)(k + 1) * A.seg_len < L; ++k) {
-        x = f * x + s[k * A.seg_size];
-        s[k * A.seg_size] = x;
+    float* s = r.seg + bh * states * A.seg_size + e;
+    int n = 0;                                          // states that are wanted
+    while (n < states && (int64_t)(n + 1) * A.seg_len < L) ++n;
+    for (int k = 0; k < n; k += U) {
+        float v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = k + u < n ? s[(int64_t)(k + u) * A.seg_size] : 0.f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            x = f * x + v[u];
+            if (k + u < n) s[(int64_t)(k + u) * A.seg_size] = x;
+        }
     }
 }
 
 template <typename T, int DP, bool EVEN>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void mix_kernel(Args A) {
-    constexpr int kN = Piece<T>::kN, kInner = 4 * kN;      // inner values of one mma
+    constexpr int kN = Piece<T>::kN, kInner = 4 * kN, kK = DP / kInner;      // inner values of one mma
     extern __shared__ __attribute__((aligned(16))) char lds_[];
     Lds<T, DP>& l = *reinterpret_cast<Lds<T, DP>*>(lds_);
+    constexpr int kRow = LdsKv<T, DP>::kRow;
     Place p;
     if (!place_of(A, A.nseg, p)) return;
     // (by value: a reference into the arguments makes the compiler keep a copy of all of them in scratch memory)
     const Role r = A.r[p.role];
-    const int64_t in_a = r.in_a, in_c = r.in_c, seg_a = r.seg_a, seg_c = r.seg_c;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
     const int64_t at = (int64_t)p.seg * A.seg_len, bh = (int64_t)p.b * A.H + p.h;
     const int64_t to = at + A.seg_len < p.L ? at + A.seg_len : p.L;         // this segment's positions
-    const int da = r.a.dim, dc = r.c.dim, na = (da + 15) / 16, nc = (dc + 15) / 16;
+    const int da = r.a.dim, dc = r.c.dim;
     const int64_t out_row = (int64_t)A.H * dc;
     const int64_t out_at = ((int64_t)p.b * A.T * A.H + p.h) * dc;
     SAMX_GLOBAL char* const outp = (SAMX_GLOBAL char*)r.out + out_at * (r.out_f32 ? 4 : (int)sizeof(T));
@@ -401,109 +451,86 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void mix_kernel(A
             for (int d = lane * 4; d < dc; d += 256) put4(t, d, f32x4{0.f, 0.f, 0.f, 0.f});
     }
     State<DP> S;
-#pragma unroll
-    for (int j = 0; j < State<DP>::kJ; ++j)
-#pragma unroll
-        for (int i = 0; i < State<DP>::kI; ++i) S.x[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     const SAMX_GLOBAL float* s_in = r.s_in ? (const SAMX_GLOBAL float*)r.s_in + bh * da * dc : nullptr;
     SAMX_GLOBAL float* s_out = r.s_out ? (SAMX_GLOBAL float*)r.s_out + bh * da * dc : nullptr;
     if (p.L == 0) {    // nothing to read: the state goes through
-        if (p.seg == 0 && s_out)
-            each<DP>(S, da, dc, [=](int i, int j, float) { return s_out[i * in_a + j * in_c] = s_in ? s_in[i * in_a + j * in_c] : 0.f; });
+        if (p.seg == 0 && s_out) {
+            if (s_in) state_load<DP>(S, s_in, da, dc, r.in_a, r.in_c, 1.f);
+            else S.zero();
+            state_store<DP>(S, s_out, da, dc, r.in_a, r.in_c);
+        }
         return;
     }
     if (at >= to) return;
-    const bool last = to == p.L;           // this segment makes the state behind the last position
-    bool have = false;                     // X is not zero
-    if (p.seg > 0) {
-        const SAMX_GLOBAL float* s = (const SAMX_GLOBAL float*)r.seg + (bh * (A.nseg - 1) + p.seg - 1) * A.seg_size;
-        each<DP>(S, da, dc, [=](int i, int j, float) { return s[i * seg_a + j * seg_c]; });
-        have = true;
-    } else if (s_in) {
-        const float f = r.rev ? 1.f : power(p.g, 1);
-        each<DP>(S, da, dc, [=](int i, int j, float) { return s_in[i * in_a + j * in_c] * f; });
-        have = true;
-    }
     const Rows<T, EVEN> a(r.a, p, r.rev), b(r.b, p, r.rev), c(r.c, p, r.rev);
-    if (threadIdx.x <= kChunk) l.lam[threadIdx.x] = power(p.g, threadIdx.x);
-    auto keep = [&]() {                    // X's copy for the products with a
+    const int row = w * 16 + r16;          // of a chunk: this lane's
+    Staged<T, DP> st;
+    Piece<T> af[kK], an[kK];               // a's rows of this wave, whole: the chunk's, the next one's
+    auto fetch = [&](int64_t base) {
+        const int n = (int)(to - base < kChunk ? to - base : kChunk);
+        st.load(b, c, base, n);
 #pragma unroll
-        for (int j = 0; j < State<DP>::kJ; ++j)
+        for (int k = 0; k < kK; ++k) an[k] = a.piece(base + row, k * kInner + q * kN, row < n);
+    };
+    fetch(at);
+    const bool last = to == p.L;           // this segment makes the state behind the last position
+    if (p.seg > 0) seg_load<DP>(S, (const SAMX_GLOBAL float*)r.seg + (bh * (A.nseg - 1) + p.seg - 1) * A.seg_size, r.turned);
+    else if (s_in) state_load<DP>(S, s_in, da, dc, r.in_a, r.in_c, r.rev ? 1.f : power(p.g, 1));
+    else S.zero();
+    if (threadIdx.x <= kChunk) l.lam[threadIdx.x] = power(p.g, threadIdx.x);
+    for (int64_t base = at; base < to; base += kChunk) {
+        const int n = (int)(to - base < kChunk ? to - base : kChunk);
+        const bool more = base + kChunk < to;
+        st.store(l);
+#pragma unroll
+        for (int j = 0; j < State<DP>::kJ; ++j)          // X's copy for the products with a
 #pragma unroll
             for (int i = 0; i < State<DP>::kI; ++i) {
                 const float v[4] = {S.x[j][i][0], S.x[j][i][1], S.x[j][i][2], S.x[j][i][3]};
                 lds_put4(&l.x[(w + 4 * j) * 16 + r16][i * 16 + q * 4], v);
             }
-    };
-    if (have) keep();
-    Staged<T, DP> st;
-    st.load(b, c, at, (int)(to - at < kChunk ? to - at : kChunk));
-    for (int64_t base = at; base < to; base += kChunk) {
-        const int n = (int)(to - base < kChunk ? to - base : kChunk);
-        const bool more = base + kChunk < to;
-        __syncthreads();                   // the chunk before is done with
-        st.store(l);
-        // a's rows of this wave, whole
-        const int row = w * 16 + r16;
-        Piece<T> af[DP / kInner];
 #pragma unroll
-        for (int k = 0; k < DP / kInner; ++k)
-            if (k * kInner < da) af[k] = a.piece(base + row, k * kInner + q * kN, row < n);
-        // scores, transposed: column = this wave's row, rows = positions s
-        f32x4 sc[4];
-#pragma unroll
+        for (int k = 0; k < kK; ++k) af[k] = an[k];
+        __syncthreads();
+        if (more) fetch(base + kChunk);
+        // scores, transposed: column = this wave's row, rows = positions s; masked and decayed
+#pragma unroll 2
         for (int t = 0; t < 4; ++t) {
-            sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (t > w) continue;
-            const int s = t * 16 + r16;
+            f32x4 sc = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (t <= w) {
 #pragma unroll
-            for (int k = 0; k < DP / kInner; ++k)
-                if (k * kInner < da) sc[t] = mma(b.piece(base + s, k * kInner + q * kN, s < n), af[k], sc[t]);
-        }
-        __syncthreads();                   // bt, ct, lam and X's copy are there
-        if (more) st.load(b, c, base + kChunk, (int)(to - base - kChunk < kChunk ? to - base - kChunk : kChunk));
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
+                for (int k = 0; k < kK; ++k) sc = mma(lds_piece(&l.b[t * 16 + r16][k * kInner + q * kN]), af[k], sc);
+            }
             float v[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int d = row - (t * 16 + q * 4 + e);
-                v[e] = d >= 0 ? r.ps * l.lam[d] * sc[t][e] : 0.f;
+                v[e] = d >= 0 ? r.ps * l.lam[d < 0 ? 0 : d] * sc[e] : 0.f;
             }
             lds_put4(&l.p[w][r16][t * 16 + q * 4], v);
         }
         wave_sync();
         // out, transposed: column = this wave's row, rows = columns of c
         const float decayed = r.so * l.lam[row];
-#pragma unroll
+#pragma unroll 2
         for (int j = 0; j < DP / 16; ++j) {
-            if (j >= nc) continue;
             f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (have) {
 #pragma unroll
-                for (int k = 0; k < DP / kInner; ++k)
-                    if (k * kInner < da) o = mma(lds_piece(&l.x[j * 16 + r16][k * kInner + q * kN]), af[k], o);
-                o *= decayed;
-            }
+            for (int k = 0; k < kK; ++k) o = mma(lds_piece(&l.x[j * 16 + r16][k * kInner + q * kN]), af[k], o);
+            o *= decayed;
 #pragma unroll
             for (int k = 0; k < kChunk; k += kInner)
-                if (k <= w * 16 + 15) o = mma(lds_piece(&l.ct[j * 16 + r16][k + q * kN]), lds_piece(&l.p[w][r16][k + q * kN]), o);
-            if (row < n) {
-                const int64_t tok = r.rev ? p.L - 1 - (base + row) : base + row;
-                put4(tok, j * 16 + q * 4, o);
-            }
+                if (k <= w * 16 + 15)
+                    o = mma(lds_column(&l.c[k + q * kN][j * 16], kRow), lds_piece(&l.p[w][r16][k + q * kN]), o);
+            if (row < n) put4(r.rev ? p.L - 1 - (base + row) : base + row, j * 16 + q * 4, o);
         }
         if (more || (last && s_out)) {
             // behind the last row the state of the forward recurrence has not been decayed once more
-            update<T, DP>(S, l, more ? kChunk : r.rev ? n : n - 1, r.kv, na, nc);
-            have = true;
-            if (more) {
-                __syncthreads();           // everybody has read X's copy
-                keep();
-            }
+            update<T, DP>(S, l, more ? kChunk : r.rev ? n : n - 1, r.kv);
         }
+        if (more) __syncthreads();         // everybody has read the chunk
     }
-    if (last && s_out) each<DP>(S, da, dc, [=](int i, int j, float v) { return s_out[i * in_a + j * in_c] = v; });
+    if (last && s_out) state_store<DP>(S, s_out, da, dc, r.in_a, r.in_c);
 }
 
 // sums of the query heads that share a key head: float32 [rows, HK, grp, dim] -> [rows, HK, dim] of the type
@@ -593,8 +620,7 @@ int launch(Args& a, const int (&joined)[2], int joins, hipStream_t st) {
         if (int rc = grant.ensure((const void*)kv_kernel<T, DP, EVEN>, sizeof(LdsKv<T, DP>))) return rc;
         kv_kernel<T, DP, EVEN><<<grid_of(k, a.nseg - 1), kThreads, sizeof(LdsKv<T, DP>), st>>>(k);
         SAMX_LAUNCH_CHECK();
-        const int most = a.r[0].b.dim * a.r[0].c.dim;    // (the same product for every role)
-        join_kernel<<<dim3((unsigned)((most + 255) / 256), (unsigned)(a.B * a.H), (unsigned)joins), 256, 0, st>>>(k, a.nseg - 1);
+        join_kernel<DP><<<dim3(DP * DP / 256, (unsigned)(a.B * a.H), (unsigned)joins), 256, 0, st>>>(k);
         SAMX_LAUNCH_CHECK();
     }
     static samx::LdsGrant grant;
@@ -618,7 +644,8 @@ int launch_type(int dtype, Args& a, int most, const int (&joined)[2], int joins,
     return launch_dim<f16>(a, most, joined, joins, st);
 }
 
-int64_t up4(int64_t n) { return (n + 3) / 4 * 4; }
+// a segment's state: whole tiles of the kernel that takes these dimensions
+int64_t seg_size(int D, int DV) { return D <= 64 && DV <= 64 ? 64 * 64 : kMaxDim * kMaxDim; }
 
 int check(const char* who, const samx_linattn_shape* s) {
     SAMX_REQUIRE(s, "%s: null shape", who);
@@ -635,7 +662,7 @@ int check(const char* who, const samx_linattn_shape* s) {
 Mat mat(const void* p, const int64_t (&st)[3], int grp, int dim) { return Mat{p, st[0], st[1], st[2], grp, dim}; }
 
 size_t seg_bytes(const Args& a, int D, int DV) {
-    return a.nseg > 1 ? (size_t)a.B * a.H * (a.nseg - 1) * up4(D) * up4(DV) * sizeof(float) : 0;
+    return a.nseg > 1 ? (size_t)a.B * a.H * (a.nseg - 1) * seg_size(D, DV) * sizeof(float) : 0;
 }
 
 }  // namespace
@@ -663,12 +690,12 @@ int samx_linattn(const samx_linattn_shape* s, const void* q, const void* k, cons
     const size_t need = seg_bytes(a, s->D, s->DV);
     if (need && (!ws || ws_bytes < need)) return samx::fail(SAMX_ERR_WORKSPACE, "samx_linattn: workspace %zu < %zu", ws_bytes, need);
     const int rep = s->H / s->HK;
-    a.seg_size = up4(s->D) * up4(s->DV);
+    a.seg_size = seg_size(s->D, s->DV);
     Role& r = a.r[0];
     r.a = mat(q, s->q, 1, s->D); r.b = mat(k, s->k, rep, s->D); r.c = mat(v, s->v, rep, s->DV);
     r.out = out; r.kv = 1.f; r.ps = scale; r.so = scale;
     r.s_in = state_in; r.in_a = s->DV; r.in_c = 1; r.s_out = state_out;
-    r.seg = (float*)ws; r.seg_a = 1; r.seg_c = up4(s->D);
+    r.seg = (float*)ws;
     const int joined[2] = {0, 0};
     return launch_type(s->dtype, a, s->D > s->DV ? s->D : s->DV, joined, 1, (hipStream_t)stream);
 }
@@ -696,7 +723,7 @@ int samx_linattn_grad(const samx_linattn_shape* s, const void* q, const void* k,
     cut(a);
     const int rep = s->H / s->HK, D = s->D, DV = s->DV;
     const Mat Q = mat(q, s->q, 1, D), K = mat(k, s->k, rep, D), V = mat(v, s->v, rep, DV), O = mat(dout, s->o, 1, DV);
-    a.seg_size = up4(D) * up4(DV);
+    a.seg_size = seg_size(D, DV);
     float* seg0 = (float*)ws;
     float* seg1 = seg0 + seg_bytes(a, D, DV) / sizeof(float);
     float* heads = seg1 + seg_bytes(a, D, DV) / sizeof(float);
@@ -706,17 +733,17 @@ int samx_linattn_grad(const samx_linattn_shape* s, const void* q, const void* k,
     // dq: the forward states, transposed
     Role& x = a.r[0];
     x.a = O; x.b = V; x.c = K; x.out = dq; x.kv = 1.f; x.ps = scale; x.so = scale;
-    x.s_in = state_in; x.in_a = 1; x.in_c = DV; x.seg = seg0; x.seg_a = 1; x.seg_c = up4(DV);
+    x.s_in = state_in; x.in_a = 1; x.in_c = DV; x.seg = seg0;
     // dv: the gradient's states; the last of them, decayed, is the gradient of the state before the first row
     Role& y = a.r[1];
     y.a = K; y.b = Q; y.c = O; y.out = rep > 1 ? (void*)dv_h : dv; y.out_f32 = rep > 1; y.rev = 1;
     y.kv = scale; y.ps = scale; y.so = 1.f;
-    y.s_in = dstate; y.in_a = DV; y.in_c = 1; y.s_out = dstate_in; y.seg = seg1; y.seg_a = 1; y.seg_c = up4(D);
+    y.s_in = dstate; y.in_a = DV; y.in_c = 1; y.s_out = dstate_in; y.seg = seg1;
     // dk: the same states, transposed
     Role& z = a.r[2];
     z = y;
     z.a = V; z.b = O; z.c = Q; z.out = rep > 1 ? (void*)dk_h : dk; z.s_out = nullptr;
-    z.in_a = 1; z.in_c = DV; z.seg_a = up4(D); z.seg_c = 1;
+    z.in_a = 1; z.in_c = DV; z.turned = 1;
     const hipStream_t st = (hipStream_t)stream;
     const int joined[2] = {0, 1};
     if (int rc = launch_type(s->dtype, a, D > DV ? D : DV, joined, 2, st)) return rc;
