@@ -24,6 +24,7 @@
 // a known state at each segment's start.
 #include "seq_dev.h"
 #include "../../include/samx.h"
+#include <type_traits>
 
 namespace {
 
@@ -33,7 +34,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kChunk = 64, kThreads = 256, kMaxDim = 128;
+constexpr int kChunk = 64, kMaxDim = 128;
+constexpr int kWaves = 4, kThreads = kWaves * 64;   // a wave for each 16 rows of a chunk
 
 // D += A B^T for 16 rows each and the kN * 4 inner values that 64 lanes' pieces hold: lane l has row l % 16, inner values
 // (l / 16) * kN + [0, kN).  D: lane l has column l % 16 (B's row), rows (l / 16) * 4 + [0, 4).
@@ -114,38 +116,47 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef u32x2 u32x2_any __attribute__((aligned(2)));
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 
-// a matrix of this place in the order of positions: its row 0, the step from one position to the next.  EVEN: its rows
-// are whole pieces.  (The pointer says that it is one to global memory, which the compiler cannot see behind the choice
-// of a role: it would use the instructions that may also mean LDS.)
+// a matrix of this place in the order of positions.  EVEN: its rows are whole pieces and a chunk of them lies within 2^31
+// bytes, so that a lane's place in a chunk is one offset to an address that all lanes share: no branch, nothing that waits.
+// (The pointer says that it is one to global memory, which the compiler cannot see behind the choice of a role: it would
+// use the instructions that may also mean LDS.)
 template <typename T, bool EVEN>
 struct Rows {
     static constexpr int kN = Piece<T>::kN;
-    const SAMX_GLOBAL char* p; int64_t step; int dim;
+    const SAMX_GLOBAL char* p;             // position 0
+    int64_t step;                          // bytes from one position to the next
+    int dim;
     __device__ Rows(Mat m, Place q, int rev) : dim(m.dim) {
         p = (const SAMX_GLOBAL char*)m.p + (int64_t)sizeof(T) * (q.b * m.sb + (int64_t)(q.h / m.grp) * m.sh + (rev ? (q.L - 1) * m.st : 0));
         step = (int64_t)sizeof(T) * (rev ? -m.st : m.st);
     }
-    // elements [at, at + kN) of position `pos`; zeros behind the row's end and where there is no such position
-    __device__ __forceinline__ Piece<T> piece(int64_t pos, int at, bool there) const {
+    // elements [at, at + kN) of position base + pos.  What lies behind the chunk's n positions or behind the row's end is
+    // not what comes here: the caller does not use it.
+    __device__ __forceinline__ Piece<T> piece(int64_t base, int pos, int at, int n) const {
         Piece<T> r;
+        const int row = pos < n ? pos : n - 1;
         if constexpr (EVEN) {
-            there = there && at < dim;
-            const u32x4 v = *(const SAMX_GLOBAL u32x4_any*)(there ? p + pos * step + at * (int)sizeof(T) : p);
+            // (backwards the shared address is that of the chunk's last position, below which nothing lies)
+            const bool back = step < 0;
+            const SAMX_GLOBAL char* chunk = p + base * step + (back ? (n - 1) * step : 0);
+            const uint32_t off = (back ? (uint32_t)(n - 1) * (uint32_t)-step : 0u) + (uint32_t)row * (uint32_t)step +
+                                 (at < dim ? (uint32_t)at * (uint32_t)sizeof(T) : 0u);
+            const u32x4 v = *(const SAMX_GLOBAL u32x4_any*)(chunk + off);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) r.w[j] = there ? v[j] : 0u;
+            for (int j = 0; j < 4; ++j) r.w[j] = v[j];
         } else {
-            const SAMX_GLOBAL char* e = p + (there ? pos * step : 0) + at * (int)sizeof(T);
-            const int n = there ? dim - at : 0;
-            if (n >= kN) {
+            const SAMX_GLOBAL char* e = p + (base + row) * step + at * (int)sizeof(T);
+            const int m = dim - at;
+            if (m >= kN) {
                 const u32x4 v = *(const SAMX_GLOBAL u32x4_any*)e;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) r.w[j] = v[j];
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if constexpr (sizeof(T) == 4) r.w[j] = j < n ? *(const SAMX_GLOBAL uint32_t*)(e + 4 * j) : 0u;
-                    else r.w[j] = (2 * j < n ? (uint32_t)*(const SAMX_GLOBAL uint16_t*)(e + 4 * j) : 0u) |
-                                  (2 * j + 1 < n ? (uint32_t)*(const SAMX_GLOBAL uint16_t*)(e + 4 * j + 2) : 0u) << 16;
+                    if constexpr (sizeof(T) == 4) r.w[j] = j < m ? *(const SAMX_GLOBAL uint32_t*)(e + 4 * j) : 0u;
+                    else r.w[j] = (2 * j < m ? (uint32_t)*(const SAMX_GLOBAL uint16_t*)(e + 4 * j) : 0u) |
+                                  (2 * j + 1 < m ? (uint32_t)*(const SAMX_GLOBAL uint16_t*)(e + 4 * j + 2) : 0u) << 16;
                 }
             }
         }
@@ -203,7 +214,7 @@ template <typename T, int DP>
 struct LdsKv {
     static constexpr int kRow = DP + Piece<T>::kN;
     T b[kChunk][kRow], c[kChunk][kRow];                  // the chunk's rows
-    float lam[kChunk + 4];                               // l^n
+    float lam[2 * kChunk + 4];                           // l^(n - kChunk), 0 below kChunk
 };
 template <typename T, int DP>
 struct Lds : LdsKv<T, DP> {
@@ -211,6 +222,24 @@ struct Lds : LdsKv<T, DP> {
     T p[4][16][kTok];                                    // each wave's 16 rows of scores
     T x[DP][LdsKv<T, DP>::kRow];                         // X, a row for each column
 };
+
+// N groups of products, group g's operands read (into buf[g % (AHEAD + 1)]) AHEAD groups before they are used; nothing is
+// moved across the groups.  (Left to itself the compiler saves registers by reading what it multiplies next.)
+template <int N, int AHEAD, int I = 0, typename Read, typename Use>
+__device__ __forceinline__ void in_groups(Read read, Use use) {
+    if constexpr (I == 0) {
+#pragma unroll
+        for (int g = 0; g < (AHEAD < N ? AHEAD : N); ++g) read(g, g % (AHEAD + 1));
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (I < N) {
+        if constexpr (I + AHEAD < N) read(I + AHEAD, (I + AHEAD) % (AHEAD + 1));
+        __builtin_amdgcn_sched_barrier(0);
+        use(I, I % (AHEAD + 1));
+        __builtin_amdgcn_sched_barrier(0);
+        in_groups<N, AHEAD, I + 1>(read, use);
+    }
+}
 
 // A chunk's rows of b and c on their way to LDS
 template <typename T, int DP>
@@ -221,26 +250,31 @@ struct Staged {
     __device__ __forceinline__ void load(const Rows<T, EVEN>& mb, const Rows<T, EVEN>& mc, int64_t base, int n) {
         const int t = threadIdx.x / kAcross, d = threadIdx.x % kAcross * kN;
 #pragma unroll
-        for (int u = 0; u < kPer; ++u) b[u] = mb.piece(base + t + u * kDown, d, t + u * kDown < n);
+        for (int u = 0; u < kPer; ++u) b[u] = mb.piece(base, t + u * kDown, d, n);
 #pragma unroll
-        for (int u = 0; u < kPer; ++u) c[u] = mc.piece(base + t + u * kDown, d, t + u * kDown < n);
+        for (int u = 0; u < kPer; ++u) c[u] = mc.piece(base, t + u * kDown, d, n);
     }
+    // zeros behind the rows' ends and behind the n positions
     template <typename L>
-    __device__ __forceinline__ void store(L& l) const {
+    __device__ __forceinline__ void store(L& l, int db, int dc, int n) const {
         const int t = threadIdx.x / kAcross, d = threadIdx.x % kAcross * kN;
 #pragma unroll
         for (int u = 0; u < kPer; ++u) {
-            lds_put(&l.b[t + u * kDown][d], b[u]);
-            lds_put(&l.c[t + u * kDown][d], c[u]);
+            const uint32_t kb = d < db && t + u * kDown < n ? ~0u : 0u, kc = d < dc && t + u * kDown < n ? ~0u : 0u;
+            Piece<T> x, y;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { x.w[j] = b[u].w[j] & kb; y.w[j] = c[u].w[j] & kc; }
+            lds_put(&l.b[t + u * kDown][d], x);
+            lds_put(&l.c[t + u * kDown][d], y);
         }
     }
 };
 
-// X of a workgroup: wave w owns the tiles of 16 columns w, w + 4, ...; tile (j, i): lane l has column l % 16, rows
+// X of a workgroup: wave w owns the tiles of 16 columns w, w + kWaves, ...; tile (j, i): lane l has column l % 16, rows
 // (l / 16) * 4 + [0, 4) of the a side
 template <int DP>
 struct State {
-    static constexpr int kJ = DP / 64, kI = DP / 16;
+    static constexpr int kJ = DP / 16 / kWaves, kI = DP / 16;
     f32x4 x[kJ][kI];
     __device__ __forceinline__ void zero() {
 #pragma unroll
@@ -260,7 +294,7 @@ template <typename T, int DP, typename L>
 __device__ __forceinline__ void update(State<DP>& S, const L& l, int end, float kv) {
     constexpr int kN = Piece<T>::kN, kJ = State<DP>::kJ, kI = State<DP>::kI, kP = kParts<T>;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane >> 4;
-    const float whole = l.lam[end];
+    const float whole = l.lam[kChunk + end];
 #pragma unroll
     for (int j = 0; j < kJ; ++j)
 #pragma unroll
@@ -269,18 +303,18 @@ __device__ __forceinline__ void update(State<DP>& S, const L& l, int end, float 
     for (int k = 0; k < kChunk; k += 4 * kN) {
         const int s0 = k + q * kN;
         float f[kN];
+        Piece<T> c[kJ];
 #pragma unroll
-        for (int e = 0; e < kN; ++e) {
-            const int n = end - s0 - e;
-            f[e] = kv * l.lam[n < 0 ? 0 : n];   // (rows behind the end are zeros)
-        }
+        for (int e = 0; e < kN; ++e) f[e] = l.lam[kChunk + end - s0 - e];   // (rows behind the end are zeros, and their factors)
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) c[j] = lds_column(&l.c[s0][(w + kWaves * j) * 16], L::kRow);
+        __builtin_amdgcn_sched_barrier(0);
         Piece<T> part[kJ][kP];
 #pragma unroll
         for (int j = 0; j < kJ; ++j) {
-            const Piece<T> c = lds_column(&l.c[s0][(w + 4 * j) * 16], L::kRow);
             float v[kN];
 #pragma unroll
-            for (int e = 0; e < kN; ++e) v[e] = c.f(e) * f[e];
+            for (int e = 0; e < kN; ++e) v[e] = c[j].f(e) * (kv * f[e]);
 #pragma unroll
             for (int u = 0; u < kP; ++u) {
                 part[j][u] = pack<T>(v);
@@ -288,14 +322,20 @@ __device__ __forceinline__ void update(State<DP>& S, const L& l, int end, float 
                 for (int e = 0; e < kN; ++e) v[e] -= part[j][u].f(e);
             }
         }
+        Piece<T> b[2][4];
+        in_groups<kI / 4, 1>(
+            [&](int g, int at) {
 #pragma unroll
-        for (int i = 0; i < kI; ++i) {
-            const Piece<T> b = lds_column(&l.b[s0][i * 16], L::kRow);
+                for (int i = 0; i < 4; ++i) b[at][i] = lds_column(&l.b[s0][(g * 4 + i) * 16], L::kRow);
+            },
+            [&](int g, int at) {
 #pragma unroll
-            for (int j = 0; j < kJ; ++j)
+                for (int u = 0; u < kP; ++u)
 #pragma unroll
-                for (int u = 0; u < kP; ++u) S.x[j][i] = mma(b, part[j][u], S.x[j][i]);
-        }
+                    for (int j = 0; j < kJ; ++j)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) S.x[j][g * 4 + i] = mma(b[at][i], part[j][u], S.x[j][g * 4 + i]);
+            });
     }
 }
 
@@ -309,7 +349,7 @@ __device__ __forceinline__ void state_load(State<DP>& S, const SAMX_GLOBAL float
         for (int i = 0; i < State<DP>::kI; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int c = (w + 4 * j) * 16 + r16, a = i * 16 + q * 4 + e;
+                const int c = (w + kWaves * j) * 16 + r16, a = i * 16 + q * 4 + e;
                 const bool there = a < da && c < dc;
                 const float v = m[(uint32_t)(there ? a * sa + c * sc : 0)];      // (no branch: the loads go out together)
                 S.x[j][i][e] = there ? v * f : 0.f;
@@ -324,7 +364,7 @@ __device__ __forceinline__ void state_store(const State<DP>& S, SAMX_GLOBAL floa
         for (int i = 0; i < State<DP>::kI; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int c = (w + 4 * j) * 16 + r16, a = i * 16 + q * 4 + e;
+                const int c = (w + kWaves * j) * 16 + r16, a = i * 16 + q * 4 + e;
                 if (a < da && c < dc) m[(uint32_t)(a * sa + c * sc)] = S.x[j][i][e];
             }
 }
@@ -336,7 +376,7 @@ __device__ __forceinline__ void seg_load(State<DP>& S, const SAMX_GLOBAL float* 
     for (int j = 0; j < State<DP>::kJ; ++j)
 #pragma unroll
         for (int i = 0; i < State<DP>::kI; ++i) {
-            const uint32_t c = (w + 4 * j) * 16 + r16, a = i * 16 + q * 4;
+            const uint32_t c = (w + kWaves * j) * 16 + r16, a = i * 16 + q * 4;
             if (!turned) {
                 S.x[j][i] = *(const SAMX_GLOBAL f32x4*)(m + c * DP + a);
             } else {
@@ -352,7 +392,7 @@ __device__ __forceinline__ void seg_store(const State<DP>& S, SAMX_GLOBAL float*
     for (int j = 0; j < State<DP>::kJ; ++j)
 #pragma unroll
         for (int i = 0; i < State<DP>::kI; ++i)
-            *(SAMX_GLOBAL f32x4*)(m + (uint32_t)(((w + 4 * j) * 16 + r16) * DP + i * 16 + q * 4)) = S.x[j][i];
+            *(SAMX_GLOBAL f32x4*)(m + (uint32_t)(((w + kWaves * j) * 16 + r16) * DP + i * 16 + q * 4)) = S.x[j][i];
 }
 
 template <typename T, int DP, bool EVEN>
@@ -365,14 +405,14 @@ __global__ __launch_bounds__(kThreads, 2) void kv_kernel(Args A) {
     if (p.L <= at + A.seg_len) return;                  // nobody follows
     const Role r = A.r[p.role];
     const Rows<T, EVEN> b(r.b, p, r.rev), c(r.c, p, r.rev);
-    if (threadIdx.x <= kChunk) l.lam[threadIdx.x] = power(p.g, threadIdx.x);
+    if (threadIdx.x <= 2 * kChunk) l.lam[threadIdx.x] = threadIdx.x < kChunk ? 0.f : power(p.g, threadIdx.x - kChunk);
     State<DP> S;
     S.zero();
     Staged<T, DP> st;
     st.load(b, c, at, kChunk);
     for (int64_t k = 0; k < A.seg_len; k += kChunk) {
         __syncthreads();
-        st.store(l);
+        st.store(l, r.b.dim, r.c.dim, kChunk);
         __syncthreads();
         if (k + kChunk < A.seg_len) st.load(b, c, at + k + kChunk, kChunk);
         update<T, DP>(S, l, kChunk, r.kv);
@@ -411,7 +451,7 @@ __global__ __launch_bounds__(256) void join_kernel(Args A) {
 }
 
 template <typename T, int DP, bool EVEN>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void mix_kernel(Args A) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void mix_kernel(Args A) {
     constexpr int kN = Piece<T>::kN, kInner = 4 * kN, kK = DP / kInner;      // inner values of one mma
     extern __shared__ __attribute__((aligned(16))) char lds_[];
     Lds<T, DP>& l = *reinterpret_cast<Lds<T, DP>*>(lds_);
@@ -420,7 +460,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void mix_kernel(A
     if (!place_of(A, A.nseg, p)) return;
     // (by value: a reference into the arguments makes the compiler keep a copy of all of them in scratch memory)
     const Role r = A.r[p.role];
+    // wave w: columns of a state; of a chunk, rows 16 w + [0, 16) of out
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
+    constexpr int kTiles = DP / 16;
     const int64_t at = (int64_t)p.seg * A.seg_len, bh = (int64_t)p.b * A.H + p.h;
     const int64_t to = at + A.seg_len < p.L ? at + A.seg_len : p.L;         // this segment's positions
     const int da = r.a.dim, dc = r.c.dim;
@@ -428,8 +470,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void mix_kernel(A
     const int64_t out_at = ((int64_t)p.b * A.T * A.H + p.h) * dc;
     SAMX_GLOBAL char* const outp = (SAMX_GLOBAL char*)r.out + out_at * (r.out_f32 ? 4 : (int)sizeof(T));
     // four of a row's outputs from d on, those that exist
-    auto put4 = [=](int64_t row, int d, f32x4 v) {
-        if (sizeof(T) == 4 || r.out_f32) {
+    auto put4 = [=](auto f32, int64_t row, int d, f32x4 v) {
+        if constexpr (decltype(f32)::value) {
             SAMX_GLOBAL float* o = (SAMX_GLOBAL float*)outp + row * out_row + d;
             if (EVEN) { if (d < dc) *(SAMX_GLOBAL f32x4_any*)o = v; return; }
 #pragma unroll
@@ -445,10 +487,14 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void mix_kernel(A
             if (d + 3 < dc) o[3] = (uint16_t)(hi >> 16);
         }
     };
+    const bool wide = sizeof(T) == 4 || r.out_f32;
     {   // rows behind the trajectory's end
         const int64_t z0 = at > p.L ? at : p.L, z1 = at + A.seg_len < A.T ? at + A.seg_len : A.T;
-        for (int64_t t = z0 + threadIdx.x / 64; t < z1; t += 4)
-            for (int d = lane * 4; d < dc; d += 256) put4(t, d, f32x4{0.f, 0.f, 0.f, 0.f});
+        for (int64_t t = z0 + w; t < z1; t += kWaves)
+            for (int d = lane * 4; d < dc; d += 256) {
+                if (wide) put4(std::true_type(), t, d, f32x4{0.f, 0.f, 0.f, 0.f});
+                else put4(std::false_type(), t, d, f32x4{0.f, 0.f, 0.f, 0.f});
+            }
     }
     State<DP> S;
     const SAMX_GLOBAL float* s_in = r.s_in ? (const SAMX_GLOBAL float*)r.s_in + bh * da * dc : nullptr;
@@ -465,64 +511,107 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void mix_kernel(A
     const Rows<T, EVEN> a(r.a, p, r.rev), b(r.b, p, r.rev), c(r.c, p, r.rev);
     const int row = w * 16 + r16;          // of a chunk: this lane's
     Staged<T, DP> st;
-    Piece<T> af[kK], an[kK];               // a's rows of this wave, whole: the chunk's, the next one's
-    auto fetch = [&](int64_t base) {
-        const int n = (int)(to - base < kChunk ? to - base : kChunk);
-        st.load(b, c, base, n);
+    // a's rows of this wave, whole; behind their ends there is something of the row, which only meets zeros of b and X, and
+    // a row that the chunk does not have is another one, whose outputs are not written
+    Piece<T> af[kK];
+    auto rows_at = [&](int64_t base) { return (int)(to - base < kChunk ? to - base : kChunk); };
+    auto fetch_a = [&](int64_t base) {
 #pragma unroll
-        for (int k = 0; k < kK; ++k) an[k] = a.piece(base + row, k * kInner + q * kN, row < n);
+        for (int k = 0; k < kK; ++k) af[k] = a.piece(base, row, k * kInner + q * kN, rows_at(base));
     };
-    fetch(at);
+    st.load(b, c, at, rows_at(at));
+    fetch_a(at);
     const bool last = to == p.L;           // this segment makes the state behind the last position
     if (p.seg > 0) seg_load<DP>(S, (const SAMX_GLOBAL float*)r.seg + (bh * (A.nseg - 1) + p.seg - 1) * A.seg_size, r.turned);
     else if (s_in) state_load<DP>(S, s_in, da, dc, r.in_a, r.in_c, r.rev ? 1.f : power(p.g, 1));
     else S.zero();
-    if (threadIdx.x <= kChunk) l.lam[threadIdx.x] = power(p.g, threadIdx.x);
+    if (threadIdx.x <= 2 * kChunk) l.lam[threadIdx.x] = threadIdx.x < kChunk ? 0.f : power(p.g, threadIdx.x - kChunk);
     for (int64_t base = at; base < to; base += kChunk) {
         const int n = (int)(to - base < kChunk ? to - base : kChunk);
         const bool more = base + kChunk < to;
-        st.store(l);
+        st.store(l, da, dc, n);
 #pragma unroll
         for (int j = 0; j < State<DP>::kJ; ++j)          // X's copy for the products with a
 #pragma unroll
             for (int i = 0; i < State<DP>::kI; ++i) {
                 const float v[4] = {S.x[j][i][0], S.x[j][i][1], S.x[j][i][2], S.x[j][i][3]};
-                lds_put4(&l.x[(w + 4 * j) * 16 + r16][i * 16 + q * 4], v);
+                lds_put4(&l.x[(w + kWaves * j) * 16 + r16][i * 16 + q * 4], v);
             }
-#pragma unroll
-        for (int k = 0; k < kK; ++k) af[k] = an[k];
         __syncthreads();
-        if (more) fetch(base + kChunk);
-        // scores, transposed: column = this wave's row, rows = positions s; masked and decayed
-#pragma unroll 2
-        for (int t = 0; t < 4; ++t) {
-            f32x4 sc = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (t <= w) {
+        if (more) st.load(b, c, base + kChunk, rows_at(base + kChunk));
+        // scores, transposed: column = this wave's row, rows = positions s.  (Nothing here branches on the wave: no read
+        // would be ahead of its use across a branch.)
+        f32x4 sc[4];
 #pragma unroll
-                for (int k = 0; k < kK; ++k) sc = mma(lds_piece(&l.b[t * 16 + r16][k * kInner + q * kN]), af[k], sc);
-            }
+        for (int t = 0; t < 4; ++t) sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        // out, transposed: column = this wave's row, rows = columns of c
+        f32x4 o[kTiles];
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        constexpr int kFour = kTiles / 4;
+        Piece<T> f[3][4];
+        in_groups<kK * (1 + kFour), 2>(
+            [&](int g, int at) {
+                const int k = g % kK, j = (g / kK - 1) * 4;
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                    f[at][t] = g < kK ? lds_piece(&l.b[t * 16 + r16][k * kInner + q * kN])
+                                      : lds_piece(&l.x[(j + t) * 16 + r16][k * kInner + q * kN]);
+            },
+            [&](int g, int at) {
+                const int k = g % kK, j = (g / kK - 1) * 4;
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    if (g < kK) sc[t] = mma(f[at][t], af[k], sc[t]);
+                    else o[j + t] = mma(f[at][t], af[k], o[j + t]);
+                }
+            });
+        if (more) fetch_a(base + kChunk);
+        const float decayed = r.so * l.lam[kChunk + row];
+        float lam[4][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) lam[t][e] = l.lam[kChunk + row - (t * 16 + q * 4 + e)];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) o[j] *= decayed;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
             float v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int d = row - (t * 16 + q * 4 + e);
-                v[e] = d >= 0 ? r.ps * l.lam[d < 0 ? 0 : d] * sc[e] : 0.f;
+            for (int e = 0; e < 4; ++e) {   // (l^d is 0 behind the row, but 0 times a NaN is none)
+                const float x = r.ps * lam[t][e] * sc[t][e];
+                v[e] = row >= t * 16 + q * 4 + e ? x : 0.f;
             }
             lds_put4(&l.p[w][r16][t * 16 + q * 4], v);
         }
         wave_sync();
-        // out, transposed: column = this wave's row, rows = columns of c
-        const float decayed = r.so * l.lam[row];
-#pragma unroll 2
-        for (int j = 0; j < DP / 16; ++j) {
-            f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+        Piece<T> pk[kChunk / kInner];
 #pragma unroll
-            for (int k = 0; k < kK; ++k) o = mma(lds_piece(&l.x[j * 16 + r16][k * kInner + q * kN]), af[k], o);
-            o *= decayed;
+        for (int k = 0; k < kChunk / kInner; ++k) pk[k] = lds_piece(&l.p[w][r16][k * kInner + q * kN]);
+        in_groups<kChunk / kInner * kFour, 2>(
+            [&](int g, int at) {
 #pragma unroll
-            for (int k = 0; k < kChunk; k += kInner)
-                if (k <= w * 16 + 15)
-                    o = mma(lds_column(&l.c[k + q * kN][j * 16], kRow), lds_piece(&l.p[w][r16][k + q * kN]), o);
-            if (row < n) put4(r.rev ? p.L - 1 - (base + row) : base + row, j * 16 + q * 4, o);
+                for (int t = 0; t < 4; ++t)
+                    f[at][t] = lds_column(&l.c[g / kFour * kInner + q * kN][(g % kFour * 4 + t) * 16], kRow);
+            },
+            [&](int g, int at) {
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    f32x4& d = o[g % kFour * 4 + t];
+                    d = mma(f[at][t], pk[g / kFour], d);
+                }
+            });
+        if (row < n) {
+            const int64_t tok = r.rev ? p.L - 1 - (base + row) : base + row;
+            if (wide) {
+#pragma unroll
+                for (int j = 0; j < kTiles; ++j) put4(std::true_type(), tok, j * 16 + q * 4, o[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kTiles; ++j) put4(std::false_type(), tok, j * 16 + q * 4, o[j]);
+            }
         }
         if (more || (last && s_out)) {
             // behind the last row the state of the forward recurrence has not been decayed once more
@@ -590,24 +679,24 @@ __global__ __launch_bounds__(256) void step_kernel(Mat Q, Mat K, Mat V, const fl
 
 // ---------------------------------------------------------------- host
 
-// Workgroups that a device keeps busy: two for each of its units.
-int segments(int64_t B, int H, int roles, int64_t T) {
-    const int64_t units = B * H * roles, want = 2 * (int64_t)cu_count();
-    int64_t n = (want + units - 1) / (units > 0 ? units : 1);
-    const int64_t most = T / 256;          // four chunks at least
-    n = n < most ? n : most;
-    return (int)(n < 1 ? 1 : n);
-}
-int64_t seg_len_of(int64_t T, int nseg) {
-    const int64_t s = (T + nseg - 1) / nseg;
-    return (s + kChunk - 1) / kChunk * kChunk;
-}
+// How many segments time is cut into.  In the time that a workgroup takes for a chunk (4 us at 128 dimensions of 16 bits):
+// a sequence of c chunks takes c; in n segments it takes c / n, and half as much again for kv_kernel, 6 for the other two
+// launches and the states' way through memory, times the rounds in which the device takes all the workgroups, one for each
+// of its units (two at once take twice as long: they are bound by memory).  Measured (us), 2 x 4096 rows, 16 heads of 128,
+// bfloat16: n = 4 123, 8 81, 16 83; 8 x 512 rows: n = 1 45, 2 61, 4 64.
 void cut(Args& a) {
-    a.nseg = segments(a.B, a.H, a.roles, a.T);
-    a.seg_len = seg_len_of(a.T, a.nseg);
-    if (a.seg_len < kChunk) a.seg_len = kChunk;
-    a.nseg = (int)((a.T + a.seg_len - 1) / a.seg_len);
-    if (a.nseg < 1) a.nseg = 1;
+    const int64_t c = (a.T + kChunk - 1) / kChunk, units = (int64_t)a.B * a.H * a.roles, cu = cu_count();
+    double best = 0.0;
+    a.nseg = 1;
+    a.seg_len = (c < 1 ? 1 : c) * kChunk;
+    for (int64_t n = 1; n <= c && n <= 64; ++n) {
+        const int64_t each = (c + n - 1) / n, rounds = (units * n + cu - 1) / cu;
+        const double cost = (double)(each * rounds) * (n > 1 ? 1.5 : 1.0) + (n > 1 ? 6.0 : 0.0);
+        if (n > 1 && cost >= best) continue;
+        best = cost;
+        a.seg_len = each * kChunk;
+        a.nseg = (int)((c + each - 1) / each);
+    }
 }
 
 template <typename T, int DP, bool EVEN>
@@ -633,8 +722,13 @@ int launch(Args& a, const int (&joined)[2], int joins, hipStream_t st) {
 template <typename T>
 int launch_dim(Args& a, int most, const int (&joined)[2], int joins, hipStream_t st) {
     const int n = Piece<T>::kN;
-    if (a.r[0].b.dim % n == 0 && a.r[0].c.dim % n == 0)
-        return most <= 64 ? launch<T, 64, true>(a, joined, joins, st) : launch<T, 128, true>(a, joined, joins, st);
+    bool even = true;
+    for (int i = 0; i < a.roles; ++i)
+        for (const Mat* m : {&a.r[i].a, &a.r[i].b, &a.r[i].c}) {
+            const int64_t st = m->st < 0 ? -m->st : m->st;
+            even = even && m->dim % n == 0 && st < (int64_t(1) << 31) / ((int64_t)sizeof(T) * kChunk) - kMaxDim;
+        }
+    if (even) return most <= 64 ? launch<T, 64, true>(a, joined, joins, st) : launch<T, 128, true>(a, joined, joins, st);
     return most <= 64 ? launch<T, 64, false>(a, joined, joins, st) : launch<T, 128, false>(a, joined, joins, st);
 }
 
