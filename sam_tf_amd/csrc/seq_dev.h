@@ -5,6 +5,7 @@
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 #include <math.h>
+#include <atomic>
 #include "samx_common.h"
 
 namespace samx {
@@ -192,11 +193,17 @@ __device__ __forceinline__ void row_reduce(V (&v)[C], V* sh, int waves, int& tur
     }
 }
 
+// units of the current device (asked once for each)
 inline int cu_count() {
-    int dev = 0, n = 0;
-    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
-        return 256;
-    return n > 0 ? n : 256;
+    static std::atomic<int> known[64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+    int n = known[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+        known[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
 }
 
 }  // namespace seq

@@ -922,27 +922,37 @@ SEQ_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # SAMX_F3
 _NORM = {'rms': 0, 'layer': 1}
 
 
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
 def _seq_dtype(t, name):
+    """(type code, device) of the tensor that a call goes by; the device has to be the current one."""
     if not (isinstance(t, torch.Tensor) and t.is_cuda):
         raise TypeError('%s must be a CUDA tensor' % name)
     code = SEQ_DTYPES.get(t.dtype)
     if code is None:
         raise TypeError('%s must be float32, bfloat16 or float16, got %s' % (name, t.dtype))
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError('%s is on %s, the current device is cuda:%d' % (name, t.device, torch.cuda.current_device()))
-    return code
+    dev = t.device
+    if dev.index != _current_device():
+        raise ValueError('%s is on %s, the current device is cuda:%d' % (name, dev, _current_device()))
+    return code, dev
 
 
-def _on(t, like, dtype, shape, name):
-    """_chk, and on the device of `like`."""
-    _chk(t, dtype, shape, name)
-    if t.device != like.device:
-        raise ValueError('%s is on %s, expected %s' % (name, t.device, like.device))
-    return t
+def _on(t, dev, dtype, shape, name):
+    """The address of a dense tensor of this type and shape on `dev`."""
+    if not isinstance(t, torch.Tensor) or t.device != dev:
+        raise TypeError('%s must be a tensor on %s' % (name, dev))
+    if t.dtype != dtype:
+        raise TypeError('%s must be %s, got %s' % (name, dtype, t.dtype))
+    if t.shape != shape:
+        raise ValueError('%s has shape %s, expected %s' % (name, tuple(t.shape), tuple(shape)))
+    if not t.is_contiguous():
+        raise ValueError('%s must be contiguous' % name)
+    return t.data_ptr()
 
 
-def _opt_on(t, like, dtype, shape, name):
-    return None if t is None else _on(t, like, dtype, shape, name)
+def _opt_on(t, dev, dtype, shape, name):
+    return None if t is None else _on(t, dev, dtype, shape, name)
 
 
 def _apart(named):
@@ -955,22 +965,24 @@ def _apart(named):
 
 
 def _norm_args(y, gate, post_w, post_b, pre_w, pre_b, kind):
-    code = _seq_dtype(y, 'y')
+    code, dev = _seq_dtype(y, 'y')
     if y.dim() != 2:
         raise ValueError('y must be [rows, channels], got %s' % (tuple(y.shape),))
     N, D = y.shape
     if kind not in _NORM:
         raise ValueError("kind must be 'rms' or 'layer', got %r" % (kind,))
-    _on(post_w, y, F32, (D,), 'post_w'); _on(pre_w, y, F32, (D,), 'pre_w')
+    w = (_on(post_w, dev, F32, (D,), 'post_w'), _on(pre_w, dev, F32, (D,), 'pre_w'))
     if kind == 'layer':
-        _on(post_b, y, F32, (D,), 'post_b'); _on(pre_b, y, F32, (D,), 'pre_b')
+        b = (_on(post_b, dev, F32, (D,), 'post_b'), _on(pre_b, dev, F32, (D,), 'pre_b'))
     elif post_b is not None or pre_b is not None:
         raise ValueError("the RMS norm has no bias")
-    gate_kind = 0
+    else:
+        b = (None, None)
+    gate_kind, g = 0, None
     if gate is not None:
         gate_kind = 1 if gate.dim() == 1 else 2
-        _on(gate, y, F32 if gate_kind == 1 else y.dtype, (D,) if gate_kind == 1 else (N, D), 'gate')
-    return code, N, D, gate_kind
+        g = _on(gate, dev, F32 if gate_kind == 1 else y.dtype, (D,) if gate_kind == 1 else y.shape, 'gate')
+    return code, dev, N, D, w, b, gate_kind, g, _on(y, dev, y.dtype, y.shape, 'y')
 
 
 def block_norm(x, y, post_w, pre_w, post_b=None, pre_b=None, gate=None, res_scale=1.0, kind='rms', eps=1e-8, h=None,
@@ -979,13 +991,15 @@ def block_norm(x, y, post_w, pre_w, post_b=None, pre_b=None, gate=None, res_scal
     h = res_scale * x + gate * N(y; post_w, post_b), u = N(h; pre_w, pre_b).  x, y [rows, channels] in float32, bfloat16
     or float16; weights and biases float32 [channels] (biases with kind 'layer' only); gate None, float32 [channels] or
     like y.  Returns (h, u); they may be given, x's and y's own buffers among them (samx_block_norm)."""
-    code, N, D, gate_kind = _norm_args(y, gate, post_w, post_b, pre_w, pre_b, kind)
-    _on(x, y, y.dtype, (N, D), 'x')
-    h = torch.empty_like(y) if h is None else _on(h, y, y.dtype, (N, D), 'h')
-    u = torch.empty_like(y) if u is None else _on(u, y, y.dtype, (N, D), 'u')
-    _apart((('h', h), ('u', u)))
-    check(_L().samx_block_norm(ptr(x), ptr(y), code, N, D, ptr(post_w), ptr(post_b), gate_kind, ptr(gate), ptr(pre_w),
-                               ptr(pre_b), float(res_scale), _NORM[kind], float(eps), ptr(h), ptr(u), stream_ptr()))
+    code, dev, N, D, w, b, gate_kind, g, py = _norm_args(y, gate, post_w, post_b, pre_w, pre_b, kind)
+    px = _on(x, dev, y.dtype, y.shape, 'x')
+    if h is not None or u is not None:
+        _apart((('h', h), ('u', u)))
+    h = torch.empty_like(y) if h is None else h
+    u = torch.empty_like(y) if u is None else u
+    check(_L().samx_block_norm(px, py, code, N, D, w[0], b[0], gate_kind, g, w[1], b[1], res_scale, _NORM[kind], eps,
+                               _on(h, dev, y.dtype, y.shape, 'h'), _on(u, dev, y.dtype, y.shape, 'u'),
+                               _raw_stream(dev.index)))
     return h, u
 
 
@@ -994,60 +1008,57 @@ def block_norm_grad(y, h, dh, du, post_w, pre_w, post_b=None, pre_b=None, gate=N
     """The gradient of block_norm from dh (the gradient of h by the residual path) and du (of u); y as it went in, h as it
     came out.  Returns a dict: x, y, gate (None without one), post_w, post_b, pre_w, pre_b (biases None with 'rms')
     (samx_block_norm_grad)."""
-    code, N, D, gate_kind = _norm_args(y, gate, post_w, post_b, pre_w, pre_b, kind)
-    for t, n in ((h, 'h'), (dh, 'dh'), (du, 'du')):
-        _on(t, y, y.dtype, (N, D), n)
+    code, dev, N, D, w, b, gate_kind, g, py = _norm_args(y, gate, post_w, post_b, pre_w, pre_b, kind)
+    ph, pdh, pdu = (_on(t, dev, y.dtype, y.shape, n) for t, n in ((h, 'h'), (dh, 'dh'), (du, 'du')))
     L = _L()
-    nb = int(L.samx_block_norm_grad_ws_bytes(code, N, D))
-    if ws is None:
-        ws = torch.empty(max(nb, 1), dtype=torch.uint8, device=y.device)
-    _on(ws, y, torch.uint8, (ws.numel(),), 'ws')
+    ws, pws, nws = _seq_ws(ws, L.samx_block_norm_grad_ws_bytes(code, N, D), dev)
     layer = kind == 'layer'
-    sums = torch.empty((2 + 2 * layer + (gate_kind == 1), D), dtype=F32, device=y.device)
+    sums = torch.empty((2 + 2 * layer + (gate_kind == 1), D), dtype=F32, device=dev)
     out = dict(x=torch.empty_like(y), y=torch.empty_like(y), gate=None, post_w=sums[0], post_b=None, pre_w=sums[1],
                pre_b=None)
     if layer:
         out['post_b'], out['pre_b'] = sums[2], sums[3]
     if gate_kind:
         out['gate'] = sums[-1] if gate_kind == 1 else torch.empty_like(y)
-    check(L.samx_block_norm_grad(
-        ptr(y), ptr(h), ptr(dh), ptr(du), code, N, D, ptr(post_w), ptr(post_b), gate_kind, ptr(gate), ptr(pre_w),
-        float(res_scale), _NORM[kind], float(eps), ptr(out['x']), ptr(out['y']), ptr(out['gate']), ptr(out['post_w']),
-        ptr(out['post_b']), ptr(out['pre_w']), ptr(out['pre_b']), ptr(ws), ws.numel(), stream_ptr()))
+    p = {n: None if t is None else t.data_ptr() for n, t in out.items()}
+    check(L.samx_block_norm_grad(py, ph, pdh, pdu, code, N, D, w[0], b[0], gate_kind, g, w[1], res_scale, _NORM[kind],
+                                 eps, p['x'], p['y'], p['gate'], p['post_w'], p['post_b'], p['pre_w'], p['pre_b'], pws,
+                                 nws, _raw_stream(dev.index)))
     return out
 
 
-def _heads(t, like, shape, name):
-    """[B, T, heads, dim] dense in the last dimension -> its strides (batch, row, head)."""
-    if not (isinstance(t, torch.Tensor) and t.device == like.device and t.dtype == like.dtype):
-        raise TypeError('%s must be %s on %s' % (name, like.dtype, like.device))
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError('%s has shape %s, expected %s' % (name, tuple(t.shape), tuple(shape)))
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError('%s must be dense in its last dimension' % name)
-    return t.stride()[:-1]
-
-
-def _linattn_args(q, k, v, decay, dout=None):
-    code = _seq_dtype(q, 'q')
-    if q.dim() != 4 or not isinstance(k, torch.Tensor) or k.dim() != 4 or not isinstance(v, torch.Tensor) or v.dim() != 4:
-        raise ValueError('q, k and v must be [batch, rows, heads, dim]')
-    B, T, H, D = q.shape
-    HK, DV = k.shape[2], v.shape[3]
-    s = _lib.LinattnShape(code, H, HK, D, DV, 0, B, T)
-    s.q[:] = _heads(q, q, (B, T, H, D), 'q')
-    s.k[:] = _heads(k, q, (B, T, HK, D), 'k')
-    s.v[:] = _heads(v, q, (B, T, HK, DV), 'v')
-    if dout is not None:
-        s.o[:] = _heads(dout, q, (B, T, H, DV), 'dout')
-    _on(decay, q, F32, (H,), 'decay')
-    return s
-
-
-def _linattn_ws(s, ws, nbytes, like):
+def _seq_ws(ws, nbytes, dev):
+    """(workspace, its address, its bytes): the caller's, or one from torch's allocator."""
     if ws is None:
-        return torch.empty(max(1, nbytes), dtype=torch.uint8, device=like.device)
-    return _on(ws, like, torch.uint8, (ws.numel(),), 'ws')
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    return ws, _on(ws, dev, torch.uint8, (ws.numel(),), 'ws'), ws.numel()
+
+
+def _heads(t, to, dev, dtype, shape, name):
+    """The address of [..., heads, dim], dense in the last dimension; its strides (batch, row, head) go to `to`."""
+    if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != dtype:
+        raise TypeError('%s must be %s on %s' % (name, dtype, dev))
+    if t.shape != shape:
+        raise ValueError('%s has shape %s, expected %s' % (name, tuple(t.shape), tuple(shape)))
+    st = t.stride()
+    if st[-1] != 1 and shape[-1] > 1:
+        raise ValueError('%s must be dense in its last dimension' % name)
+    to[0], to[1], to[2] = st[0], st[-3], st[-2]
+    return t.data_ptr()
+
+
+def _linattn_args(q, k, v, decay, dims):
+    """The shape (without the strides) and the addresses of q, k, v, decay; dims: 4 with rows, 3 without."""
+    code, dev = _seq_dtype(q, 'q')
+    if not (isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor) and q.dim() == k.dim() == v.dim() == dims):
+        raise ValueError('q, k and v must be [batch, %sheads, dim]' % ('rows, ' if dims == 4 else ''))
+    lead = tuple(q.shape[:-2])
+    H, D = q.shape[-2:]
+    HK, DV = k.shape[-2], v.shape[-1]
+    s = _lib.LinattnShape(code, H, HK, D, DV, 0, lead[0], lead[1] if dims == 4 else 1)
+    dt = q.dtype
+    return (s, dev, lead, _heads(q, s.q, dev, dt, q.shape, 'q'), _heads(k, s.k, dev, dt, lead + (HK, D), 'k'),
+            _heads(v, s.v, dev, dt, lead + (HK, DV), 'v'), _on(decay, dev, F32, (H,), 'decay'))
 
 
 def linattn(q, k, v, decay, scale=1.0, state=None, lengths=None, out=None, state_out=None, ws=None):
@@ -1055,53 +1066,50 @@ def linattn(q, k, v, decay, scale=1.0, state=None, lengths=None, out=None, state
     whole sequences: q [B, T, H, D], k [B, T, HK, D], v [B, T, HK, DV] in float32, bfloat16 or float16 (views of a joint
     projection may be given), decay float32 [H], state float32 [B, H, D, DV] before the first row (None: zero), lengths
     int32 [B] (None: T).  Returns (out [B, T, H, DV], the state behind the last row) (samx_linattn)."""
-    s = _linattn_args(q, k, v, decay)
+    s, dev, lead, pq, pk, pv, pd = _linattn_args(q, k, v, decay, 4)
     shape = (s.B, s.H, s.D, s.DV)
-    _opt_on(state, q, F32, shape, 'state'); _opt_on(lengths, q, I32, (s.B,), 'lengths')
-    made = out is None or state_out is None
-    out = torch.empty((s.B, s.T, s.H, s.DV), dtype=q.dtype, device=q.device) if out is None else \
-        _on(out, q, q.dtype, (s.B, s.T, s.H, s.DV), 'out')
-    state_out = torch.empty(shape, dtype=F32, device=q.device) if state_out is None else \
-        _on(state_out, q, F32, shape, 'state_out')
-    if not made:
-        _apart((('out', out), ('state_out', state_out)))
-    if state is not None and state.data_ptr() == state_out.data_ptr() and state.numel():
-        raise ValueError('state_out is state: the segments of a sequence read it while others write')
+    ps, pl = _opt_on(state, dev, F32, shape, 'state'), _opt_on(lengths, dev, I32, (s.B,), 'lengths')
+    if out is not None or state_out is not None:
+        _apart((('out', out), ('state_out', state_out), ('state', state)))
+    out = torch.empty(lead + (s.H, s.DV), dtype=q.dtype, device=dev) if out is None else out
+    state_out = torch.empty(shape, dtype=F32, device=dev) if state_out is None else state_out
     L = _L()
-    ws = _linattn_ws(s, ws, L.samx_linattn_ws_bytes(C.byref(s)), q)
-    check(L.samx_linattn(C.byref(s), q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr(decay), float(scale), ptr(state),
-                         ptr(lengths), ptr(out), ptr(state_out), ptr(ws), ws.numel(), stream_ptr()))
+    ws, pws, nws = _seq_ws(ws, L.samx_linattn_ws_bytes(C.byref(s)), dev)
+    check(L.samx_linattn(C.byref(s), pq, pk, pv, pd, scale, ps, pl, _on(out, dev, q.dtype, lead + (s.H, s.DV), 'out'),
+                         _on(state_out, dev, F32, shape, 'state_out'), pws, nws, _raw_stream(dev.index)))
     return out, state_out
 
 
 def linattn_grad(q, k, v, decay, dout, scale=1.0, state=None, dstate=None, lengths=None, ws=None):
     """The gradient of linattn from dout and dstate (of the state behind the last row, None: zero); decay counts as a
     constant.  Returns (dq, dk, dv, the gradient of the state before the first row) (samx_linattn_grad)."""
-    s = _linattn_args(q, k, v, decay, dout)
+    s, dev, lead, pq, pk, pv, pd = _linattn_args(q, k, v, decay, 4)
+    po = _heads(dout, s.o, dev, q.dtype, lead + (s.H, s.DV), 'dout')
     shape = (s.B, s.H, s.D, s.DV)
-    _opt_on(state, q, F32, shape, 'state'); _opt_on(dstate, q, F32, shape, 'dstate')
-    _opt_on(lengths, q, I32, (s.B,), 'lengths')
+    ps, pds = _opt_on(state, dev, F32, shape, 'state'), _opt_on(dstate, dev, F32, shape, 'dstate')
+    pl = _opt_on(lengths, dev, I32, (s.B,), 'lengths')
     L = _L()
-    ws = _linattn_ws(s, ws, L.samx_linattn_grad_ws_bytes(C.byref(s)), q)
-    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
-    ds = torch.empty(shape, dtype=F32, device=q.device)
-    check(L.samx_linattn_grad(C.byref(s), q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr(decay), dout.data_ptr(),
-                              float(scale), ptr(state), ptr(dstate), ptr(lengths), ptr(dq), ptr(dk), ptr(dv), ptr(ds),
-                              ptr(ws), ws.numel(), stream_ptr()))
+    ws, pws, nws = _seq_ws(ws, L.samx_linattn_grad_ws_bytes(C.byref(s)), dev)
+    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=dev) for t in (q, k, v))
+    ds = torch.empty(shape, dtype=F32, device=dev)
+    check(L.samx_linattn_grad(C.byref(s), pq, pk, pv, pd, po, scale, ps, pds, pl, dq.data_ptr(), dk.data_ptr(),
+                              dv.data_ptr(), ds.data_ptr(), pws, nws, _raw_stream(dev.index)))
     return dq, dk, dv, ds
 
 
 def linattn_step(q, k, v, decay, state, scale=1.0, out=None):
     """One row of each sequence (acting): q [B, H, D], k [B, HK, D], v [B, HK, DV], state float32 [B, H, D, DV], updated in
     place.  Returns out [B, H, DV] (samx_linattn_step)."""
-    if not all(isinstance(t, torch.Tensor) and t.dim() == 3 for t in (q, k, v)):
-        raise ValueError('q, k and v must be [batch, heads, dim]')
-    s = _linattn_args(q[:, None], k[:, None], v[:, None], decay)
-    _on(state, q, F32, (s.B, s.H, s.D, s.DV), 'state')
-    out = torch.empty((s.B, s.H, s.DV), dtype=q.dtype, device=q.device) if out is None else \
-        _on(out, q, q.dtype, (s.B, s.H, s.DV), 'out')
-    check(_L().samx_linattn_step(C.byref(s), q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr(decay), float(scale),
-                                 ptr(state), ptr(out), stream_ptr()))
+    s, dev, lead, pq, pk, pv, pd = _linattn_args(q, k, v, decay, 3)
+    shape = lead + (s.H, s.DV)
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=dev)
+        po = out.data_ptr()
+    else:
+        _apart((('out', out), ('state', state)))
+        po = _on(out, dev, q.dtype, shape, 'out')
+    check(_L().samx_linattn_step(C.byref(s), pq, pk, pv, pd, scale, _on(state, dev, F32, lead + (s.H, s.D, s.DV), 'state'),
+                                 po, _raw_stream(dev.index)))
     return out
 
 
@@ -1113,16 +1121,17 @@ def _rows2(t, name):
 
 
 def _distill_args(logits, idx, teacher, lse, weight, loss):
-    code = _seq_dtype(logits, 'logits')
+    code, dev = _seq_dtype(logits, 'logits')
     ld = _rows2(logits, 'logits')
     N, V = logits.shape
     if not (isinstance(idx, torch.Tensor) and idx.dim() == 2):
         raise ValueError('idx must be [rows, K]')
     K = idx.shape[1]
-    _on(idx, logits, I32, (N, K), 'idx'); _on(teacher, logits, F32, (N, K), 'teacher')
-    _opt_on(lse, logits, F32, (N,), 'lse'); _opt_on(weight, logits, F32, (N,), 'weight')
-    loss = torch.empty(N, dtype=F32, device=logits.device) if loss is None else _on(loss, logits, F32, (N,), 'loss')
-    return code, ld, N, V, K, loss
+    if loss is None:
+        loss = torch.empty(N, dtype=F32, device=dev)
+    return (dev, ld, N, V, K, loss, (logits.data_ptr(), ld, code, N, V, _on(idx, dev, I32, (N, K), 'idx'),
+                                     _on(teacher, dev, F32, (N, K), 'teacher'), K),
+            _opt_on(lse, dev, F32, (N,), 'lse'), _opt_on(weight, dev, F32, (N,), 'weight'), _on(loss, dev, F32, (N,), 'loss'))
 
 
 def distill_loss(logits, idx, teacher, tau=1.0, lse=None, weight=None, loss=None):
@@ -1130,9 +1139,8 @@ def distill_loss(logits, idx, teacher, tau=1.0, lse=None, weight=None, loss=None
     tau)[idx_k]) with p_k = exp(teacher_k / tau - lse) (lse None: normalised over the K entries).  logits [rows, V] in
     float32, bfloat16 or float16, rows may be apart; idx int32 [rows, K] (entries outside [0, V) do not count), teacher
     float32 [rows, K]; lse, weight float32 [rows] (samx_distill_loss)."""
-    code, ld, N, V, K, loss = _distill_args(logits, idx, teacher, lse, weight, loss)
-    check(_L().samx_distill_loss(C.c_void_p(logits.data_ptr()), ld, code, N, V, ptr(idx), ptr(teacher), K, float(tau),
-                                 ptr(lse), ptr(weight), ptr(loss), stream_ptr()))
+    dev, _, _, _, _, loss, a, pn, pw, pl = _distill_args(logits, idx, teacher, lse, weight, loss)
+    check(_L().samx_distill_loss(*a, tau, pn, pw, pl, _raw_stream(dev.index)))
     return loss
 
 
@@ -1140,18 +1148,16 @@ def distill_grad(logits, idx, teacher, tau=1.0, lse=None, weight=None, scale=1.0
     """distill_loss and the gradient of scale * its sum: (loss, grad).  grad has the logits' type and shape (and a row
     stride up to 255 columns wider than V); it may be given, the logits themselves among them; columns behind V stay as
     they were (samx_distill_grad)."""
-    code, ld, N, V, K, loss = _distill_args(logits, idx, teacher, lse, weight, loss)
+    dev, ld, N, V, K, loss, a, pn, pw, pl = _distill_args(logits, idx, teacher, lse, weight, loss)
     if grad is None:
-        grad = torch.empty((N, ld if V <= ld < V + 256 else V), dtype=logits.dtype, device=logits.device)[:, :V]
-    elif grad.dtype != logits.dtype or grad.shape != logits.shape or grad.device != logits.device:
-        raise ValueError('grad must be like logits: %s %s on %s' % (logits.dtype, tuple(logits.shape), logits.device))
-    ldg = _rows2(grad, 'grad')
-    if grad.data_ptr() != logits.data_ptr() and N:
-        a, b = logits.data_ptr(), grad.data_ptr()
-        e = logits.element_size()
-        if a < b + ((N - 1) * ldg + V) * e and b < a + ((N - 1) * ld + V) * e:
+        ldg = ld if V <= ld < V + 256 else V
+        grad = torch.empty((N, ldg), dtype=logits.dtype, device=dev)[:, :V]
+    else:
+        if grad.dtype != logits.dtype or grad.shape != logits.shape or grad.device != dev:
+            raise ValueError('grad must be like logits: %s %s on %s' % (logits.dtype, tuple(logits.shape), dev))
+        ldg = _rows2(grad, 'grad')
+        x, y, e = logits.data_ptr(), grad.data_ptr(), logits.element_size()
+        if x != y and N and x < y + ((N - 1) * ldg + V) * e and y < x + ((N - 1) * ld + V) * e:
             raise ValueError('grad overlaps the logits without being them')
-    check(_L().samx_distill_grad(C.c_void_p(logits.data_ptr()), ld, code, N, V, ptr(idx), ptr(teacher), K, float(tau),
-                                 ptr(lse), ptr(weight), float(scale), ptr(loss), C.c_void_p(grad.data_ptr()), ldg,
-                                 stream_ptr()))
+    check(_L().samx_distill_grad(*a, tau, pn, pw, scale, pl, grad.data_ptr(), ldg, _raw_stream(dev.index)))
     return loss, grad
