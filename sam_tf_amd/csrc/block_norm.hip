@@ -21,6 +21,8 @@ namespace {
 
 using namespace samx::seq;
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
 enum Gate { kNone = 0, kChannel = 1, kFull = 2 };
 
 struct Args {
@@ -38,9 +40,14 @@ struct Args {
 template <typename T, int G, int P>
 struct Cols {
     static constexpr int N = Piece<T>::kN, E = P * N;
+    static constexpr int R = (G < 256 ? 256 : G) / G;   // rows of the workgroup
     int D, at[P], first[P];               // first: elements that are the neighbour's (kN: all, no piece)
+    uint32_t slot;                        // which of the workgroup's rows (the same in a whole wave where it can be)
     uint32_t keep[P][4];
-    __device__ Cols(int D_, int lane) : D(D_) {
+    __device__ explicit Cols(int D_) : D(D_) {
+        const int lane = threadIdx.x % G;
+        slot = threadIdx.x / G;
+        if constexpr (G >= 64) slot = __builtin_amdgcn_readfirstlane(slot);
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             const int want = (p * G + lane) * N, last = D >= N ? D - N : 0;
@@ -57,41 +64,57 @@ struct Cols {
     __device__ __forceinline__ bool own(int i) const {
         return i % N >= first[i / N] && at[i / N] + i % N < D;
     }
+    __device__ __forceinline__ void channels(const float* w, int p, float* out) const {
+#pragma unroll
+        for (int j = 0; j < N; ++j) out[j] = own(p * N + j) ? w[at[p] + j] : 0.f;
+    }
     __device__ __forceinline__ void channels(const float* w, float (&out)[E]) const {
 #pragma unroll
-        for (int i = 0; i < E; ++i) out[i] = own(i) ? w[at[i / N] + i % N] : 0.f;
+        for (int p = 0; p < P; ++p) channels(w, p, out + p * N);
     }
-    __device__ __forceinline__ void load(const void* base, int64_t row, int64_t rows, Piece<T> (&r)[P]) const {
-        const T* x = (const T*)base + (row < rows ? row : 0) * (int64_t)D;
+    // The pieces of row first + slot as they stand in memory (some row's where there is none): nothing waits for them
+    // here.  The address is the workgroup's first row, and a 32-bit distance from it for each thread.
+    __device__ __forceinline__ void load(const void* base, int64_t first_row, int64_t rows, Piece<T> (&r)[P]) const {
+        const char* x = (const char*)base + (first_row < rows ? first_row : 0) * (int64_t)D * (int)sizeof(T);
+        const uint32_t mine = first_row + slot < rows ? slot * (uint32_t)D : 0u;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             if (D >= N) {
-                const Raw16 v = *reinterpret_cast<const Raw16*>(x + at[p]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) r[p].w[j] = row < rows ? v.w[j] & keep[p][j] : 0u;
+                const Raw16 v = *reinterpret_cast<const Raw16*>(x + (mine + (uint32_t)at[p]) * (uint32_t)sizeof(T));
+                __builtin_memcpy(&r[p], &v, 16);
             } else {
-                r[p] = load_piece(x, 0, row < rows && first[p] == 0 ? D : 0, 0u);
+                r[p] = load_piece((const T*)x + mine, 0, first[p] == 0 ? D : 0, 0u);
             }
         }
     }
-    __device__ __forceinline__ void store(void* base, int64_t row, const float (&v)[E]) const {
-        T* x = (T*)base + row * (int64_t)D;
+    // what of them is the thread's own, the rest zeros
+    __device__ __forceinline__ void take(const Piece<T> (&r)[P], bool live, Piece<T> (&c)[P]) const {
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            const Piece<T> o = pack<T>(v + p * N);
-            if (first[p] == 0 && D >= N) {
-                Raw16 r;
-                __builtin_memcpy(&r, &o, 16);
-                *reinterpret_cast<Raw16*>(x + at[p]) = r;
-            } else {
+        for (int p = 0; p < P; ++p)
 #pragma unroll
-                for (int j = 0; j < N; ++j)
-                    if (own(p * N + j)) {
-                        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(x + at[p] + j) = o.w[j];
-                        else *reinterpret_cast<uint16_t*>(x + at[p] + j) = (uint16_t)o.bits(j);
-                    }
-            }
+            for (int j = 0; j < 4; ++j) c[p].w[j] = r[p].w[j] & (live ? keep[p][j] : 0u);
+    }
+    // piece p of a row from kN values
+    __device__ __forceinline__ void store(void* base, int64_t first_row, int p, const float* v) const {
+        char* b = (char*)base + first_row * (int64_t)D * (int)sizeof(T);
+        T* x = (T*)(b + (slot * (uint32_t)D + (uint32_t)at[p]) * (uint32_t)sizeof(T));
+        const Piece<T> o = pack<T>(v);
+        if (first[p] == 0 && D >= N) {
+            Raw16 r;
+            __builtin_memcpy(&r, &o, 16);
+            *reinterpret_cast<Raw16*>(x) = r;
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (own(p * N + j)) {
+                    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(x + j) = o.w[j];
+                    else *reinterpret_cast<uint16_t*>(x + j) = (uint16_t)o.bits(j);
+                }
         }
+    }
+    __device__ __forceinline__ void store(void* base, int64_t first_row, const float (&v)[E]) const {
+#pragma unroll
+        for (int p = 0; p < P; ++p) store(base, first_row, p, v + p * N);
     }
 };
 
@@ -101,7 +124,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void forward_kernel(Args a) {
     __shared__ float sh[2 * W];
     int turn = 0;
     const int D = a.D;
-    const Cols<T, G, P> cols(D, threadIdx.x % G);
+    const Cols<T, G, P> cols(D);
     const float inv = 1.f / (float)D;
     float w1[E], w2[E], b1[E], b2[E];
     cols.channels(a.w1, w1);
@@ -120,17 +143,25 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void forward_kernel(Args a) {
         }
     }
     const int64_t step = (int64_t)gridDim.x * R;
-    int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / G;
+    const int64_t start = (int64_t)blockIdx.x * R;
     Piece<T> ry[P], rx[P], rg[P];
-    cols.load(a.y, row, a.N, ry);
-    cols.load(a.x, row, a.N, rx);
-    if constexpr (GATE == kFull) cols.load(a.gate, row, a.N, rg);
-    for (int64_t base = (int64_t)blockIdx.x * R; base < a.N; base += step, row += step) {
+    cols.load(a.y, start, a.N, ry);
+    cols.load(a.x, start, a.N, rx);
+    if constexpr (GATE == kFull) cols.load(a.gate, start, a.N, rg);
+    for (int64_t base = start; base < a.N; base += step) {
+        Piece<T> cy[P], cx[P], cg[P];
+        const bool live = base + cols.slot < a.N;
+        cols.take(ry, live, cy);
+        cols.take(rx, live, cx);
+        if constexpr (GATE == kFull) cols.take(rg, live, cg);
+        cols.load(a.y, base + step, a.N, ry);
+        cols.load(a.x, base + step, a.N, rx);
+        if constexpr (GATE == kFull) cols.load(a.gate, base + step, a.N, rg);
         float h[E];
         float v[1] = {0.f};
         if constexpr (LAYER) {
 #pragma unroll
-            for (int i = 0; i < E; ++i) { h[i] = ry[i / N].f(i % N); v[0] += h[i]; }
+            for (int i = 0; i < E; ++i) { h[i] = cy[i / N].f(i % N); v[0] += h[i]; }
             row_reduce<OpSum, G>(v, sh, W, turn);
             const float m = v[0] * inv;
             v[0] = 0.f;
@@ -138,17 +169,8 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void forward_kernel(Args a) {
             for (int i = 0; i < E; ++i) { h[i] = cols.own(i) ? h[i] - m : 0.f; v[0] += h[i] * h[i]; }
         } else {
 #pragma unroll
-            for (int i = 0; i < E; ++i) { h[i] = ry[i / N].f(i % N); v[0] += h[i] * h[i]; }
+            for (int i = 0; i < E; ++i) { h[i] = cy[i / N].f(i % N); v[0] += h[i] * h[i]; }
         }
-        float x[E], g[E];
-#pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = rx[i / N].f(i % N);
-        if constexpr (GATE == kFull)
-#pragma unroll
-            for (int i = 0; i < E; ++i) g[i] = rg[i / N].f(i % N);
-        cols.load(a.y, row + step, a.N, ry);
-        cols.load(a.x, row + step, a.N, rx);
-        if constexpr (GATE == kFull) cols.load(a.gate, row + step, a.N, rg);
         row_reduce<OpSum, G>(v, sh, W, turn);
         const float sy = 1.f / sqrtf(v[0] * inv + a.eps);
         v[0] = 0.f;
@@ -156,11 +178,11 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void forward_kernel(Args a) {
         for (int i = 0; i < E; ++i) {
             float n = h[i] * sy * w1[i];
             if constexpr (LAYER) n += b1[i];
-            if constexpr (GATE == kFull) n *= g[i];
-            h[i] = a.res * x[i] + n;
+            if constexpr (GATE == kFull) n *= cg[i / N].f(i % N);
+            h[i] = a.res * cx[i / N].f(i % N) + n;
             v[0] += LAYER ? h[i] : h[i] * h[i];
         }
-        if (row < a.N) cols.store(a.o1, row, h);
+        if (live) cols.store(a.o1, base, h);
         row_reduce<OpSum, G>(v, sh, W, turn);
         if constexpr (LAYER) {
             const float m = v[0] * inv;
@@ -175,7 +197,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void forward_kernel(Args a) {
             h[i] = h[i] * su * w2[i];
             if constexpr (LAYER) h[i] += b2[i];
         }
-        if (row < a.N) cols.store(a.o2, row, h);
+        if (live) cols.store(a.o2, base, h);
     }
 }
 
@@ -189,104 +211,152 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 4) void backward_kernel(Args a) 
     __shared__ float sh[2 * W * 4];
     int turn = 0;
     const int D = a.D;
-    const Cols<T, G, P> cols(D, threadIdx.x % G);
+    const Cols<T, G, P> cols(D);
     const float inv = 1.f / (float)D;
-    float w1[E], w2[E], b1[E];
-    cols.channels(a.w1, w1);
-    cols.channels(a.w2, w2);
-    if constexpr (LAYER && GATE == kFull) cols.channels(a.b1, b1);
-    if constexpr (GATE == kChannel) {
-        float gc[E];
-        cols.channels((const float*)a.gate, gc);
+    // The channels' parameters stand in LDS, each thread's own (so nothing waits for another's), and leave the registers
+    // to the sums: in registers the LayerNorm of 16-bit rows spilt 30 to 60 of them and took 403 us for 16384 x 4096.
+    constexpr int kB1 = LAYER && GATE == kFull && P == 1;
+    __shared__ f32x4 par[2 + kB1][E / 4][B];
+    const auto keep_own = [&](int which, const float (&v)[E]) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) w1[i] *= gc[i];
+        for (int i = 0; i < E; i += 4) par[which][i / 4][threadIdx.x] = (f32x4){v[i], v[i + 1], v[i + 2], v[i + 3]};
+    };
+    const auto own_of = [&](int which, int p, float (&v)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const f32x4 x = par[which][(p * N + i) / 4][threadIdx.x];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[i + j] = x[j];
+        }
+    };
+    {
+        float w[E], gc[E];
+        cols.channels(a.w2, w);
+        keep_own(1, w);
+        cols.channels(a.w1, w);
+        if constexpr (GATE == kChannel) {
+            cols.channels((const float*)a.gate, gc);
+#pragma unroll
+            for (int i = 0; i < E; ++i) w[i] *= gc[i];
+        }
+        keep_own(0, w);
+        if constexpr (kB1) {
+            cols.channels(a.b1, w);
+            keep_own(2, w);
+        }
     }
     float sa[E], sw[E], sb[E], sv[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) sa[i] = sw[i] = sb[i] = sv[i] = 0.f;
     const int64_t step = (int64_t)gridDim.x * R;
-    int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / G;
+    const int64_t start = (int64_t)blockIdx.x * R;
+    // The next row's pieces are fetched ahead where a thread holds one piece of a row; where it holds two the registers
+    // are needed for the sums.  The current row's stay packed (unpacked again at each use).
+    constexpr bool kAhead = P == 1;
     Piece<T> ry[P], rh[P], rdu[P], rdh[P], rg[P];
-    cols.load(a.y, row, a.N, ry);
-    cols.load(a.h, row, a.N, rh);
-    cols.load(a.du, row, a.N, rdu);
-    cols.load(a.dh, row, a.N, rdh);
-    if constexpr (GATE == kFull) cols.load(a.gate, row, a.N, rg);
-    for (int64_t base = (int64_t)blockIdx.x * R; base < a.N; base += step, row += step) {
-        float y[E], h[E], du[E], dh[E], g[E];
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            y[i] = ry[i / N].f(i % N);
-            h[i] = rh[i / N].f(i % N);
-            du[i] = rdu[i / N].f(i % N);
-            dh[i] = rdh[i / N].f(i % N);
-            if constexpr (GATE == kFull) g[i] = rg[i / N].f(i % N);
-        }
-        cols.load(a.y, row + step, a.N, ry);
-        cols.load(a.h, row + step, a.N, rh);
-        cols.load(a.du, row + step, a.N, rdu);
-        cols.load(a.dh, row + step, a.N, rdh);
-        if constexpr (GATE == kFull) cols.load(a.gate, row + step, a.N, rg);
+    auto load = [&](int64_t r) {
+        cols.load(a.y, r, a.N, ry);
+        cols.load(a.h, r, a.N, rh);
+        cols.load(a.du, r, a.N, rdu);
+        cols.load(a.dh, r, a.N, rdh);
+        if constexpr (GATE == kFull) cols.load(a.gate, r, a.N, rg);
+    };
+    if constexpr (kAhead) load(start);
+    for (int64_t base = start; base < a.N; base += step) {
+        if constexpr (!kAhead) load(base);
+        const bool live = base + cols.slot < a.N;
+        Piece<T> y[P], h[P], du[P], dh[P], g[P];
+        cols.take(ry, live, y);
+        cols.take(rh, live, h);
+        cols.take(rdu, live, du);
+        cols.take(rdh, live, dh);
+        if constexpr (GATE == kFull) cols.take(rg, live, g);
+        forget(y);
+        forget(h);
+        forget(du);
+        forget(dh);
+        if constexpr (GATE == kFull) forget(g);
+        if constexpr (kAhead) load(base + step);
+        float my = 0.f, mh = 0.f;
         if constexpr (LAYER) {
             float v[2] = {0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < E; ++i) { v[0] += y[i]; v[1] += h[i]; }
+            for (int i = 0; i < E; ++i) { v[0] += y[i / N].f(i % N); v[1] += h[i / N].f(i % N); }
             row_reduce<OpSum, G>(v, sh, W, turn);
-            const float my = v[0] * inv, mh = v[1] * inv;
+            my = v[0] * inv;
+            mh = v[1] * inv;
+            forget(y);
+            forget(h);
+        }
+        // {sum y^2, sum h^2, sum k h, sum k}, k = w2 du (zero where an element is not the thread's own)
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        asm volatile("" ::: "memory");   // (the parameters are read again for each row, not kept)
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const bool in = cols.own(i);
-                y[i] = in ? y[i] - my : 0.f;
-                h[i] = in ? h[i] - mh : 0.f;
+        for (int p = 0; p < P; ++p) {
+            float w2[N];
+            own_of(1, p, w2);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const float k = du[p].f(j) * w2[j], yc = y[p].f(j) - my, hc = h[p].f(j) - mh;
+                const bool in = !LAYER || cols.own(p * N + j);
+                v[0] += in ? yc * yc : 0.f;
+                v[1] += in ? hc * hc : 0.f;
+                v[2] += k * hc;
+                if constexpr (LAYER) v[3] += k;
             }
         }
-        // {sum y^2, sum h^2, sum k h, sum k}, k = w2 du
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const float k = du[i] * w2[i];
-            v[0] += y[i] * y[i];
-            v[1] += h[i] * h[i];
-            v[2] += k * h[i];
-            if constexpr (LAYER) v[3] += k;
-        }
         row_reduce<OpSum, G>(v, sh, W, turn);
+        forget(y);
+        forget(h);
+        forget(du);
         // (a group without a row adds nothing: its spread is not one over a zero)
-        const float sy = row < a.N ? 1.f / sqrtf(v[0] * inv + a.eps) : 0.f;
-        const float s = row < a.N ? 1.f / sqrtf(v[1] * inv + a.eps) : 0.f;
+        const float sy = live ? 1.f / sqrtf(v[0] * inv + a.eps) : 0.f;
+        const float s = live ? 1.f / sqrtf(v[1] * inv + a.eps) : 0.f;
         const float kh = v[2] * s * inv, km = LAYER ? v[3] * inv : 0.f;
-        // dh becomes the whole gradient of h, y the normalised y, h k', du the gate's gradient
-        float t[2] = {0.f, 0.f};
+        float kp[E], t[2] = {0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const float hh = h[i] * s;
-            dh[i] += s * (du[i] * w2[i] - hh * kh - km);
-            sw[i] += du[i] * hh;
-            if constexpr (LAYER) sv[i] += du[i];
-            y[i] *= sy;
-            float dn = dh[i];
-            if constexpr (GATE == kFull) dn *= g[i];
-            sa[i] += dn * y[i];
-            if constexpr (LAYER) sb[i] += dn;
-            h[i] = dn * w1[i];
-            t[0] += h[i] * y[i];
-            if constexpr (LAYER) t[1] += h[i];
-            if constexpr (GATE == kFull) du[i] = dh[i] * (LAYER ? y[i] * w1[i] + b1[i] : y[i] * w1[i]);
-            dh[i] *= a.res;
-        }
-        if (row < a.N) {
-            cols.store(a.o1, row, dh);
-            if constexpr (GATE == kFull) cols.store(a.og, row, du);
+        for (int p = 0; p < P; ++p) {
+            float dx[N], dg[N], w1[N], w2[N], b1[N];
+            own_of(0, p, w1);
+            own_of(1, p, w2);
+            if constexpr (kB1) own_of(2, p, b1);
+            else if constexpr (LAYER && GATE == kFull) cols.channels(a.b1, p, b1);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int i = p * N + j;
+                const float hh = (h[p].f(j) - mh) * s, yh = (y[p].f(j) - my) * sy, d = du[p].f(j);
+                const float all = dh[p].f(j) + s * (d * w2[j] - hh * kh - km);
+                float dn = all;
+                if constexpr (GATE == kFull) dn *= g[p].f(j);
+                sw[i] += d * hh;
+                sa[i] += dn * yh;
+                if constexpr (LAYER) { sv[i] += d; sb[i] += dn; }
+                kp[i] = dn * w1[j];
+                t[0] += kp[i] * yh;
+                if constexpr (LAYER) t[1] += kp[i];
+                if constexpr (GATE == kFull) dg[j] = all * (LAYER ? yh * w1[j] + b1[j] : yh * w1[j]);
+                dx[j] = a.res * all;
+            }
+            if (live) {
+                cols.store(a.o1, base, p, dx);
+                if constexpr (GATE == kFull) cols.store(a.og, base, p, dg);
+            }
         }
         row_reduce<OpSum, G>(t, sh, W, turn);
+        forget(y);
         const float ky = t[0] * inv, kn = LAYER ? t[1] * inv : 0.f;
 #pragma unroll
-        for (int i = 0; i < E; ++i) h[i] = sy * (h[i] - y[i] * ky - kn);
-        if (row < a.N) cols.store(a.o2, row, h);
+        for (int p = 0; p < P; ++p) {
+            float o[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) o[j] = sy * (kp[p * N + j] - (y[p].f(j) - my) * sy * ky - kn);
+            if (live) cols.store(a.o2, base, p, o);
+        }
     }
-    // this row group's sums; the groups of a wave are added first
+    // the workgroup's sums: groups of a wave first, then its waves one after the other
     constexpr int S = kSums<LAYER>, GW = G < 64 ? 64 : G;
-    float* part = a.part + ((int64_t)blockIdx.x * (B / GW) + threadIdx.x / GW) * S * D;
+    float* part = a.part + (int64_t)blockIdx.x * S * D;
+    float all[4][E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
         float v[4] = {sa[i], sw[i], sb[i], sv[i]};
@@ -294,10 +364,29 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 4) void backward_kernel(Args a) 
         for (int o = G; o < 64; o <<= 1)
 #pragma unroll
             for (int c = 0; c < S; ++c) v[c] += __shfl_xor(v[c], o, 64);
-        if (cols.own(i) && threadIdx.x % GW < G)
 #pragma unroll
-            for (int c = 0; c < S; ++c) part[c * D + cols.at[i / N] + i % N] = v[c];
+        for (int c = 0; c < S; ++c) all[c][i] = v[c];
     }
+    if constexpr (GW < B) {
+        __shared__ float red[E][B];
+#pragma unroll
+        for (int c = 0; c < S; ++c) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < E; ++i) red[i][threadIdx.x] = all[c][i];
+            __syncthreads();
+            if (threadIdx.x < G)
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    for (int w = GW; w < B; w += GW) all[c][i] += red[i][threadIdx.x + w];
+        }
+    }
+    if (threadIdx.x < G)
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (cols.own(i))
+#pragma unroll
+                for (int c = 0; c < S; ++c) part[c * D + cols.at[i / N] + i % N] = all[c][i];
 }
 
 struct Columns { const float *w1, *b1, *gate; float *dw1, *dw2, *db1, *db2, *dgate; };
@@ -347,9 +436,6 @@ int grid_of(int64_t N, int threads_row) {
     const int64_t most = (int64_t)cu_count() * (1024 / block), want = (N + R - 1) / R;
     return (int)(want < most ? want : most);
 }
-
-// column sums that a workgroup leaves
-int parts_of(int threads_row) { return threads_row <= 64 ? 4 : threads_row <= 256 ? 256 / threads_row : 1; }
 
 template <typename T, bool LAYER, int GATE, bool BACK>
 int launch(const Args& a, int G, int grid, hipStream_t st) {
@@ -424,7 +510,7 @@ int samx_block_norm(const void* x, const void* y, int dtype, int64_t N, int64_t 
 size_t samx_block_norm_grad_ws_bytes(int dtype, int64_t N, int64_t D) {
     if (dtype < 0 || dtype > 2 || N < 0 || D <= 0 || D > most_dim(dtype)) return 0;
     const int G = threads_of(dtype, (int)D);
-    return (size_t)grid_of(N, G) * parts_of(G) * 4 * D * sizeof(float) + 256;
+    return (size_t)grid_of(N, G) * 4 * D * sizeof(float) + 256;
 }
 
 int samx_block_norm_grad(const void* y, const void* h, const void* dh, const void* du, int dtype, int64_t N, int64_t D,
@@ -456,8 +542,8 @@ int samx_block_norm_grad(const void* y, const void* h, const void* dh, const voi
     const Columns c{post_w, post_b, channel ? (const float*)gate : nullptr, dpost_w, dpre_w, dpost_b, dpre_b,
                     channel ? (float*)dgate : nullptr};
     const unsigned blocks = (unsigned)((D + 15) / 16);
-    if (kind == SAMX_NORM_LAYER) column_kernel<true><<<blocks, 1024, 0, st>>>((const float*)ws, grid * parts_of(G), (int)D, c);
-    else column_kernel<false><<<blocks, 1024, 0, st>>>((const float*)ws, grid * parts_of(G), (int)D, c);
+    if (kind == SAMX_NORM_LAYER) column_kernel<true><<<blocks, 1024, 0, st>>>((const float*)ws, grid, (int)D, c);
+    else column_kernel<false><<<blocks, 1024, 0, st>>>((const float*)ws, grid, (int)D, c);
     SAMX_LAUNCH_CHECK();
     return SAMX_OK;
 }
