@@ -68,6 +68,15 @@ struct Cols {
 #pragma unroll
         for (int j = 0; j < N; ++j) out[j] = own(p * N + j) ? w[at[p] + j] : 0.f;
     }
+    // the same of a row of at least a piece, the neighbour's elements with it
+    __device__ __forceinline__ void channels_all(const float* w, int p, float* out) const {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            const Raw16 v = *reinterpret_cast<const Raw16*>((const char*)w + (uint32_t)(at[p] + j) * 4u);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) out[j + u] = __uint_as_float(v.w[u]);
+        }
+    }
     __device__ __forceinline__ void channels(const float* w, float (&out)[E]) const {
 #pragma unroll
         for (int p = 0; p < P; ++p) channels(w, p, out + p * N);
@@ -205,8 +214,14 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void forward_kernel(Args a) {
 // gate is a factor of its sums: dw1 = g A, db1 = g B, dgate = w1 A + b1 B.
 template <bool LAYER> constexpr int kSums = LAYER ? 4 : 2;
 
+// Waves a SIMD that the gradient's registers leave room for.  Four are better than fewer as long as little is spilt
+// (16384 x 4096 bf16 LayerNorm: 225 us with 16 registers spilt, 273 us with two waves and none); with a full gate 40 are,
+// and fewer waves win (377 us against 291; 16384 x 1024: 124 against 94 with three).
+template <typename T, int G, bool LAYER, int GATE>
+constexpr int kWaves = LAYER && GATE == kFull && sizeof(T) == 2 && G <= 512 ? G == 512 ? 2 : 3 : 4;
+
 template <typename T, int G, int P, bool LAYER, int GATE>
-__global__ __launch_bounds__(G < 256 ? 256 : G, 4) void backward_kernel(Args a) {
+__global__ __launch_bounds__(G < 256 ? 256 : G, (kWaves<T, G, LAYER, GATE>)) void backward_kernel(Args a) {
     constexpr int B = G < 256 ? 256 : G, W = B / 64, N = Piece<T>::kN, E = P * N, R = B / G;
     __shared__ float sh[2 * W * 4];
     int turn = 0;
@@ -215,44 +230,71 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 4) void backward_kernel(Args a) 
     const float inv = 1.f / (float)D;
     // The channels' parameters stand in LDS, each thread's own (so nothing waits for another's), and leave the registers
     // to the sums: in registers the LayerNorm of 16-bit rows spilt 30 to 60 of them and took 403 us for 16384 x 4096.
-    constexpr int kB1 = LAYER && GATE == kFull && P == 1;
-    __shared__ f32x4 par[2 + kB1][E / 4][B];
-    const auto keep_own = [&](int which, const float (&v)[E]) {
+    // Where a thread holds two pieces of a row (kTwo) two of the sums stand there instead, and the parameters are read
+    // from the cache for each row: either alone leaves 100 registers and more spilt (4096 x 16384 RMS: 460 us).
+    constexpr bool kTwo = P > 1;
+    constexpr int kB1 = LAYER && GATE == kFull && !kTwo;
+    __shared__ f32x4 mine[2 + kB1][E / 4][B];
+    const auto put = [&](int which, const float (&v)[E]) {
 #pragma unroll
-        for (int i = 0; i < E; i += 4) par[which][i / 4][threadIdx.x] = (f32x4){v[i], v[i + 1], v[i + 2], v[i + 3]};
+        for (int i = 0; i < E; i += 4) mine[which][i / 4][threadIdx.x] = (f32x4){v[i], v[i + 1], v[i + 2], v[i + 3]};
     };
-    const auto own_of = [&](int which, int p, float (&v)[N]) {
+    const auto get = [&](int which, int p, float (&v)[N]) {
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
-            const f32x4 x = par[which][(p * N + i) / 4][threadIdx.x];
+            const f32x4 x = mine[which][(p * N + i) / 4][threadIdx.x];
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[i + j] = x[j];
         }
     };
-    {
-        float w[E], gc[E];
+    const auto add = [&](int which, int p, const float (&v)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) mine[which][(p * N + i) / 4][threadIdx.x] += (f32x4){v[i], v[i + 1], v[i + 2], v[i + 3]};
+    };
+    const auto w1_of = [&](int p, float (&v)[N]) {   // a channel's gate is a factor of its weight
+        if constexpr (!kTwo) get(0, p, v);
+        else {
+            cols.channels_all(a.w1, p, v);
+            if constexpr (GATE == kChannel) {
+                float gc[N];
+                cols.channels_all((const float*)a.gate, p, gc);
+#pragma unroll
+                for (int j = 0; j < N; ++j) v[j] *= gc[j];
+            }
+        }
+    };
+    const auto w2_of = [&](int p, float (&v)[N]) {
+        if constexpr (!kTwo) get(1, p, v);
+        else cols.channels_all(a.w2, p, v);
+    };
+    float sa[E], sw[E], sb[E], sv[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) sa[i] = sw[i] = sb[i] = sv[i] = 0.f;
+    if constexpr (kTwo) {
+        put(0, sa);
+        put(1, sw);
+    } else {
+        float w[E];
         cols.channels(a.w2, w);
-        keep_own(1, w);
+        put(1, w);
         cols.channels(a.w1, w);
         if constexpr (GATE == kChannel) {
+            float gc[E];
             cols.channels((const float*)a.gate, gc);
 #pragma unroll
             for (int i = 0; i < E; ++i) w[i] *= gc[i];
         }
-        keep_own(0, w);
+        put(0, w);
         if constexpr (kB1) {
             cols.channels(a.b1, w);
-            keep_own(2, w);
+            put(2, w);
         }
     }
-    float sa[E], sw[E], sb[E], sv[E];
-#pragma unroll
-    for (int i = 0; i < E; ++i) sa[i] = sw[i] = sb[i] = sv[i] = 0.f;
     const int64_t step = (int64_t)gridDim.x * R;
     const int64_t start = (int64_t)blockIdx.x * R;
     // The next row's pieces are fetched ahead where a thread holds one piece of a row; where it holds two the registers
     // are needed for the sums.  The current row's stay packed (unpacked again at each use).
-    constexpr bool kAhead = P == 1;
+    constexpr bool kAhead = !kTwo;
     Piece<T> ry[P], rh[P], rdu[P], rdh[P], rg[P];
     auto load = [&](int64_t r) {
         cols.load(a.y, r, a.N, ry);
@@ -294,7 +336,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 4) void backward_kernel(Args a) 
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             float w2[N];
-            own_of(1, p, w2);
+            w2_of(p, w2);
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 const float k = du[p].f(j) * w2[j], yc = y[p].f(j) - my, hc = h[p].f(j) - mh;
@@ -316,11 +358,11 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 4) void backward_kernel(Args a) 
         float kp[E], t[2] = {0.f, 0.f};
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            float dx[N], dg[N], w1[N], w2[N], b1[N];
-            own_of(0, p, w1);
-            own_of(1, p, w2);
-            if constexpr (kB1) own_of(2, p, b1);
-            else if constexpr (LAYER && GATE == kFull) cols.channels(a.b1, p, b1);
+            float dx[N], dg[N], w1[N], w2[N], b1[N], ta[N], tw[N];
+            w1_of(p, w1);
+            w2_of(p, w2);
+            if constexpr (kB1) get(2, p, b1);
+            else if constexpr (LAYER && GATE == kFull) cols.channels_all(a.b1, p, b1);
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 const int i = p * N + j;
@@ -328,14 +370,18 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 4) void backward_kernel(Args a) 
                 const float all = dh[p].f(j) + s * (d * w2[j] - hh * kh - km);
                 float dn = all;
                 if constexpr (GATE == kFull) dn *= g[p].f(j);
-                sw[i] += d * hh;
-                sa[i] += dn * yh;
+                if constexpr (kTwo) { tw[j] = d * hh; ta[j] = dn * yh; }
+                else { sw[i] += d * hh; sa[i] += dn * yh; }
                 if constexpr (LAYER) { sv[i] += d; sb[i] += dn; }
-                kp[i] = dn * w1[j];
+                kp[i] = LAYER && kTwo && !cols.own(i) ? 0.f : dn * w1[j];
                 t[0] += kp[i] * yh;
                 if constexpr (LAYER) t[1] += kp[i];
                 if constexpr (GATE == kFull) dg[j] = all * (LAYER ? yh * w1[j] + b1[j] : yh * w1[j]);
                 dx[j] = a.res * all;
+            }
+            if constexpr (kTwo) {
+                add(0, p, ta);
+                add(1, p, tw);
             }
             if (live) {
                 cols.store(a.o1, base, p, dx);
@@ -356,6 +402,17 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, 4) void backward_kernel(Args a) 
     // the workgroup's sums: groups of a wave first, then its waves one after the other
     constexpr int S = kSums<LAYER>, GW = G < 64 ? 64 : G;
     float* part = a.part + (int64_t)blockIdx.x * S * D;
+    if constexpr (kTwo)
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            float t[N];
+            get(0, p, t);
+#pragma unroll
+            for (int j = 0; j < N; ++j) sa[p * N + j] = t[j];
+            get(1, p, t);
+#pragma unroll
+            for (int j = 0; j < N; ++j) sw[p * N + j] = t[j];
+        }
     float all[4][E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
@@ -430,10 +487,10 @@ template <typename T> int row_threads(int D) {
     return n <= 8 ? 8 : n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : n <= 512 ? 512 : 1024;
 }
 
-// workgroups: as many as the device holds at once (two waves of work each a SIMD), each row group with a row at least
-int grid_of(int64_t N, int threads_row) {
+// workgroups: as many as the device holds at once (`waves` a SIMD), each row group with a row at least
+int grid_of(int64_t N, int threads_row, int waves = 4) {
     const int block = threads_row < 256 ? 256 : threads_row, R = block / threads_row;
-    const int64_t most = (int64_t)cu_count() * (1024 / block), want = (N + R - 1) / R;
+    const int64_t most = (int64_t)cu_count() * (256 * waves / block), want = (N + R - 1) / R;
     return (int)(want < most ? want : most);
 }
 
@@ -530,7 +587,9 @@ int samx_block_norm_grad(const void* y, const void* h, const void* dh, const voi
     Args a{};
     a.y = y; a.h = h; a.dh = dh; a.du = du; a.gate = gate; a.w1 = post_w; a.b1 = post_b; a.w2 = pre_w;
     a.o1 = dx; a.o2 = dy; a.og = dgate; a.part = (float*)ws; a.N = N; a.D = (int)D; a.res = res_scale; a.eps = eps;
-    const int G = threads_of(dtype, (int)D), grid = grid_of(N, G);
+    const int G = threads_of(dtype, (int)D);
+    const bool fewer = kind == SAMX_NORM_LAYER && gate_kind == kFull && dtype != kF32 && G <= 512;   // (kWaves)
+    const int grid = grid_of(N, G, fewer ? G == 512 ? 2 : 3 : 4);
     const hipStream_t st = (hipStream_t)stream;
     if (N > 0) {
         const int rc = dtype == kF32 ? pick<float, true>(a, G, grid, kind, gate_kind, st)
