@@ -634,21 +634,21 @@ __global__ __launch_bounds__(256) void group_kernel(const float* __restrict__ in
     out[e] = from_float<T>(v);
 }
 
-// One row: S <- l S + k v^T, out = c q^T S, in place.  A workgroup has C columns of a state (16 bytes for each of C / 4
-// lanes); its other lanes take the rows by turns.
+// One row: S <- l S + k v^T, out = c q^T S, in place.  A workgroup has a head's state (four columns for each of cols / 4
+// lanes); the other lanes take the rows by turns.
 template <typename T>
 __global__ __launch_bounds__(256) void step_kernel(Mat Q, Mat K, Mat V, const float* __restrict__ decay, float* __restrict__ state,
-                                                   T* __restrict__ out, int H, int D, int DV, float scale, int cols, int per_head) {
+                                                   T* __restrict__ out, int H, int D, int DV, float scale, int cols) {
     __shared__ float sq[kMaxDim], sk[kMaxDim];
     __shared__ float part[256 * 4];
-    const int64_t unit = blockIdx.x / per_head;
-    const int h = (int)(unit % H), c0 = (int)(blockIdx.x % per_head) * cols;
+    const int64_t unit = blockIdx.x;
+    const int h = (int)(unit % H);
     const int64_t b = unit / H;
     const T* q = (const T*)Q.p + b * Q.sb + h * Q.sh;
     const T* k = (const T*)K.p + b * K.sb + (int64_t)(h / K.grp) * K.sh;
     const T* v = (const T*)V.p + b * V.sb + (int64_t)(h / V.grp) * V.sh;
     for (int i = threadIdx.x; i < D; i += 256) { sq[i] = to_float(q[i]); sk[i] = to_float(k[i]); }
-    const int lanes = cols / 4, c = c0 + threadIdx.x % lanes * 4, rows = 256 / lanes;
+    const int lanes = cols / 4, c = threadIdx.x % lanes * 4, rows = 256 / lanes;
     float ve[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) ve[e] = c + e < DV ? to_float(v[c + e]) : 0.f;
@@ -670,10 +670,10 @@ __global__ __launch_bounds__(256) void step_kernel(Mat Q, Mat K, Mat V, const fl
     for (int e = 0; e < 4; ++e) part[threadIdx.x * 4 + e] = acc[e];
     __syncthreads();
     const int col = threadIdx.x;
-    if (col < cols && c0 + col < DV) {
+    if (col < DV) {
         float o = 0.f;
         for (int i = 0; i < rows; ++i) o += part[i * cols + col];
-        out[(b * H + h) * DV + c0 + col] = from_float<T>(o * scale);
+        out[(b * H + h) * DV + col] = from_float<T>(o * scale);
     }
 }
 
@@ -867,12 +867,11 @@ int samx_linattn_step(const samx_linattn_shape* s, const void* q, const void* k,
     const Mat Q = mat(q, s->q, 1, s->D), K = mat(k, s->k, rep, s->D), V = mat(v, s->v, rep, s->DV);
     int cols = 16;
     while (cols < s->DV && cols < 128) cols *= 2;
-    const int per = (s->DV + cols - 1) / cols;
-    const unsigned g = (unsigned)(s->B * s->H * per);
+    const unsigned g = (unsigned)(s->B * s->H);
     const hipStream_t st = (hipStream_t)stream;
-    if (s->dtype == kF32) step_kernel<float><<<g, 256, 0, st>>>(Q, K, V, decay, state, (float*)out, s->H, s->D, s->DV, scale, cols, per);
-    else if (s->dtype == kBF16) step_kernel<bf16><<<g, 256, 0, st>>>(Q, K, V, decay, state, (bf16*)out, s->H, s->D, s->DV, scale, cols, per);
-    else step_kernel<f16><<<g, 256, 0, st>>>(Q, K, V, decay, state, (f16*)out, s->H, s->D, s->DV, scale, cols, per);
+    if (s->dtype == kF32) step_kernel<float><<<g, 256, 0, st>>>(Q, K, V, decay, state, (float*)out, s->H, s->D, s->DV, scale, cols);
+    else if (s->dtype == kBF16) step_kernel<bf16><<<g, 256, 0, st>>>(Q, K, V, decay, state, (bf16*)out, s->H, s->D, s->DV, scale, cols);
+    else step_kernel<f16><<<g, 256, 0, st>>>(Q, K, V, decay, state, (f16*)out, s->H, s->D, s->DV, scale, cols);
     SAMX_LAUNCH_CHECK();
     return SAMX_OK;
 }
