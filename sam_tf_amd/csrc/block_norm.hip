@@ -324,7 +324,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, (kWaves<T, G, LAYER, GATE>)) voi
             float v[2] = {0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < E; ++i) { v[0] += y[i / N].f(i % N); v[1] += h[i / N].f(i % N); }
-            row_reduce<OpSum, G>(v, sh, W, turn);
+            row_reduce<OpSum, G>(v, sh, 4 * W, turn);
             my = v[0] * inv;
             mh = v[1] * inv;
             forget(y);
@@ -347,7 +347,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, (kWaves<T, G, LAYER, GATE>)) voi
                 if constexpr (LAYER) v[3] += k;
             }
         }
-        row_reduce<OpSum, G>(v, sh, W, turn);
+        row_reduce<OpSum, G>(v, sh, 4 * W, turn);
         forget(y);
         forget(h);
         forget(du);
@@ -388,7 +388,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, (kWaves<T, G, LAYER, GATE>)) voi
                 if constexpr (GATE == kFull) cols.store(a.og, base, p, dg);
             }
         }
-        row_reduce<OpSum, G>(t, sh, W, turn);
+        row_reduce<OpSum, G>(t, sh, 4 * W, turn);
         forget(y);
         const float ky = t[0] * inv, kn = LAYER ? t[1] * inv : 0.f;
 #pragma unroll

@@ -143,7 +143,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void row_kernel(Args a) {
     for (int v = 0; v < NV; ++v)
 #pragma unroll
         for (int j = 0; j < N; ++j) mx[0] = OpMax::f(mx[0], raw[v].f(j));
-    row_reduce<OpMax, G>(mx, shf, W, turn);
+    row_reduce<OpMax, G>(mx, shf, 2 * W, turn);
     forget(raw);
     RowStat r;
     r.m = mx[0] == -INFINITY ? 0.f : mx[0];
@@ -153,14 +153,14 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void row_kernel(Args a) {
     for (int v = 0; v < NV; ++v)
 #pragma unroll
         for (int j = 0; j < N; ++j) s[0] += __builtin_amdgcn_exp2f((raw[v].f(j) - r.m) * c2);
-    row_reduce<OpSum, G>(s, shf, W, turn);
+    row_reduce<OpSum, G>(s, shf, 2 * W, turn);
     r.rs = s[0] > 0.f || s[0] != s[0] ? 1.f / s[0] : 0.f;
     const double lse_z = row_lse(r.m, s[0], a.inv_tau);
     double lse_t = 0.0;
     if (on) lse_t = a.lse ? (double)a.lse[row] : row_lse(mt, s[1], a.inv_tau);
     double tl[2];
     te.terms(a.inv_tau, lse_t, lse_z, lane, tl);
-    row_reduce<OpSum, G>(tl, shd, W, turnd);
+    row_reduce<OpSum, G>(tl, shd, 2 * W, turnd);
     if (live && lane == 0) a.loss[row] = on ? (float)((double)w * tl[1]) : 0.f;
     if constexpr (GRAD) {
         const float cp = on ? (float)(a.scale * (double)w) : 0.f, cq = on ? (float)(a.scale * (double)w * tl[0]) : 0.f;
@@ -222,19 +222,19 @@ __global__ __launch_bounds__(1024) void wide_kernel(Args a) {
         mx[0] = m;
     }
     const float own = mx[0];
-    row_reduce<OpMax, G>(mx, shf, W, turn);
+    row_reduce<OpMax, G>(mx, shf, 2 * W, turn);
     RowStat r;
     r.m = mx[0] == -INFINITY ? 0.f : mx[0];
     const float mt = mx[1] == -INFINITY ? 0.f : mx[1];
     float s[2] = {part * __builtin_amdgcn_exp2f((own - r.m) * c2), a.lse ? 0.f : te.sum(mt, c2, lane)};
-    row_reduce<OpSum, G>(s, shf, W, turn);
+    row_reduce<OpSum, G>(s, shf, 2 * W, turn);
     r.rs = s[0] > 0.f || s[0] != s[0] ? 1.f / s[0] : 0.f;
     const double lse_z = row_lse(r.m, s[0], a.inv_tau);
     double lse_t = 0.0;
     if (on) lse_t = a.lse ? (double)a.lse[row] : row_lse(mt, s[1], a.inv_tau);
     double tl[2];
     te.terms(a.inv_tau, lse_t, lse_z, lane, tl);
-    row_reduce<OpSum, G>(tl, shd, W, turnd);
+    row_reduce<OpSum, G>(tl, shd, 2 * W, turnd);
     if (lane == 0) a.loss[row] = on ? (float)((double)w * tl[1]) : 0.f;
     if constexpr (GRAD) {
         const float cp = on ? (float)(a.scale * (double)w) : 0.f, cq = on ? (float)(a.scale * (double)w * tl[0]) : 0.f;

@@ -158,15 +158,16 @@ __device__ __forceinline__ void lane_reduce(V (&v)[C]) {
 }
 
 // The same over the G threads of a row (G a power of two; the waves of a row lie side by side in the workgroup).
-// sh: [2][waves of the workgroup][C], used by turns (`turn` alternates between calls), so that one barrier is enough: a
-// wave writes a half again only behind the next call's barrier, when all have read it.  Where a row has several waves
+// sh: two halves of `half` values (at least C for each wave of the workgroup; the same for all calls that share sh, whatever
+// their C), used by turns (`turn` alternates between calls), so that one barrier is enough: a wave writes a half again only
+// behind the next call's barrier, when all have read it.  Where a row has several waves
 // every thread of the workgroup has to come here.
 template <typename Op, int G, int C, typename V>
-__device__ __forceinline__ void row_reduce(V (&v)[C], V* sh, int waves, int& turn) {
+__device__ __forceinline__ void row_reduce(V (&v)[C], V* sh, int half, int& turn) {
     lane_reduce<Op, (G < 64 ? G : 64)>(v);
     if constexpr (G > 64) {
         const int wave = threadIdx.x >> 6;
-        V* mine = sh + (turn ? waves * C : 0);
+        V* mine = sh + (turn ? half : 0);
         turn ^= 1;
         if ((threadIdx.x & 63) == 0)
 #pragma unroll
