@@ -66,18 +66,27 @@ struct Teacher {
         for (int k = lane; k < K; k += G) s += __builtin_amdgcn_exp2f((sp[k] - mt) * c2);
         return s;
     }
-    // sp <- p_k; this thread's part of {P, loss}
-    __device__ __forceinline__ void terms(double inv_tau, double lse_t, double lse_z, int lane, double (&v)[2]) {
-        v[0] = v[1] = 0.0;
+    // p of a teacher's logit: by the caller's normaliser, or by the K entries' own maximum and sum
+    struct Prob { bool given; float lse, mt, rt, c2; double inv_tau; };
+    static __device__ __forceinline__ float prob(const Prob& o, float t) {
+        return o.given ? expf((float)((double)t * o.inv_tau - (double)o.lse)) : __builtin_amdgcn_exp2f((t - o.mt) * o.c2) * o.rt;
+    }
+    // this thread's part of P
+    __device__ __forceinline__ float mass(const Prob& o, int lane) const {
+        float v = 0.f;
+        for (int k = lane; k < K; k += G) v += prob(o, sp[k]);
+        return v;
+    }
+    // this thread's part of the loss; sp <- p_k
+    __device__ __forceinline__ double terms(const Prob& o, double lse_t, double lse_z, int lane) {
+        double v = 0.0;
         for (int k = lane; k < K; k += G) {
-            const double x = (double)sp[k] * inv_tau - lse_t;
-            const float p = expf((float)x);
+            const float t = sp[k], p = prob(o, t);
             sp[k] = p;
-            if (p != 0.f) {   // (a NaN comes through)
-                v[0] += (double)p;
-                v[1] += (double)p * (x - ((double)sz[k] * inv_tau - lse_z));
-            }
+            if (p != 0.f)     // (a NaN comes through)
+                v += (double)p * (((double)t * o.inv_tau - lse_t) - ((double)sz[k] * o.inv_tau - lse_z));
         }
+        return v;
     }
     // the entries' own gradients, over what the row's stores have left there; an index that stands twice is written by
     // the first of its entries, with the sum of all
@@ -107,13 +116,29 @@ __device__ __forceinline__ double row_lse(float m, float s, double inv_tau) {
     return s > 0.f || s != s ? (double)m * inv_tau + log((double)s) : 0.0;
 }
 
+// Behind the dense part of a row: its loss, and the K entries' own gradients.  (The logarithms in float64 and the float64
+// terms stand here, where nothing else of the row is in registers any more: before the stores they cost 30 of them.)
+template <typename T, int G, bool GRAD>
+__device__ __forceinline__ void finish(const Args& a, Teacher<T, G>& te, const typename Teacher<T, G>::Prob& o, const RowStat& r,
+                                       float ss, float st, float w, float cq, float cp, int64_t row, int lane, bool live,
+                                       bool on, double* shd, int& turn) {
+    const double lse_z = row_lse(r.m, ss, a.inv_tau), lse_t = o.given ? (double)o.lse : row_lse(o.mt, st, a.inv_tau);
+    double v[1] = {te.terms(o, lse_t, lse_z, lane)};
+    row_reduce<OpSum, G>(v, shd, (G < 256 ? 256 : G) / 64, turn);
+    if (live && lane == 0) a.loss[row] = on ? (float)((double)w * v[0]) : 0.f;
+    if constexpr (GRAD) {
+        __syncthreads();        // the row's dense part stands in memory, its p in LDS
+        if (on) te.write((T*)a.grad + row * a.ldg, o.c2, r, cq, cp, lane);
+    }
+}
+
 // One row for every G threads, the row in their registers: NV whole pieces each, and of the last V % kN values one.
 template <typename T, int G, int NV, bool GRAD>
-__global__ __launch_bounds__(G < 256 ? 256 : G) void row_kernel(Args a) {
+__global__ __launch_bounds__(G < 256 ? 256 : G, NV <= 8 ? 8 : 4) void row_kernel(Args a) {
     constexpr int B = G < 256 ? 256 : G, W = B / 64, N = Piece<T>::kN;
     extern __shared__ char lds[];
     __shared__ float shf[2 * W * 2];
-    __shared__ double shd[2 * W * 2];
+    __shared__ double shd[2 * W];
     int turn = 0, turnd = 0;
     const int lane = threadIdx.x % G, slot = __builtin_amdgcn_readfirstlane(threadIdx.x / G);
     const int V = (int)a.V, whole = V / N * N, tail = V - whole;
@@ -155,15 +180,16 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void row_kernel(Args a) {
         for (int j = 0; j < N; ++j) s[0] += __builtin_amdgcn_exp2f((raw[v].f(j) - r.m) * c2);
     row_reduce<OpSum, G>(s, shf, 2 * W, turn);
     r.rs = s[0] > 0.f || s[0] != s[0] ? 1.f / s[0] : 0.f;
-    const double lse_z = row_lse(r.m, s[0], a.inv_tau);
-    double lse_t = 0.0;
-    if (on) lse_t = a.lse ? (double)a.lse[row] : row_lse(mt, s[1], a.inv_tau);
-    double tl[2];
-    te.terms(a.inv_tau, lse_t, lse_z, lane, tl);
-    row_reduce<OpSum, G>(tl, shd, 2 * W, turnd);
-    if (live && lane == 0) a.loss[row] = on ? (float)((double)w * tl[1]) : 0.f;
+    typename Teacher<T, G>::Prob o{a.lse != nullptr, on && a.lse ? a.lse[row] : 0.f, mt, s[1] > 0.f || s[1] != s[1] ? 1.f / s[1] : 0.f,
+                                   c2, a.inv_tau};
+    float cp = 0.f, cq = 0.f;
     if constexpr (GRAD) {
-        const float cp = on ? (float)(a.scale * (double)w) : 0.f, cq = on ? (float)(a.scale * (double)w * tl[0]) : 0.f;
+        float mass[1] = {te.mass(o, lane)};
+        row_reduce<OpSum, G>(mass, shf, 2 * W, turn);
+        if (on) {
+            cp = (float)(a.scale * (double)w);
+            cq = (float)(a.scale * (double)w * (double)mass[0]);
+        }
         T* g = (T*)a.grad + (live ? row : 0) * a.ldg;
         const float f = cq * r.rs;
         forget(raw);
@@ -180,12 +206,12 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void row_kernel(Args a) {
                     __builtin_memcpy(&x, &p, 16);
                     *reinterpret_cast<Raw16*>(g + at) = x;
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
             if (lane < tail) g[whole + lane] = from_float<T>(f * __builtin_amdgcn_exp2f((zt - r.m) * c2));
         }
-        __syncthreads();
-        if (on) te.write(g, c2, r, cq, cp, lane);
     }
+    finish<T, G, GRAD>(a, te, o, r, s[0], s[1], w, cq, cp, row, lane, live, on, shd, turnd);
 }
 
 // A row that does not fit: 1024 threads read it twice.
@@ -194,7 +220,7 @@ __global__ __launch_bounds__(1024) void wide_kernel(Args a) {
     constexpr int G = 1024, W = G / 64, N = Piece<T>::kN, U = 4;
     extern __shared__ char lds[];
     __shared__ float shf[2 * W * 2];
-    __shared__ double shd[2 * W * 2];
+    __shared__ double shd[2 * W];
     int turn = 0, turnd = 0;
     const int lane = threadIdx.x;
     const int64_t row = blockIdx.x;
@@ -229,15 +255,16 @@ __global__ __launch_bounds__(1024) void wide_kernel(Args a) {
     float s[2] = {part * __builtin_amdgcn_exp2f((own - r.m) * c2), a.lse ? 0.f : te.sum(mt, c2, lane)};
     row_reduce<OpSum, G>(s, shf, 2 * W, turn);
     r.rs = s[0] > 0.f || s[0] != s[0] ? 1.f / s[0] : 0.f;
-    const double lse_z = row_lse(r.m, s[0], a.inv_tau);
-    double lse_t = 0.0;
-    if (on) lse_t = a.lse ? (double)a.lse[row] : row_lse(mt, s[1], a.inv_tau);
-    double tl[2];
-    te.terms(a.inv_tau, lse_t, lse_z, lane, tl);
-    row_reduce<OpSum, G>(tl, shd, 2 * W, turnd);
-    if (lane == 0) a.loss[row] = on ? (float)((double)w * tl[1]) : 0.f;
+    typename Teacher<T, G>::Prob o{a.lse != nullptr, on && a.lse ? a.lse[row] : 0.f, mt, s[1] > 0.f || s[1] != s[1] ? 1.f / s[1] : 0.f,
+                                   c2, a.inv_tau};
+    float cp = 0.f, cq = 0.f;
     if constexpr (GRAD) {
-        const float cp = on ? (float)(a.scale * (double)w) : 0.f, cq = on ? (float)(a.scale * (double)w * tl[0]) : 0.f;
+        float mass[1] = {te.mass(o, lane)};
+        row_reduce<OpSum, G>(mass, shf, 2 * W, turn);
+        if (on) {
+            cp = (float)(a.scale * (double)w);
+            cq = (float)(a.scale * (double)w * (double)mass[0]);
+        }
         T* g = (T*)a.grad + row * a.ldg;
         const float f = cq * r.rs;
         for (int64_t at = (int64_t)lane * N; at < a.V; at += (int64_t)U * G * N) {
@@ -252,9 +279,8 @@ __global__ __launch_bounds__(1024) void wide_kernel(Args a) {
                 store_piece(g, at + (int64_t)u * G * N, a.V, pack<T>(o));
             }
         }
-        __syncthreads();
-        if (on) te.write(g, c2, r, cq, cp, lane);
     }
+    finish<T, G, GRAD>(a, te, o, r, s[0], s[1], w, cq, cp, row, lane, true, on, shd, turnd);
 }
 
 template <typename T, int G, int NV, bool GRAD>
