@@ -6,10 +6,11 @@
 //   loss = w sum_k p_k (x_k - (z_{i_k} / tau - lse_z))
 //   grad_j = (scale w / tau) (P q_j - sum_{k: i_k = j} p_k),   q = softmax(z / tau),  P = sum_k p_k
 //
-// Bound: HBM, the logits read once and the gradient written once.  A row therefore stays in the registers of the threads
-// that read it (up to 16 pieces of 16 bytes for each of 1024 threads: 131072 bf16 or 65536 float32 values); only a wider
-// row is read twice.  Sums and statistics are float32, the K terms of the loss float64 (they cancel where student and
-// teacher agree); each gradient value is rounded once.
+// Bound: HBM, the logits read once and the gradient written once (4096 x 32000 bf16: 133 us for 524 MB, 3960 GB/s, where a
+// large copy reaches 4750; the loss alone 63 us, 4200 GB/s).  A row therefore stays packed in the registers of the threads
+// that read it, up to 8 pieces of 16 bytes for each of 1024 threads (65536 values of 16 bits; twice that for the gradient of
+// float32 rows); a wider row is read twice.  Sums and statistics are float32, the K terms of the loss float64 (they cancel
+// where student and teacher agree); each gradient value is rounded once.
 #include "seq_dev.h"
 #include "../../include/samx.h"
 
@@ -302,7 +303,11 @@ int launch(const Args& a, hipStream_t st) {
     if (n <= 2048) return launch_row<T, 256, 8, GRAD>(a, st);
     if (n <= 4096) return launch_row<T, 512, 8, GRAD>(a, st);
     if (n <= 8192) return launch_row<T, 1024, 8, GRAD>(a, st);
-    if (n <= 16384) return launch_row<T, 1024, 16, GRAD>(a, st);
+    // Behind that 16 pieces a thread leave one row a unit, and nothing runs while it is reduced: two workgroups that read
+    // their rows twice (the second time out of a cache) are as good or better, but for float32 gradients.  4096 x 128000
+    // bf16: loss 286 -> 226 us, gradient 550 -> 519; 4096 x 64000 float32: loss 233 -> 183, gradient 453 against 485.
+    if constexpr (GRAD && sizeof(T) == 4)
+        if (n <= 16384) return launch_row<T, 1024, 16, GRAD>(a, st);
     wide_kernel<T, GRAD><<<(unsigned)a.N, 1024, row_lds(a.K), st>>>(a);
     SAMX_LAUNCH_CHECK();
     return SAMX_OK;
