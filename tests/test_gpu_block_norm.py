@@ -58,6 +58,7 @@ def _tol_forward(c, res, kind, eps, dtype):
 
 SHAPES = [(1, 1), (3, 2), (1, 7), (5, 64), (33, 65), (9, 100), (70, 128), (7, 513), (1025, 96), (4, 1000), (2, 2048),
           (600, 4096), (3, 4100), (2, 8192)]
+LONG = [(300, 8195), (3, 16384)]      # rows of 16 bits of which a thread holds two pieces
 
 
 @pytest.mark.parametrize('gate', ['none', 'channel', 'full'])
@@ -65,7 +66,7 @@ SHAPES = [(1, 1), (3, 2), (1, 7), (5, 64), (33, 65), (9, 100), (70, 128), (7, 51
 @pytest.mark.parametrize('dtype', [F32, BF16, F16])
 def test_forward(dtype, kind, gate):
     from sam_tf_amd import ops
-    for N, D in SHAPES:
+    for N, D in SHAPES + (LONG if dtype != F32 else []):
         eps = 1e-6
         c = _case(N, D, dtype, kind, gate, seed=N + D)
         k = _gpu(c)
@@ -83,7 +84,7 @@ def test_forward(dtype, kind, gate):
 @pytest.mark.parametrize('dtype', [F32, BF16, F16])
 def test_gradient(dtype, kind, gate):
     from sam_tf_amd import ops
-    for N, D in [s for s in SHAPES if s[1] > 1]:
+    for N, D in [s for s in SHAPES if s[1] > 1] + (LONG if dtype != F32 else []):
         eps, res = 1e-6, 0.75
         c = _case(N, D, dtype, kind, gate, seed=N + 7 * D)
         k, d = _gpu(c), _d(c)

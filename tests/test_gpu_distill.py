@@ -68,7 +68,7 @@ def test_sizes(V, K, dtype):
         _check(_case(N, V, K, dtype, seed=V + N, pad=pad, lse=lse, tau=tau), tau, scale, dtype, 'N %d' % N)
 
 
-@pytest.mark.parametrize('V,dtype', [(32769, BF16), (65537, F32), (131073, BF16), (131073, F16)])
+@pytest.mark.parametrize('V,dtype', [(32769, BF16), (65537, F32), (131073, BF16), (131073, F16), (65543, BF16), (65544, BF16), (131073, F32)])
 def test_wide_rows(V, dtype):
     _check(_case(3, V, 70, dtype, seed=1, lse=True), 1.0, 1.0, dtype)
 
