@@ -648,7 +648,7 @@ int samx_step_apply(const samx_learner* L, int64_t B, int mode, float grad_scale
  * N is LayerNorm (with its bias; helpers/network_util.py:43-56 has it behind a layer) or, without one, the RMS norm.
  * x, y, h, u: dense [N, D] of the element type; weights and biases float32 [D]; g by gate_kind: none, float32 [D]
  * (SAMX_GATE_CHANNEL) or the element type [N, D] (SAMX_GATE_FULL).  D at most 16384 (float32: 8192).  Statistics are float32,
- * of h before it is rounded.  h may be x's own buffer or y's, u the other one. */
+ * of h before it is rounded.  h may be x's own buffer or y's, u the other one; otherwise outputs do not overlap inputs. */
 #define SAMX_NORM_RMS 0
 #define SAMX_NORM_LAYER 1
 #define SAMX_GATE_NONE 0
@@ -673,9 +673,9 @@ int samx_block_norm_grad(const void* y, const void* h, const void* dh, const voi
  * strides (in elements: batch, row, head) as given; decay float32 [H], the logarithm of the factor (<= 0, -inf: no memory);
  * state float32 [B, H, D, DV] dense, state_in NULL: zero.  lengths int32 [B] (NULL: T): rows of each sequence that are there
  * (taken into [0, T]); rows behind them are not read, their outputs are zeros, the state behind a sequence is that of its
- * last row.  out, dq, dk, dv are dense.  Scores and the state are float32; products of 16-bit types take the scores and, for
- * out, the state in their own type (of float16, both have to be within its range).  A row's inputs have to be finite for the
- * outputs of the 63 rows before it to be. */
+ * last row.  out, dq, dk, dv are dense; no output overlaps an input.  Scores and the state are float32; products of 16-bit
+ * types take the scores and, for out, the state in their own type (of float16, both have to be within its range).  An infinity
+ * or a NaN of a row reaches what the recurrence takes it to and nothing else; behind it an infinity may have become a NaN. */
 typedef struct samx_linattn_shape {
     int32_t dtype, H, HK, D, DV, pad;
     int64_t B, T;

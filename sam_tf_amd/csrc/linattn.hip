@@ -130,6 +130,15 @@ struct Rows {
         p = (const SAMX_GLOBAL char*)m.p + (int64_t)sizeof(T) * (q.b * m.sb + (int64_t)(q.h / m.grp) * m.sh + (rev ? (q.L - 1) * m.st : 0));
         step = (int64_t)sizeof(T) * (rev ? -m.st : m.st);
     }
+    __device__ __forceinline__ float value(int64_t pos, int i) const {
+        T v;
+        if constexpr (sizeof(T) == 4) v = *(const SAMX_GLOBAL float*)(p + pos * step + i * 4);
+        else {
+            const uint16_t u = *(const SAMX_GLOBAL uint16_t*)(p + pos * step + i * 2);
+            __builtin_memcpy(&v, &u, 2);
+        }
+        return to_float(v);
+    }
     // elements [at, at + kN) of position base + pos.  What lies behind the chunk's n positions or behind the row's end is
     // not what comes here: the caller does not use it.
     __device__ __forceinline__ Piece<T> piece(int64_t base, int pos, int at, int n) const {
@@ -214,11 +223,13 @@ template <typename T, int DP>
 struct LdsKv {
     static constexpr int kRow = DP + Piece<T>::kN;
     T b[kChunk][kRow], c[kChunk][kRow];                  // the chunk's rows
-    float lam[2 * kChunk + 4];                           // l^(n - kChunk), 0 below kChunk
+    float lam[2 * kChunk + 1];                           // l^(n - kChunk), 0 below kChunk
+    uint32_t odd, pad[2];                                // 1 + the last chunk whose c has an infinity or a NaN
 };
 template <typename T, int DP>
 struct Lds : LdsKv<T, DP> {
     static constexpr int kTok = kChunk + Piece<T>::kN;
+    static_assert(sizeof(LdsKv<T, DP>) % 16 == 0, "pieces are read whole");
     T p[4][16][kTok];                                    // each wave's 16 rows of scores
     T x[DP][LdsKv<T, DP>::kRow];                         // X, a row for each column
 };
@@ -241,6 +252,14 @@ __device__ __forceinline__ void in_groups(Read read, Use use) {
     }
 }
 
+// a bit of a dword's element(s) whose exponent is all ones, gathered by "or"
+template <typename T>
+__device__ __forceinline__ uint32_t odd_bits(uint32_t w) {
+    constexpr uint32_t e = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, f16>::value ? 0x7c007c00u : 0x7f807f80u;
+    constexpr uint32_t one = sizeof(T) == 4 ? 0x00800000u : std::is_same<T, f16>::value ? 0x04000400u : 0x00800080u;
+    return ((w & e) + one) & (sizeof(T) == 4 ? 0x80000000u : 0x80008000u);
+}
+
 // A chunk's rows of b and c on their way to LDS
 template <typename T, int DP>
 struct Staged {
@@ -256,17 +275,19 @@ struct Staged {
     }
     // zeros behind the rows' ends and behind the n positions
     template <typename L>
-    __device__ __forceinline__ void store(L& l, int db, int dc, int n) const {
+    __device__ __forceinline__ uint32_t store(L& l, int db, int dc, int n) const {
         const int t = threadIdx.x / kAcross, d = threadIdx.x % kAcross * kN;
+        uint32_t odd = 0;                 // whether c has something that is not finite
 #pragma unroll
         for (int u = 0; u < kPer; ++u) {
             const uint32_t kb = d < db && t + u * kDown < n ? ~0u : 0u, kc = d < dc && t + u * kDown < n ? ~0u : 0u;
             Piece<T> x, y;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { x.w[j] = b[u].w[j] & kb; y.w[j] = c[u].w[j] & kc; }
+            for (int j = 0; j < 4; ++j) { x.w[j] = b[u].w[j] & kb; y.w[j] = c[u].w[j] & kc; odd |= odd_bits<T>(y.w[j]); }
             lds_put(&l.b[t + u * kDown][d], x);
             lds_put(&l.c[t + u * kDown][d], y);
         }
+        return odd;
     }
 };
 
@@ -526,10 +547,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
     else if (s_in) state_load<DP>(S, s_in, da, dc, r.in_a, r.in_c, r.rev ? 1.f : power(p.g, 1));
     else S.zero();
     if (threadIdx.x <= 2 * kChunk) l.lam[threadIdx.x] = threadIdx.x < kChunk ? 0.f : power(p.g, threadIdx.x - kChunk);
+    if (threadIdx.x == 0) l.odd = 0u;
+    __syncthreads();
     for (int64_t base = at; base < to; base += kChunk) {
         const int n = (int)(to - base < kChunk ? to - base : kChunk);
         const bool more = base + kChunk < to;
-        st.store(l, da, dc, n);
+        const uint32_t chunk = (uint32_t)((base - at) / kChunk) + 1u;
+        if (st.store(l, da, dc, n)) l.odd = chunk;
 #pragma unroll
         for (int j = 0; j < State<DP>::kJ; ++j)          // X's copy for the products with a
 #pragma unroll
@@ -611,6 +635,28 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
             } else {
 #pragma unroll
                 for (int j = 0; j < kTiles; ++j) put4(std::false_type(), tok, j * 16 + q * 4, o[j]);
+            }
+        }
+        if (__builtin_amdgcn_readfirstlane(l.odd) == chunk && row < n) {
+            // Zeros behind a row's own position times an infinity or a NaN there were NaN in what has just been written: once
+            // more, one product after the other, up to the row.  (Kept out of the way of the products above: as their other
+            // branch it cost them their reads ahead, 146 -> 183 us for the gradient of 4 x 2048 rows.)
+            const int64_t tok = r.rev ? p.L - 1 - (base + row) : base + row;
+            for (int d = q * 4; d < dc; d += 16) {
+                f32x4 v = {0.f, 0.f, 0.f, 0.f};
+                for (int i = 0; i < da; ++i) {
+                    const float x = a.value(base + row, i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] += x * to_float(l.x[d + e][i]);
+                }
+                v *= decayed;
+                for (int t = 0; t <= row; ++t) {
+                    const float x = to_float(l.p[w][r16][t]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] += x * to_float(l.c[t][d + e]);
+                }
+                if (wide) put4(std::true_type(), tok, d, v);
+                else put4(std::false_type(), tok, d, v);
             }
         }
         if (more || (last && s_out)) {

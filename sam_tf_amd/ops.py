@@ -964,6 +964,25 @@ def _apart(named):
             raise ValueError('%s and %s overlap' % (a, c))
 
 
+def _extent(t):
+    """The bytes from a tensor's first element to its last (strides are never negative)."""
+    n = 1 + sum((s - 1) * d for s, d in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (n * t.element_size() if t.numel() else 0)
+
+
+def _clear(out, name, same, others):
+    """An output that is given does not overlap an input, or is the whole of one of those that it may replace (`same`)."""
+    if out is None:
+        return
+    b, e = _extent(out)
+    for n, t in others:
+        if t is None:
+            continue
+        c, d = _extent(t)
+        if b < d and c < e and not (n in same and b == c and e == d and out.dtype == t.dtype):
+            raise ValueError('%s overlaps %s' % (name, n))
+
+
 def _norm_args(y, gate, post_w, post_b, pre_w, pre_b, kind):
     code, dev = _seq_dtype(y, 'y')
     if y.dim() != 2:
@@ -995,6 +1014,9 @@ def block_norm(x, y, post_w, pre_w, post_b=None, pre_b=None, gate=None, res_scal
     px = _on(x, dev, y.dtype, y.shape, 'x')
     if h is not None or u is not None:
         _apart((('h', h), ('u', u)))
+        for n, t in (('h', h), ('u', u)):
+            _clear(t, n, ('x', 'y'), (('x', x), ('y', y), ('gate', gate), ('post_w', post_w), ('pre_w', pre_w),
+                                      ('post_b', post_b), ('pre_b', pre_b)))
     h = torch.empty_like(y) if h is None else h
     u = torch.empty_like(y) if u is None else u
     check(_L().samx_block_norm(px, py, code, N, D, w[0], b[0], gate_kind, g, w[1], b[1], res_scale, _NORM[kind], eps,
@@ -1071,6 +1093,8 @@ def linattn(q, k, v, decay, scale=1.0, state=None, lengths=None, out=None, state
     ps, pl = _opt_on(state, dev, F32, shape, 'state'), _opt_on(lengths, dev, I32, (s.B,), 'lengths')
     if out is not None or state_out is not None:
         _apart((('out', out), ('state_out', state_out), ('state', state)))
+        for n, t in (('out', out), ('state_out', state_out)):
+            _clear(t, n, (), (('q', q), ('k', k), ('v', v), ('decay', decay), ('lengths', lengths)))
     out = torch.empty(lead + (s.H, s.DV), dtype=q.dtype, device=dev) if out is None else out
     state_out = torch.empty(shape, dtype=F32, device=dev) if state_out is None else state_out
     L = _L()
@@ -1107,6 +1131,7 @@ def linattn_step(q, k, v, decay, state, scale=1.0, out=None):
         po = out.data_ptr()
     else:
         _apart((('out', out), ('state', state)))
+        _clear(out, 'out', (), (('q', q), ('k', k), ('v', v), ('decay', decay)))
         po = _on(out, dev, q.dtype, shape, 'out')
     check(_L().samx_linattn_step(C.byref(s), pq, pk, pv, pd, scale, _on(state, dev, F32, lead + (s.H, s.D, s.DV), 'state'),
                                  po, _raw_stream(dev.index)))

@@ -301,6 +301,71 @@ def test_captured_and_replayed():
         assert all(torch.equal(a, b) for a, b in zip(out, want)) and torch.equal(s, acting)
 
 
+@pytest.mark.parametrize('what', ['q', 'k', 'v', 'dout'])
+@pytest.mark.parametrize('bad', [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize('dtype,D,DV', [(F32, 24, 40), (BF16, 40, 24), (F16, 64, 64), (BF16, 128, 128), (F32, 100, 128)])
+def test_what_is_not_finite_stays_with_its_rows(dtype, D, DV, bad, what):
+    """Row 75 of sequence 1, key head 0 or query head 1: rows and heads that do not meet it are as they were: bit for bit
+    outside of its chunk, in it the same products in another order (each order within _errors of the sum of magnitudes,
+    rounded once each)."""
+    from sam_tf_amd import ops
+    B, T, H, HK, at = 2, 150, 4, 2, 75
+    c0 = _case(B, T, H, HK, D, DV, dtype, seed=5)
+    a = _abs(_d(c0))
+    most = (R.linattn(a['q'], a['k'], a['v'], a['decay'], 0.5, a['state'], None)[0],) + R.linattn_grad(
+        a['q'], a['k'], a['v'], a['decay'], a['dout'], 0.5, a['state'], a['dstate'], None)[:3]
+    e, h = _errors(dtype, T, D, DV)[0], 1.01 * half_step(dtype)
+    c = _gpu(c0)
+    run = lambda: (ops.linattn(c['q'], c['k'], c['v'], c['decay'], 0.5, c['state']) +
+                   ops.linattn_grad(c['q'], c['k'], c['v'], c['decay'], c['dout'], 0.5, c['state'], c['dstate']))
+    want = run()
+    head = 1 if what in ('q', 'dout') else 0
+    c[what][1, at, head, 3] = bad
+    got = run()
+    heads = [1] if what in ('q', 'dout') else [0, 1]               # query heads that meet it
+    behind, upto, only, none = slice(at, None), slice(None, at + 1), slice(at, at + 1), slice(0, 0)
+    # rows of (out, dq, dk, dv) that may change, and whether the state behind and the gradient of the one before may
+    rows, ends = {'q': ((only, none, upto, upto), (False, True)), 'dout': ((none, only, upto, upto), (False, True)),
+                  'k': ((behind, behind, none, only), (True, False)), 'v': ((behind, behind, only, none), (True, False))}[what]
+    for x, w, r, m, name in zip((got[0], got[2], got[3], got[4]), (want[0], want[2], want[3], want[4]), rows, most, ('out', 'dq', 'dk', 'dv')):
+        touched = torch.zeros(x.shape[:3], dtype=torch.bool, device='cuda')
+        for h in heads if name in ('out', 'dq') else sorted({h * HK // H for h in heads}):
+            touched[1, r, h] = True
+        same = ~touched.cpu()
+        within(x.cpu()[same], w.cpu()[same], (2 * e * m + 2 * h * w.cpu().double().abs() + 2 * smallest(dtype))[same], name)
+        assert torch.equal(x[0], w[0]), name
+        far = slice(0, 64) if name in ('out', 'dq') else slice(T - 64, T)       # chunks are counted from either end
+        if not bool(touched[1, far].any()):
+            assert torch.equal(x[1, far], w[1, far]), name
+        if bool(touched.any()):
+            assert not bool(torch.isfinite(x[touched]).all(-1).any()), name
+    for x, w, may in ((got[1], want[1], ends[0]), (got[5], want[5], ends[1])):
+        touched = torch.zeros(x.shape[:2], dtype=torch.bool, device='cuda')
+        touched[1, heads] = may
+        assert torch.equal(x[~touched], w[~touched])
+        if may:
+            assert not bool(torch.isfinite(x[touched].flatten(1)).all(-1).any())
+
+
+def test_outputs_apart_from_inputs():
+    from sam_tf_amd import ops
+    g = _gpu(_case(2, 8, 4, 4, 16, 16, F32))
+    with pytest.raises(ValueError):
+        ops.linattn(g['q'], g['k'], g['v'], g['decay'], out=g['q'])
+    with pytest.raises(ValueError):
+        ops.linattn_step(g['q'][:, 0], g['k'][:, 0], g['v'][:, 0], g['decay'], g['state'], out=g['v'].view(-1)[:2 * 4 * 16].view(2, 4, 16))
+    from tests.test_gpu_block_norm import _case as norms, _gpu as to
+    c = to(norms(9, 64, F32, 'rms', 'full'))
+    room = torch.empty(10, 64, device='cuda')
+    room[:9] = c['x']
+    with pytest.raises(ValueError):
+        ops.block_norm(room[:9], c['y'], c['post_w'], c['pre_w'], gate=c['gate'], kind='rms', h=room[1:])
+    with pytest.raises(ValueError):
+        ops.block_norm(c['x'], c['y'], c['post_w'], c['pre_w'], gate=c['gate'], kind='rms', u=c['gate'])
+    h, u = ops.block_norm(c['x'], c['y'], c['post_w'], c['pre_w'], gate=c['gate'], kind='rms', h=c['y'], u=c['x'])
+    assert h is c['y'] and u is c['x']
+
+
 def test_refusals():
     from sam_tf_amd import ops
     from sam_tf_amd._lib import SamxError
