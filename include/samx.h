@@ -14,7 +14,7 @@
  *  - Matrices are row-major float32.  Flat parameter / gradient vectors use the reference's variable
  *    creation order (networks.py:50-70,359-404 ; tf_util.py:137-151):
  *       W1[in,h1] b1[h1] (beta1[h1] gamma1[h1]) W2[h1,h2] b2[h2] (beta2 gamma2) W3[h2,out] b3[out]
- *  - Calls that need scratch take `ws`/`ws_bytes`; ask samx_*_ws_bytes() for the size.  The library
+ *  - Calls that need scratch take `ws`/`ws_bytes` (16-byte aligned); ask samx_*_ws_bytes() for the size.  The library
  *    itself allocates nothing on these paths.
  */
 #ifndef SAMX_H

@@ -68,7 +68,13 @@ int host_pow_stage(const void* owner, int64_t n, hipStream_t st, PowStage* s) {
     if (cap) {
         if (!held) held = new (std::nothrow) std::map<std::pair<int, const void*>, Held>();
         if (!held) return fail(SAMX_ERR_WORKSPACE, "host pow: out of host memory");
-        Held& h = (*held)[std::make_pair(dev, owner)];
+        Held* at = nullptr;
+        try {
+            at = &(*held)[std::make_pair(dev, owner)];
+        } catch (const std::bad_alloc&) {
+            return fail(SAMX_ERR_WORKSPACE, "host pow: out of host memory");
+        }
+        Held& h = *at;
         if (h.cap < n) {
             if (chunk_left < n)
                 return fail(SAMX_ERR_WORKSPACE, "host pow: no pinned memory left for a captured call of %lld values: make "

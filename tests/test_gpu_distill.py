@@ -174,6 +174,19 @@ def test_captured_and_replayed():
         assert torch.equal(loss, a) and torch.equal(grad, b)
 
 
+def test_rows_far_apart():
+    """Rows 2^32 bytes from each other: offsets of 64 bits, and the same numbers."""
+    from sam_tf_amd import ops
+    c = _case(3, 100, 5, F32, seed=3)
+    z, idx, t = c['z'].contiguous().cuda(), c['idx'].cuda(), c['t'].cuda()
+    want = ops.distill_grad(z, idx, t)
+    room = torch.empty(2 * 2 ** 30 + 100, device='cuda')
+    far = room.as_strided((3, 100), (2 ** 30, 1))
+    far.copy_(z)
+    loss, grad = ops.distill_grad(far, idx, t, grad=far)
+    assert grad is far and torch.equal(loss, want[0]) and torch.equal(far, want[1])
+
+
 def test_refusals():
     from sam_tf_amd import ops
     from sam_tf_amd._lib import SamxError

@@ -347,6 +347,26 @@ def test_what_is_not_finite_stays_with_its_rows(dtype, D, DV, bad, what):
             assert not bool(torch.isfinite(x[touched].flatten(1)).all(-1).any())
 
 
+def test_rows_far_apart():
+    """Rows 2^31 bytes from each other: offsets of 64 bits, and the same numbers."""
+    from sam_tf_amd import ops
+    B, T, H, D, DV = 1, 3, 2, 16, 24
+    c = _gpu(_case(B, T, H, H, D, DV, BF16))
+    want = ops.linattn(c['q'], c['k'], c['v'], c['decay'], 0.5, c['state'])
+    gwant = ops.linattn_grad(c['q'], c['k'], c['v'], c['decay'], c['dout'], 0.5, c['state'], c['dstate'])
+    step = 2 ** 30
+    room = torch.empty((T - 1) * step + 1024, dtype=BF16, device='cuda')
+    far, at = {}, 0
+    for n in ('q', 'k', 'v', 'dout'):
+        d = c[n].shape[-1]
+        far[n] = room.as_strided((B, T, H, d), (T * step, step, d, 1), at)
+        far[n].copy_(c[n])
+        at += H * d
+    got = ops.linattn(far['q'], far['k'], far['v'], c['decay'], 0.5, c['state'])
+    ggot = ops.linattn_grad(far['q'], far['k'], far['v'], c['decay'], far['dout'], 0.5, c['state'], c['dstate'])
+    assert all(torch.equal(a, b) for a, b in zip(want + gwant, got + ggot))
+
+
 def test_outputs_apart_from_inputs():
     from sam_tf_amd import ops
     g = _gpu(_case(2, 8, 4, 4, 16, 16, F32))

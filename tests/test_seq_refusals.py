@@ -58,6 +58,9 @@ def test_linattn_pointers_scale_and_workspace():
     # shared heads need room for each head's part of the gradient
     _refused(L.samx_linattn_grad(C.byref(s), P, P, P, P, P, 1.0, None, None, None, P, P, P, P, P, 100, None), WORKSPACE)
     _refused(L.samx_linattn_grad(C.byref(s), P, P, P, P, P, 1.0, None, None, None, P, P, P, P, None, 1 << 40, None), WORKSPACE)
+    odd = C.c_void_p(0x1008)
+    _refused(L.samx_linattn_grad(C.byref(s), P, P, P, P, P, 1.0, None, None, None, P, P, P, P, odd, 1 << 40, None), text='aligned')
+    _refused(L.samx_linattn(C.byref(_shape(T=5000)), P, P, P, P, 1.0, None, None, P, P, odd, 1 << 40, None), text='aligned')
     long = _shape(T=5000)
     assert L.samx_linattn_ws_bytes(C.byref(long)) > 4096
     _refused(L.samx_linattn(C.byref(long), P, P, P, P, 1.0, None, None, P, P, P, 16, None), WORKSPACE)
@@ -93,6 +96,7 @@ def test_block_norm():
     _refused(g(gk=1, gate=P), text='gate')
     _refused(g(kind=1, post_b=P, dpost_b=P), text='LayerNorm')
     _refused(g(ws=None))
+    _refused(g(ws=C.c_void_p(0x1008)), text='aligned')
     _refused(g(n=64), WORKSPACE)
     assert L.samx_block_norm_grad_ws_bytes(1, 8, 0) == 0 and L.samx_block_norm_grad_ws_bytes(5, 8, 64) == 0
 
