@@ -24,9 +24,9 @@
 // a known state at each segment's start.
 //
 // Measured, 16 heads of 128, bf16.  32 x 1024 rows (two workgroups for each compute unit, no segments): 155 us, 3900 GB/s of
-// 4750 that a large copy reaches.  2 x 4096 rows: 86 us in 8 segments (kv 23, join 9, mix 47), the keys and values read
-// twice.  Gradient of 4 x 2048 ragged rows: 150 us, 192 workgroups with one chunk after the other, 4.6 us each; of those
-// the state's update costs 1.2, the stores 0.7 and waiting for loads 0.6.  float32: its matrix instructions have a
+// 4750 that a large copy reaches.  2 x 4096 rows: 81 us in 8 segments (kv 23, join 9, mix 45), the keys and values read
+// twice.  Gradient of 4 x 2048 ragged rows: 111 us, two workgroups for each head's columns (of one for all of them a chunk
+// took 4.6 us: the state's update 1.2, the stores 0.7, waiting for loads 0.6, the other products' chain the rest).  float32: its matrix instructions have a
 // sixteenth of the rate, and its tiles leave LDS for one workgroup a unit (2 x 4096 rows 205 us).
 #include "seq_dev.h"
 #include "../../include/samx.h"
@@ -80,6 +80,7 @@ struct Role {
 struct Args {
     Role r[3];
     int roles, H, B;
+    int parts;                                 // workgroups that share the columns of c (and of the state)
     int64_t T, seg_len;
     int nseg;
     int64_t seg_size;                          // floats of a segment's state
@@ -90,13 +91,14 @@ struct Args {
 __device__ __forceinline__ float power(float g, int64_t n) { return n == 0 ? 1.f : expf(g * (float)n); }
 
 // where a workgroup works
-struct Place { int role, b, h, seg; int64_t L; float g; };
+struct Place { int role, part, b, h, seg; int64_t L; float g; };
 
 // 8 workgroups that follow each other run on 8 dies: the roles of one (batch, head, segment) go to the same one
 __device__ __forceinline__ bool place_of(const Args& a, int nseg, Place& p) {
     const int64_t units = (int64_t)a.B * a.H * nseg, id = blockIdx.x;
-    const int64_t x = id & 7, k = id >> 3, unit = k / a.roles * 8 + x;
+    const int64_t x = id & 7, k = id >> 3, unit = k / (a.roles * a.parts) * 8 + x;
     p.role = (int)(k % a.roles);
+    p.part = (int)(k / a.roles % a.parts);
     if (unit >= units) return false;
     p.seg = (int)(unit % nseg);
     const int64_t bh = unit / nseg;
@@ -112,7 +114,7 @@ __device__ __forceinline__ bool place_of(const Args& a, int nseg, Place& p) {
 }
 inline unsigned grid_of(const Args& a, int nseg) {
     const int64_t units = (int64_t)a.B * a.H * nseg;
-    return (unsigned)((units + 7) / 8 * 8 * a.roles);
+    return (unsigned)((units + 7) / 8 * 8 * a.roles * a.parts);
 }
 
 #define SAMX_GLOBAL __attribute__((address_space(1)))
@@ -132,8 +134,9 @@ struct Rows {
     const SAMX_GLOBAL char* p;             // position 0
     int64_t step;                          // bytes from one position to the next
     int dim;
-    __device__ Rows(Mat m, Place q, int rev) : dim(m.dim) {
-        p = (const SAMX_GLOBAL char*)m.p + (int64_t)sizeof(T) * (q.b * m.sb + (int64_t)(q.h / m.grp) * m.sh + (rev ? (q.L - 1) * m.st : 0));
+    // from column `from` on
+    __device__ Rows(Mat m, Place q, int rev, int from = 0) : dim(m.dim - from) {
+        p = (const SAMX_GLOBAL char*)m.p + (int64_t)sizeof(T) * (q.b * m.sb + (int64_t)(q.h / m.grp) * m.sh + from + (rev ? (q.L - 1) * m.st : 0));
         step = (int64_t)sizeof(T) * (rev ? -m.st : m.st);
     }
     __device__ __forceinline__ float value(int64_t pos, int i) const {
@@ -225,19 +228,19 @@ __device__ __forceinline__ void wave_sync() {
 }
 
 // LDS rows are 16 bytes longer than their contents: 16 lanes that read 16 rows at one column use all banks
-template <typename T, int DP>
+template <typename T, int DP, int DC>
 struct LdsKv {
-    static constexpr int kRow = DP + Piece<T>::kN;
-    T b[kChunk][kRow], c[kChunk][kRow];                  // the chunk's rows
+    static constexpr int kRow = DP + Piece<T>::kN, kRowC = DC + Piece<T>::kN;
+    T b[kChunk][kRow], c[kChunk][kRowC];                 // the chunk's rows
     float lam[2 * kChunk + 1];                           // l^(n - kChunk), 0 below kChunk
     uint32_t odd, pad[2];                                // 1 + the last chunk whose c has an infinity or a NaN
 };
-template <typename T, int DP>
-struct Lds : LdsKv<T, DP> {
+template <typename T, int DP, int DC>
+struct Lds : LdsKv<T, DP, DC> {
     static constexpr int kTok = kChunk + Piece<T>::kN;
-    static_assert(sizeof(LdsKv<T, DP>) % 16 == 0, "pieces are read whole");
+    static_assert(sizeof(LdsKv<T, DP, DC>) % 16 == 0, "pieces are read whole");
     T p[4][16][kTok];                                    // each wave's 16 rows of scores
-    T x[DP][LdsKv<T, DP>::kRow];                         // X, a row for each column
+    T x[DC][LdsKv<T, DP, DC>::kRow];                     // X, a row for each column
 };
 
 // N groups of products, group g's operands read (into buf[g % (AHEAD + 1)]) AHEAD groups before they are used; nothing is
@@ -267,31 +270,38 @@ __device__ __forceinline__ uint32_t odd_bits(uint32_t w) {
 }
 
 // A chunk's rows of b and c on their way to LDS
-template <typename T, int DP>
+template <typename T, int DP, int DC>
 struct Staged {
-    static constexpr int kN = Piece<T>::kN, kAcross = DP / kN, kDown = kThreads / kAcross, kPer = kChunk / kDown;
-    Piece<T> b[kPer], c[kPer];
+    static constexpr int kN = Piece<T>::kN;
+    static constexpr int kAcross = DP / kN, kDown = kThreads / kAcross, kPer = kChunk / kDown;
+    static constexpr int kAcrossC = DC / kN, kDownC = kThreads / kAcrossC, kPerC = kChunk / kDownC;
+    Piece<T> b[kPer], c[kPerC];
     template <bool EVEN>
     __device__ __forceinline__ void load(const Rows<T, EVEN>& mb, const Rows<T, EVEN>& mc, int64_t base, int n) {
         const int t = threadIdx.x / kAcross, d = threadIdx.x % kAcross * kN;
+        const int tc = threadIdx.x / kAcrossC, e = threadIdx.x % kAcrossC * kN;
 #pragma unroll
         for (int u = 0; u < kPer; ++u) b[u] = mb.piece(base, t + u * kDown, d, n);
 #pragma unroll
-        for (int u = 0; u < kPer; ++u) c[u] = mc.piece(base, t + u * kDown, d, n);
+        for (int u = 0; u < kPerC; ++u) c[u] = mc.piece(base, tc + u * kDownC, e, n);
     }
     // zeros behind the rows' ends and behind the n positions
     template <typename L>
     __device__ __forceinline__ uint32_t store(L& l, int db, int dc, int n) const {
         const int t = threadIdx.x / kAcross, d = threadIdx.x % kAcross * kN;
+        const int tc = threadIdx.x / kAcrossC, e = threadIdx.x % kAcrossC * kN;
         uint32_t odd = 0;                 // whether c has something that is not finite
 #pragma unroll
         for (int u = 0; u < kPer; ++u) {
-            const uint32_t kb = d < db && t + u * kDown < n ? ~0u : 0u, kc = d < dc && t + u * kDown < n ? ~0u : 0u;
+            const uint32_t kb = d < db && t + u * kDown < n ? ~0u : 0u, kc = e < dc && tc + u * kDownC < n ? ~0u : 0u;
             Piece<T> x, y;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { x.w[j] = b[u].w[j] & kb; y.w[j] = c[u].w[j] & kc; odd |= odd_bits<T>(y.w[j]); }
+            for (int j = 0; j < 4; ++j) {
+                x.w[j] = b[u].w[j] & kb;
+                if (u < kPerC) { y.w[j] = c[u].w[j] & kc; odd |= odd_bits<T>(y.w[j]); }
+            }
             lds_put(&l.b[t + u * kDown][d], x);
-            lds_put(&l.c[t + u * kDown][d], y);
+            if (u < kPerC) lds_put(&l.c[tc + u * kDownC][e], y);
         }
         return odd;
     }
@@ -299,9 +309,9 @@ struct Staged {
 
 // X of a workgroup: wave w owns the tiles of 16 columns w, w + kWaves, ...; tile (j, i): lane l has column l % 16, rows
 // (l / 16) * 4 + [0, 4) of the a side
-template <int DP>
+template <int DP, int DC>
 struct State {
-    static constexpr int kJ = DP / 16 / kWaves, kI = DP / 16;
+    static constexpr int kJ = DC / 16 / kWaves, kI = DP / 16;
     f32x4 x[kJ][kI];
     __device__ __forceinline__ void zero() {
 #pragma unroll
@@ -317,9 +327,9 @@ template <> inline constexpr int kParts<f16> = 2;
 template <> inline constexpr int kParts<bf16> = 3;
 
 // X <- l^end X + kv sum_s l^{end - s} b_s c_s^T, with l^{end - s} c_s in as many numbers of the type as it has
-template <typename T, int DP, typename L>
-__device__ __forceinline__ void update(State<DP>& S, const L& l, int end, float kv) {
-    constexpr int kN = Piece<T>::kN, kJ = State<DP>::kJ, kI = State<DP>::kI, kP = kParts<T>;
+template <typename T, int DP, int DC, typename L>
+__device__ __forceinline__ void update(State<DP, DC>& S, const L& l, int end, float kv) {
+    constexpr int kN = Piece<T>::kN, kJ = State<DP, DC>::kJ, kI = State<DP, DC>::kI, kP = kParts<T>;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane >> 4;
     const float whole = l.lam[kChunk + end];
 #pragma unroll
@@ -334,7 +344,7 @@ __device__ __forceinline__ void update(State<DP>& S, const L& l, int end, float 
 #pragma unroll
         for (int e = 0; e < kN; ++e) f[e] = l.lam[kChunk + end - s0 - e];   // (rows behind the end are zeros, and their factors)
 #pragma unroll
-        for (int j = 0; j < kJ; ++j) c[j] = lds_column(&l.c[s0][(w + kWaves * j) * 16], L::kRow);
+        for (int j = 0; j < kJ; ++j) c[j] = lds_column(&l.c[s0][(w + kWaves * j) * 16], L::kRowC);
         __builtin_amdgcn_sched_barrier(0);
         Piece<T> part[kJ][kP];
 #pragma unroll
@@ -367,13 +377,13 @@ __device__ __forceinline__ void update(State<DP>& S, const L& l, int end, float 
 }
 
 // A caller's state, [da, dc] values with the strides sa, sc: to and from a workgroup's registers.
-template <int DP>
-__device__ __forceinline__ void state_load(State<DP>& S, const SAMX_GLOBAL float* m, int da, int dc, int sa, int sc, float f) {
+template <int DP, int DC>
+__device__ __forceinline__ void state_load(State<DP, DC>& S, const SAMX_GLOBAL float* m, int da, int dc, int sa, int sc, float f) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
 #pragma unroll
-    for (int j = 0; j < State<DP>::kJ; ++j)
+    for (int j = 0; j < State<DP, DC>::kJ; ++j)
 #pragma unroll
-        for (int i = 0; i < State<DP>::kI; ++i)
+        for (int i = 0; i < State<DP, DC>::kI; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int c = (w + kWaves * j) * 16 + r16, a = i * 16 + q * 4 + e;
@@ -382,13 +392,13 @@ __device__ __forceinline__ void state_load(State<DP>& S, const SAMX_GLOBAL float
                 S.x[j][i][e] = there ? v * f : 0.f;
             }
 }
-template <int DP>
-__device__ __forceinline__ void state_store(const State<DP>& S, SAMX_GLOBAL float* m, int da, int dc, int sa, int sc) {
+template <int DP, int DC>
+__device__ __forceinline__ void state_store(const State<DP, DC>& S, SAMX_GLOBAL float* m, int da, int dc, int sa, int sc) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
 #pragma unroll
-    for (int j = 0; j < State<DP>::kJ; ++j)
+    for (int j = 0; j < State<DP, DC>::kJ; ++j)
 #pragma unroll
-        for (int i = 0; i < State<DP>::kI; ++i)
+        for (int i = 0; i < State<DP, DC>::kI; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int c = (w + kWaves * j) * 16 + r16, a = i * 16 + q * 4 + e;
@@ -396,13 +406,13 @@ __device__ __forceinline__ void state_store(const State<DP>& S, SAMX_GLOBAL floa
             }
 }
 // A segment's state in the workspace: all tiles, [columns][rows] dense; `turned`: the matrix that is wanted is its transpose.
-template <int DP>
-__device__ __forceinline__ void seg_load(State<DP>& S, const SAMX_GLOBAL float* m, bool turned) {
+template <int DP, int DC>
+__device__ __forceinline__ void seg_load(State<DP, DC>& S, const SAMX_GLOBAL float* m, bool turned) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
 #pragma unroll
-    for (int j = 0; j < State<DP>::kJ; ++j)
+    for (int j = 0; j < State<DP, DC>::kJ; ++j)
 #pragma unroll
-        for (int i = 0; i < State<DP>::kI; ++i) {
+        for (int i = 0; i < State<DP, DC>::kI; ++i) {
             const uint32_t c = (w + kWaves * j) * 16 + r16, a = i * 16 + q * 4;
             if (!turned) {
                 S.x[j][i] = *(const SAMX_GLOBAL f32x4*)(m + c * DP + a);
@@ -412,20 +422,20 @@ __device__ __forceinline__ void seg_load(State<DP>& S, const SAMX_GLOBAL float* 
             }
         }
 }
-template <int DP>
-__device__ __forceinline__ void seg_store(const State<DP>& S, SAMX_GLOBAL float* m) {
+template <int DP, int DC>
+__device__ __forceinline__ void seg_store(const State<DP, DC>& S, SAMX_GLOBAL float* m) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
 #pragma unroll
-    for (int j = 0; j < State<DP>::kJ; ++j)
+    for (int j = 0; j < State<DP, DC>::kJ; ++j)
 #pragma unroll
-        for (int i = 0; i < State<DP>::kI; ++i)
+        for (int i = 0; i < State<DP, DC>::kI; ++i)
             *(SAMX_GLOBAL f32x4*)(m + (uint32_t)(((w + kWaves * j) * 16 + r16) * DP + i * 16 + q * 4)) = S.x[j][i];
 }
 
 template <typename T, int DP, bool EVEN>
 __global__ __launch_bounds__(kThreads, 2) void kv_kernel(Args A) {
     extern __shared__ __attribute__((aligned(16))) char lds_[];
-    LdsKv<T, DP>& l = *reinterpret_cast<LdsKv<T, DP>*>(lds_);
+    LdsKv<T, DP, DP>& l = *reinterpret_cast<LdsKv<T, DP, DP>*>(lds_);
     Place p;
     if (!place_of(A, A.nseg - 1, p)) return;
     const int64_t at = (int64_t)p.seg * A.seg_len;
@@ -433,18 +443,18 @@ __global__ __launch_bounds__(kThreads, 2) void kv_kernel(Args A) {
     const Role r = A.r[p.role];
     const Rows<T, EVEN> b(r.b, p, r.rev), c(r.c, p, r.rev);
     if (threadIdx.x <= 2 * kChunk) l.lam[threadIdx.x] = threadIdx.x < kChunk ? 0.f : power(p.g, threadIdx.x - kChunk);
-    State<DP> S;
+    State<DP, DP> S;
     S.zero();
-    Staged<T, DP> st;
+    Staged<T, DP, DP> st;
     st.load(b, c, at, kChunk);
     for (int64_t k = 0; k < A.seg_len; k += kChunk) {
         __syncthreads();
         st.store(l, r.b.dim, r.c.dim, kChunk);
         __syncthreads();
         if (k + kChunk < A.seg_len) st.load(b, c, at + k + kChunk, kChunk);
-        update<T, DP>(S, l, kChunk, r.kv);
+        update<T, DP, DP>(S, l, kChunk, r.kv);
     }
-    seg_store<DP>(S, (SAMX_GLOBAL float*)r.seg + ((int64_t)(p.b * A.H + p.h) * (A.nseg - 1) + p.seg) * A.seg_size);
+    seg_store<DP, DP>(S, (SAMX_GLOBAL float*)r.seg + ((int64_t)(p.b * A.H + p.h) * (A.nseg - 1) + p.seg) * A.seg_size);
 }
 
 // states at the segments' starts: X_{j+1} = l^len X_j + (segment j's own), over the segments that have a follower
@@ -477,24 +487,27 @@ __global__ __launch_bounds__(256) void join_kernel(Args A) {
     }
 }
 
-template <typename T, int DP, bool EVEN>
+template <typename T, int DP, int DC, bool EVEN>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void mix_kernel(Args A) {
     constexpr int kN = Piece<T>::kN, kInner = 4 * kN, kK = DP / kInner;      // inner values of one mma
     extern __shared__ __attribute__((aligned(16))) char lds_[];
-    Lds<T, DP>& l = *reinterpret_cast<Lds<T, DP>*>(lds_);
-    constexpr int kRow = LdsKv<T, DP>::kRow;
+    Lds<T, DP, DC>& l = *reinterpret_cast<Lds<T, DP, DC>*>(lds_);
+    constexpr int kRowC = LdsKv<T, DP, DC>::kRowC;
     Place p;
     if (!place_of(A, A.nseg, p)) return;
     // (by value: a reference into the arguments makes the compiler keep a copy of all of them in scratch memory)
     const Role r = A.r[p.role];
     // wave w: columns of a state; of a chunk, rows 16 w + [0, 16) of out
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
-    constexpr int kTiles = DP / 16;
+    constexpr int kTiles = DC / 16;
     const int64_t at = (int64_t)p.seg * A.seg_len, bh = (int64_t)p.b * A.H + p.h;
     const int64_t to = at + A.seg_len < p.L ? at + A.seg_len : p.L;         // this segment's positions
-    const int da = r.a.dim, dc = r.c.dim;
-    const int64_t out_row = (int64_t)A.H * dc;
-    const int64_t out_at = ((int64_t)p.b * A.T * A.H + p.h) * dc;
+    constexpr bool kShare = DC < DP;       // a workgroup has DC of the columns
+    const int c0 = kShare ? p.part * DC : 0;
+    const int da = r.a.dim, all = r.c.dim, dc = kShare && all - c0 > DC ? DC : all - c0;
+    if (kShare && dc <= 0) return;
+    const int64_t out_row = (int64_t)A.H * all;
+    const int64_t out_at = ((int64_t)p.b * A.T * A.H + p.h) * all + c0;
     SAMX_GLOBAL char* const outp = (SAMX_GLOBAL char*)r.out + out_at * (r.out_f32 ? 4 : (int)sizeof(T));
     // four of a row's outputs from d on, those that exist
     auto put4 = [=](auto f32, int64_t row, int d, f32x4 v) {
@@ -523,21 +536,21 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
                 else put4(std::false_type(), t, d, f32x4{0.f, 0.f, 0.f, 0.f});
             }
     }
-    State<DP> S;
-    const SAMX_GLOBAL float* s_in = r.s_in ? (const SAMX_GLOBAL float*)r.s_in + bh * da * dc : nullptr;
-    SAMX_GLOBAL float* s_out = r.s_out ? (SAMX_GLOBAL float*)r.s_out + bh * da * dc : nullptr;
+    State<DP, DC> S;
+    const SAMX_GLOBAL float* s_in = r.s_in ? (const SAMX_GLOBAL float*)r.s_in + bh * da * all + c0 * r.in_c : nullptr;
+    SAMX_GLOBAL float* s_out = r.s_out ? (SAMX_GLOBAL float*)r.s_out + bh * da * all + c0 * r.in_c : nullptr;
     if (p.L == 0) {    // nothing to read: the state goes through
         if (p.seg == 0 && s_out) {
-            if (s_in) state_load<DP>(S, s_in, da, dc, r.in_a, r.in_c, 1.f);
+            if (s_in) state_load<DP, DC>(S, s_in, da, dc, r.in_a, r.in_c, 1.f);
             else S.zero();
-            state_store<DP>(S, s_out, da, dc, r.in_a, r.in_c);
+            state_store<DP, DC>(S, s_out, da, dc, r.in_a, r.in_c);
         }
         return;
     }
     if (at >= to) return;
-    const Rows<T, EVEN> a(r.a, p, r.rev), b(r.b, p, r.rev), c(r.c, p, r.rev);
+    const Rows<T, EVEN> a(r.a, p, r.rev), b(r.b, p, r.rev), c(r.c, p, r.rev, c0);
     const int row = w * 16 + r16;          // of a chunk: this lane's
-    Staged<T, DP> st;
+    Staged<T, DP, DC> st;
     // a's rows of this wave, whole; behind their ends there is something of the row, which only meets zeros of b and X, and
     // a row that the chunk does not have is another one, whose outputs are not written
     Piece<T> af[kK];
@@ -549,8 +562,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
     st.load(b, c, at, rows_at(at));
     fetch_a(at);
     const bool last = to == p.L;           // this segment makes the state behind the last position
-    if (p.seg > 0) seg_load<DP>(S, (const SAMX_GLOBAL float*)r.seg + (bh * (A.nseg - 1) + p.seg - 1) * A.seg_size, r.turned);
-    else if (s_in) state_load<DP>(S, s_in, da, dc, r.in_a, r.in_c, r.rev ? 1.f : power(p.g, 1));
+    if (p.seg > 0) seg_load<DP, DC>(S, (const SAMX_GLOBAL float*)r.seg + (bh * (A.nseg - 1) + p.seg - 1) * A.seg_size + (r.turned ? c0 : c0 * DP), r.turned);
+    else if (s_in) state_load<DP, DC>(S, s_in, da, dc, r.in_a, r.in_c, r.rev ? 1.f : power(p.g, 1));
     else S.zero();
     if (threadIdx.x <= 2 * kChunk) l.lam[threadIdx.x] = threadIdx.x < kChunk ? 0.f : power(p.g, threadIdx.x - kChunk);
     if (threadIdx.x == 0) l.odd = 0u;
@@ -561,9 +574,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
         const uint32_t chunk = (uint32_t)((base - at) / kChunk) + 1u;
         if (st.store(l, da, dc, n)) l.odd = chunk;
 #pragma unroll
-        for (int j = 0; j < State<DP>::kJ; ++j)          // X's copy for the products with a
+        for (int j = 0; j < State<DP, DC>::kJ; ++j)          // X's copy for the products with a
 #pragma unroll
-            for (int i = 0; i < State<DP>::kI; ++i) {
+            for (int i = 0; i < State<DP, DC>::kI; ++i) {
                 const float v[4] = {S.x[j][i][0], S.x[j][i][1], S.x[j][i][2], S.x[j][i][3]};
                 lds_put4(&l.x[(w + kWaves * j) * 16 + r16][i * 16 + q * 4], v);
             }
@@ -624,7 +637,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
             [&](int g, int at) {
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
-                    f[at][t] = lds_column(&l.c[g / kFour * kInner + q * kN][(g % kFour * 4 + t) * 16], kRow);
+                    f[at][t] = lds_column(&l.c[g / kFour * kInner + q * kN][(g % kFour * 4 + t) * 16], kRowC);
             },
             [&](int g, int at) {
 #pragma unroll
@@ -667,11 +680,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
         }
         if (more || (last && s_out)) {
             // behind the last row the state of the forward recurrence has not been decayed once more
-            update<T, DP>(S, l, more ? kChunk : r.rev ? n : n - 1, r.kv);
+            update<T, DP, DC>(S, l, more ? kChunk : r.rev ? n : n - 1, r.kv);
         }
         if (more) __syncthreads();         // everybody has read the chunk
     }
-    if (last && s_out) state_store<DP>(S, s_out, da, dc, r.in_a, r.in_c);
+    if (last && s_out) state_store<DP, DC>(S, s_out, da, dc, r.in_a, r.in_c);
 }
 
 // sums of the query heads that share a key head: float32 [rows, HK, grp, dim] -> [rows, HK, dim] of the type
@@ -736,11 +749,12 @@ __global__ __launch_bounds__(256) void step_kernel(Mat Q, Mat K, Mat V, const fl
 // a sequence of c chunks takes c; in n segments it takes c / n, and half as much again for kv_kernel, 6 for the other two
 // launches and the states' way through memory, times the rounds in which the device takes all the workgroups, one for each
 // of its units (two at once take twice as long: they are bound by memory).  Measured (us), 2 x 4096 rows, 16 heads of 128,
-// bfloat16: n = 4 123, 8 81, 16 83; 8 x 512 rows: n = 1 45, 2 61, 4 64.
+// bfloat16: n = 4 97, 8 80, 16 89; gradient of 4 x 2048 ragged rows: n = 1 111, 2 157.
 void cut(Args& a) {
     const int64_t c = (a.T + kChunk - 1) / kChunk, units = (int64_t)a.B * a.H * a.roles, cu = cu_count();
     double best = 0.0;
     a.nseg = 1;
+    a.parts = 1;
     a.seg_len = (c < 1 ? 1 : c) * kChunk;
     for (int64_t n = 1; n <= c && n <= 64; ++n) {
         const int64_t each = (c + n - 1) / n, rounds = (units * n + cu - 1) / cu;
@@ -757,17 +771,32 @@ int launch(Args& a, const int (&joined)[2], int joins, hipStream_t st) {
     if (a.nseg > 1) {
         Args k = a;
         k.roles = joins;
+        k.parts = 1;
         for (int i = 0; i < joins; ++i) k.r[i] = a.r[joined[i]];
         static samx::LdsGrant grant;
-        if (int rc = grant.ensure((const void*)kv_kernel<T, DP, EVEN>, sizeof(LdsKv<T, DP>))) return rc;
-        kv_kernel<T, DP, EVEN><<<grid_of(k, a.nseg - 1), kThreads, sizeof(LdsKv<T, DP>), st>>>(k);
+        if (int rc = grant.ensure((const void*)kv_kernel<T, DP, EVEN>, sizeof(LdsKv<T, DP, DP>))) return rc;
+        kv_kernel<T, DP, EVEN><<<grid_of(k, a.nseg - 1), kThreads, sizeof(LdsKv<T, DP, DP>), st>>>(k);
         SAMX_LAUNCH_CHECK();
         join_kernel<DP><<<dim3(DP * DP / 256, (unsigned)(a.B * a.H), (unsigned)joins), 256, 0, st>>>(k);
         SAMX_LAUNCH_CHECK();
     }
     static samx::LdsGrant grant;
-    if (int rc = grant.ensure((const void*)mix_kernel<T, DP, EVEN>, sizeof(Lds<T, DP>))) return rc;
-    mix_kernel<T, DP, EVEN><<<grid_of(a, a.nseg), kThreads, sizeof(Lds<T, DP>), st>>>(a);
+    // As long as the device has a unit for every workgroup two of them share a head's columns, each with all the scores: two
+    // on a unit hide each other's waits.  Where it holds more anyway the scores made twice cost more.  One against two,
+    // bf16, 16 heads of 128: 8 x 512 rows 46 and 34 us, 16 x 1024 93 and 91, 32 x 1024 155 and 171; gradient of 4 x 2048
+    // ragged rows 151 and 111, of 16 x 1024 209 and 230.  (float32's tiles would not let two run on a unit.)
+    if constexpr (sizeof(T) == 2 && DP == 128) {
+        if ((int64_t)a.B * a.H * a.roles * a.nseg <= cu_count()) {
+            a.parts = 2;
+            static samx::LdsGrant half;
+            if (int rc = half.ensure((const void*)mix_kernel<T, DP, 64, EVEN>, sizeof(Lds<T, DP, 64>))) return rc;
+            mix_kernel<T, DP, 64, EVEN><<<grid_of(a, a.nseg), kThreads, sizeof(Lds<T, DP, 64>), st>>>(a);
+            SAMX_LAUNCH_CHECK();
+            return SAMX_OK;
+        }
+    }
+    if (int rc = grant.ensure((const void*)mix_kernel<T, DP, DP, EVEN>, sizeof(Lds<T, DP, DP>))) return rc;
+    mix_kernel<T, DP, DP, EVEN><<<grid_of(a, a.nseg), kThreads, sizeof(Lds<T, DP, DP>), st>>>(a);
     SAMX_LAUNCH_CHECK();
     return SAMX_OK;
 }
