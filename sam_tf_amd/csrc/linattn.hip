@@ -784,9 +784,10 @@ int launch(Args& a, const int (&joined)[2], int joins, hipStream_t st) {
     // As long as the device has a unit for every workgroup two of them share a head's columns, each with all the scores: two
     // on a unit hide each other's waits.  Where it holds more anyway the scores made twice cost more.  One against two,
     // bf16, 16 heads of 128: 8 x 512 rows 46 and 34 us, 16 x 1024 93 and 91, 32 x 1024 155 and 171; gradient of 4 x 2048
-    // ragged rows 151 and 111, of 16 x 1024 209 and 230.  (float32's tiles would not let two run on a unit.)
-    if constexpr (sizeof(T) == 2 && DP == 128) {
-        if ((int64_t)a.B * a.H * a.roles * a.nseg <= cu_count()) {
+    // ragged rows 151 and 111, of 16 x 1024 209 and 230.  float32's tiles leave LDS for one on a unit: there as long as both halves
+    // have a unit of their own (8 x 512 rows 155 and 95; gradient of 4 x 512 rows, 8 heads of 72 and 88, 132 and 84).
+    if constexpr (DP == 128) {
+        if ((int64_t)a.B * a.H * a.roles * a.nseg * (sizeof(T) == 4 ? 2 : 1) <= cu_count()) {
             a.parts = 2;
             static samx::LdsGrant half;
             if (int rc = half.ensure((const void*)mix_kernel<T, DP, 64, EVEN>, sizeof(Lds<T, DP, 64>))) return rc;

@@ -347,7 +347,7 @@ def test_what_is_not_finite_stays_with_its_rows(dtype, D, DV, bad, what):
             assert not bool(torch.isfinite(x[touched].flatten(1)).all(-1).any())
 
 
-@pytest.mark.parametrize('dtype,D,DV', [(BF16, 72, 100), (F16, 128, 128), (BF16, 40, 88), (F16, 96, 61)])
+@pytest.mark.parametrize('dtype,D,DV', [(BF16, 72, 100), (F16, 128, 128), (BF16, 40, 88), (F16, 96, 61), (F32, 72, 100), (F32, 128, 33)])
 def test_more_heads_than_units(dtype, D, DV):
     """Enough of them that a workgroup has all columns of a head (fewer: two workgroups share them)."""
     _check(_case(66, 66, 4, 2, D, DV, dtype, seed=9, lengths=[(7 * b) % 67 for b in range(66)]), 0.5, dtype)
