@@ -353,6 +353,33 @@ def test_more_heads_than_units(dtype, D, DV):
     _check(_case(66, 66, 4, 2, D, DV, dtype, seed=9, lengths=[(7 * b) % 67 for b in range(66)]), 0.5, dtype)
 
 
+@pytest.mark.parametrize('dtype,D,DV', [(BF16, 128, 128), (BF16, 100, 61), (F16, 72, 120), (BF16, 128, 40), (F16, 24, 128), (F32, 100, 72),
+                                        (F32, 65, 127)])
+def test_two_workgroups_of_a_head(dtype, D, DV):
+    """Few heads of more than 64 columns: ragged, of no rows, with and without a state, in segments."""
+    _check(_case(6, 150, 2, 1, D, DV, dtype, seed=6, lengths=[0, 1, 64, 65, 128, 150]), 0.3, dtype)
+    _check(_case(2, 20, 2, 2, D, DV, dtype, seed=7, lengths=[0, 20], state=False), 0.3, dtype)
+    _check(_case(1, 700, 2, 2, D, DV, dtype, seed=8), 0.1, dtype)
+
+
+def test_two_streams_at_once():
+    """Calls that overlap on two streams, each with its own workspace, and one after the other: the same numbers."""
+    from sam_tf_amd import ops
+    cs = [_gpu(_case(2, 1500, 3, 3, 128, 128, BF16, seed=s)) for s in (20, 21)]
+    run = lambda c: (ops.linattn(c['q'], c['k'], c['v'], c['decay'], 0.1, c['state']) +
+                     ops.linattn_grad(c['q'], c['k'], c['v'], c['decay'], c['dout'], 0.1, c['state'], c['dstate']))
+    want = [run(c) for c in cs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for c, st in zip(cs, streams):
+            with torch.cuda.stream(st):
+                got.append(run(c))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
 def test_rows_far_apart():
     """Rows 2^31 bytes from each other: offsets of 64 bits, and the same numbers."""
     from sam_tf_amd import ops
