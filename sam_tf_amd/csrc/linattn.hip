@@ -26,8 +26,9 @@
 // Measured, 16 heads of 128, bf16.  32 x 1024 rows (two workgroups for each compute unit, no segments): 155 us, 3900 GB/s of
 // 4750 that a large copy reaches.  2 x 4096 rows: 81 us in 8 segments (kv 23, join 9, mix 45), the keys and values read
 // twice.  Gradient of 4 x 2048 ragged rows: 111 us, two workgroups for each head's columns (of one for all of them a chunk
-// took 4.6 us: the state's update 1.2, the stores 0.7, waiting for loads 0.6, the other products' chain the rest).  float32: its matrix instructions have a
-// sixteenth of the rate, and its tiles leave LDS for one workgroup a unit (2 x 4096 rows 205 us).
+// took 4.6 us: the state's update 1.2, the stores 0.7, waiting for loads 0.6, the other products' chain the rest).
+// float32: its matrix instructions have a sixteenth of the rate, and its tiles leave LDS for one workgroup a unit
+// (2 x 4096 rows 205 us).
 #include "seq_dev.h"
 #include "../../include/samx.h"
 #include <type_traits>
@@ -562,7 +563,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
     st.load(b, c, at, rows_at(at));
     fetch_a(at);
     const bool last = to == p.L;           // this segment makes the state behind the last position
-    if (p.seg > 0) seg_load<DP, DC>(S, (const SAMX_GLOBAL float*)r.seg + (bh * (A.nseg - 1) + p.seg - 1) * A.seg_size + (r.turned ? c0 : c0 * DP), r.turned);
+    if (p.seg > 0) seg_load<DP, DC>(S, (const SAMX_GLOBAL float*)r.seg + (bh * (A.nseg - 1) + p.seg - 1) * A.seg_size +
+                                           (r.turned ? c0 : c0 * DP), r.turned);
     else if (s_in) state_load<DP, DC>(S, s_in, da, dc, r.in_a, r.in_c, r.rev ? 1.f : power(p.g, 1));
     else S.zero();
     if (threadIdx.x <= 2 * kChunk) l.lam[threadIdx.x] = threadIdx.x < kChunk ? 0.f : power(p.g, threadIdx.x - kChunk);
@@ -784,8 +786,8 @@ int launch(Args& a, const int (&joined)[2], int joins, hipStream_t st) {
     // As long as the device has a unit for every workgroup two of them share a head's columns, each with all the scores: two
     // on a unit hide each other's waits.  Where it holds more anyway the scores made twice cost more.  One against two,
     // bf16, 16 heads of 128: 8 x 512 rows 46 and 34 us, 16 x 1024 93 and 91, 32 x 1024 155 and 171; gradient of 4 x 2048
-    // ragged rows 151 and 111, of 16 x 1024 209 and 230.  float32's tiles leave LDS for one on a unit: there as long as both halves
-    // have a unit of their own (8 x 512 rows 155 and 95; gradient of 4 x 512 rows, 8 heads of 72 and 88, 132 and 84).
+    // ragged rows 151 and 111, of 16 x 1024 209 and 230.  float32's tiles leave LDS for one on a unit: there as long as both
+    // halves have a unit of their own (8 x 512 rows 155 and 95; gradient of 4 x 512 rows, 8 heads of 72 and 88, 132 and 84).
     if constexpr (DP == 128) {
         if ((int64_t)a.B * a.H * a.roles * a.nseg * (sizeof(T) == 4 ? 2 : 1) <= cu_count()) {
             a.parts = 2;
@@ -866,7 +868,8 @@ int samx_linattn(const samx_linattn_shape* s, const void* q, const void* k, cons
     cut(a);
     const size_t need = seg_bytes(a, s->D, s->DV);
     SAMX_REQUIRE(!need || ((uintptr_t)ws & 15) == 0, "samx_linattn: the workspace has to be 16-byte aligned");
-    if (need && (!ws || ws_bytes < need)) return samx::fail(SAMX_ERR_WORKSPACE, "samx_linattn: workspace %zu < %zu", ws_bytes, need);
+    if (need && (!ws || ws_bytes < need))
+        return samx::fail(SAMX_ERR_WORKSPACE, "samx_linattn: workspace %zu < %zu", ws_bytes, need);
     const int rep = s->H / s->HK;
     a.seg_size = seg_size(s->D, s->DV);
     Role& r = a.r[0];
@@ -896,7 +899,8 @@ int samx_linattn_grad(const samx_linattn_shape* s, const void* q, const void* k,
     SAMX_REQUIRE(((q && k && v && dout && dq && dk && dv) || s->T == 0) && decay && dstate_in, "samx_linattn_grad: null pointer");
     const size_t need = samx_linattn_grad_ws_bytes(s) - 256;
     SAMX_REQUIRE(!need || ((uintptr_t)ws & 15) == 0, "samx_linattn_grad: the workspace has to be 16-byte aligned");
-    if (need && (!ws || ws_bytes < need)) return samx::fail(SAMX_ERR_WORKSPACE, "samx_linattn_grad: workspace %zu < %zu", ws_bytes, need);
+    if (need && (!ws || ws_bytes < need))
+        return samx::fail(SAMX_ERR_WORKSPACE, "samx_linattn_grad: workspace %zu < %zu", ws_bytes, need);
     Args a{};
     a.roles = 3; a.B = (int)s->B; a.H = s->H; a.T = s->T; a.decay = decay; a.lengths = lengths;
     cut(a);
