@@ -674,8 +674,9 @@ int samx_block_norm_grad(const void* y, const void* h, const void* dh, const voi
  * state float32 [B, H, D, DV] dense, state_in NULL: zero.  lengths int32 [B] (NULL: T): rows of each sequence that are there
  * (taken into [0, T]); rows behind them are not read, their outputs are zeros, the state behind a sequence is that of its
  * last row.  out, dq, dk, dv are dense; no output overlaps an input.  Scores and the state are float32; products of 16-bit
- * types take the scores and, for out, the state in their own type (of float16, both have to be within its range).  An infinity
- * or a NaN of a row reaches what the recurrence takes it to and nothing else; behind it an infinity may have become a NaN. */
+ * types take the scores and, for out, a copy of the state rounded to their own type, half a step each beside the output's own
+ * (float16: as fractions of a power of two, so that neither has to be within its range).  An infinity or a NaN of a row
+ * reaches what the recurrence takes it to and nothing else; behind it an infinity may have become a NaN. */
 typedef struct samx_linattn_shape {
     int32_t dtype, H, HK, D, DV, pad;
     int64_t B, T;

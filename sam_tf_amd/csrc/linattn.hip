@@ -17,7 +17,8 @@
 // X <- l^64 X + sum_s l^{64-s} b_s c_s^T.  X stays in the registers of the workgroup (float32; each wave owns whole
 // columns).  Operands of 16 bits enter the matrix cores as they are; P and the copy of X that meets a are rounded to
 // their type (an output of that type is rounded again), but l^{64-s} c_s is split into numbers of the type whose sum it is,
-// so that the state, a float32 output, is one.  float32 operands use the float32 matrix instructions throughout.
+// so that the state, a float32 output, is one.  float16, which has too few exponents for any of these, takes each as a
+// fraction of a power of two (Scale).  float32 operands use the float32 matrix instructions throughout.
 //
 // Where batch times heads is less than the device holds, time is cut into segments: kv_kernel makes each segment's own
 // contribution to the state behind it, join_kernel runs the recurrence over the segments, mix_kernel does the rest with
@@ -228,6 +229,25 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// float16: values that are to be rounded to it, or split into parts of it, are first taken to a power of two's fractions, so
+// that the largest of those that share it stands in [2^14, 2^15): none overflows, and what is below 2^-39 of the largest is all
+// that is lost.  One power for each column of c and of X and one for each row of P: lanes of one l % 16.  (Without it a value
+// of the state beyond 65504 was an infinity to its rows, and the state of values around 1e-5 had a few per cent of error.)
+// It costs: 32 x 1024 rows, 16 heads of 128, 180 us where bfloat16 takes 146; the gradient of 4 x 2048 rows 161, not 134.
+template <typename T> constexpr bool kScaled = std::is_same<T, f16>::value;
+struct Scale { float up, down; };              // the power and one over it
+// of values whose magnitudes are at most `most` (in this lane); none below 2^(least - 127 - 14)
+__device__ __forceinline__ Scale scale_of(float most, uint32_t least = 15) {
+    // (rows of lanes exchanged by the vector unit; by LDS's permutation the gradient of 2 x 4096 rows took 197 us, not 184)
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(most), __float_as_uint(most), false, false);
+    most = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
+    most = fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
+    uint32_t e = __float_as_uint(most) >> 23;
+    e = e < least ? least : e > 254u ? 254u : e;
+    return {__uint_as_float((e - 14u) << 23), __uint_as_float((268u - e) << 23)};
+}
+
 // LDS rows are 16 bytes longer than their contents: 16 lanes that read 16 rows at one column use all banks
 template <typename T, int DP, int DC>
 struct LdsKv {
@@ -242,6 +262,7 @@ struct Lds : LdsKv<T, DP, DC> {
     static_assert(sizeof(LdsKv<T, DP, DC>) % 16 == 0, "pieces are read whole");
     T p[4][16][kTok];                                    // each wave's 16 rows of scores
     T x[DC][LdsKv<T, DP, DC>::kRow];                     // X, a row for each column
+    float xs[kScaled<T> ? DC : 4];                       // the power of two of each of these rows
 };
 
 // N groups of products, group g's operands read (into buf[g % (AHEAD + 1)]) AHEAD groups before they are used; nothing is
@@ -324,7 +345,7 @@ struct State {
 
 // numbers of the type whose sum a float32 is
 template <typename T> constexpr int kParts = 1;
-template <> inline constexpr int kParts<f16> = 2;
+template <> inline constexpr int kParts<f16> = 3;
 template <> inline constexpr int kParts<bf16> = 3;
 
 // X <- l^end X + kv sum_s l^{end - s} b_s c_s^T, with l^{end - s} c_s in as many numbers of the type as it has
@@ -348,11 +369,21 @@ __device__ __forceinline__ void update(State<DP, DC>& S, const L& l, int end, fl
         for (int j = 0; j < kJ; ++j) c[j] = lds_column(&l.c[s0][(w + kWaves * j) * 16], L::kRowC);
         __builtin_amdgcn_sched_barrier(0);
         Piece<T> part[kJ][kP];
+        float up[kJ];
 #pragma unroll
         for (int j = 0; j < kJ; ++j) {
             float v[kN];
 #pragma unroll
             for (int e = 0; e < kN; ++e) v[e] = c[j].f(e) * (kv * f[e]);
+            if constexpr (kScaled<T>) {
+                float most = 0.f;
+#pragma unroll
+                for (int e = 0; e < kN; ++e) most = fmaxf(most, fabsf(v[e]));
+                const Scale s = scale_of(most);
+                up[j] = s.up;
+#pragma unroll
+                for (int e = 0; e < kN; ++e) v[e] *= s.down;
+            }
 #pragma unroll
             for (int u = 0; u < kP; ++u) {
                 part[j][u] = pack<T>(v);
@@ -367,12 +398,24 @@ __device__ __forceinline__ void update(State<DP, DC>& S, const L& l, int end, fl
                 for (int i = 0; i < 4; ++i) b[at][i] = lds_column(&l.b[s0][(g * 4 + i) * 16], L::kRow);
             },
             [&](int g, int at) {
+                f32x4 d[kJ][4];
+#pragma unroll
+                for (int j = 0; j < kJ; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) d[j][i] = kScaled<T> ? f32x4{0.f, 0.f, 0.f, 0.f} : S.x[j][g * 4 + i];
 #pragma unroll
                 for (int u = 0; u < kP; ++u)
 #pragma unroll
                     for (int j = 0; j < kJ; ++j)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) S.x[j][g * 4 + i] = mma(b[at][i], part[j][u], S.x[j][g * 4 + i]);
+                        for (int i = 0; i < 4; ++i) d[j][i] = mma(b[at][i], part[j][u], d[j][i]);
+#pragma unroll
+                for (int j = 0; j < kJ; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (kScaled<T>) S.x[j][g * 4 + i] += up[j] * d[j][i];
+                        else S.x[j][g * 4 + i] = d[j][i];
+                    }
             });
     }
 }
@@ -576,12 +619,27 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
         const uint32_t chunk = (uint32_t)((base - at) / kChunk) + 1u;
         if (st.store(l, da, dc, n)) l.odd = chunk;
 #pragma unroll
-        for (int j = 0; j < State<DP, DC>::kJ; ++j)          // X's copy for the products with a
+        for (int j = 0; j < State<DP, DC>::kJ; ++j) {        // X's copy for the products with a
+            float down = 1.f;
+            if constexpr (kScaled<T>) {
+                float most = 0.f;
+#pragma unroll
+                for (int i = 0; i < State<DP, DC>::kI; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(S.x[j][i][e]));
+                const Scale s = scale_of(most);
+                down = s.down;
+                if (q == 0) l.xs[(w + kWaves * j) * 16 + r16] = s.up;
+            }
 #pragma unroll
             for (int i = 0; i < State<DP, DC>::kI; ++i) {
-                const float v[4] = {S.x[j][i][0], S.x[j][i][1], S.x[j][i][2], S.x[j][i][3]};
+                float v[4] = {S.x[j][i][0], S.x[j][i][1], S.x[j][i][2], S.x[j][i][3]};
+                if constexpr (kScaled<T>)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] *= down;
                 lds_put4(&l.x[(w + kWaves * j) * 16 + r16][i * 16 + q * 4], v);
             }
+        }
         __syncthreads();
         if (more) st.load(b, c, base + kChunk, rows_at(base + kChunk));
         // scores, transposed: column = this wave's row, rows = positions s.  (Nothing here branches on the wave: no read
@@ -619,8 +677,24 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
 #pragma unroll
             for (int e = 0; e < 4; ++e) lam[t][e] = l.lam[kChunk + row - (t * 16 + q * 4 + e)];
         __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!kScaled<T>)
 #pragma unroll
-        for (int j = 0; j < kTiles; ++j) o[j] *= decayed;
+            for (int j = 0; j < kTiles; ++j) o[j] *= decayed;
+        Scale ps{1.f, 1.f};
+        if constexpr (kScaled<T>) {
+            float most = 0.f;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) most = fmaxf(most, row >= t * 16 + q * 4 + e ? fabsf(r.ps * lam[t][e] * sc[t][e]) : 0.f);
+            // (not below 2^-54: a X is divided by it, and such scores add nothing to an output of this type)
+            ps = scale_of(most, 127 - 40);
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j) {
+                const f32x4 s = *reinterpret_cast<const f32x4*>(&l.xs[j * 16 + q * 4]);
+                o[j] *= s * (decayed * ps.down);
+            }
+        }
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             float v[4];
@@ -628,6 +702,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
             for (int e = 0; e < 4; ++e) {   // (l^d is 0 behind the row, but 0 times a NaN is none)
                 const float x = r.ps * lam[t][e] * sc[t][e];
                 v[e] = row >= t * 16 + q * 4 + e ? x : 0.f;
+                if constexpr (kScaled<T>) v[e] *= ps.down;
             }
             lds_put4(&l.p[w][r16][t * 16 + q * 4], v);
         }
@@ -648,6 +723,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
                     d = mma(f[at][t], pk[g / kFour], d);
                 }
             });
+        if constexpr (kScaled<T>)
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j) o[j] *= ps.up;
         if (row < n) {
             const int64_t tok = r.rev ? p.L - 1 - (base + row) : base + row;
             if (wide) {
@@ -671,8 +749,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
                     for (int e = 0; e < 4; ++e) v[e] += x * to_float(l.x[d + e][i]);
                 }
                 v *= decayed;
+                if constexpr (kScaled<T>) v *= *reinterpret_cast<const f32x4*>(&l.xs[d]);
                 for (int t = 0; t <= row; ++t) {
-                    const float x = to_float(l.p[w][r16][t]);
+                    const float x = to_float(l.p[w][r16][t]) * ps.up;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] += x * to_float(l.c[t][d + e]);
                 }

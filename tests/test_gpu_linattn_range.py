@@ -1,0 +1,101 @@
+"""Linear attention of float16 near both ends of the type's range, and float32 states whatever the operands' type: against the
+float64 recurrence (tests/seq_ref.py)."""
+import pytest
+import torch
+
+from tests import seq_ref as R
+from tests.seq_ref import U32, half_step, smallest, within
+from tests.test_gpu_linattn import BF16, F16, F32, _abs, _case, _d, _errors, _gpu
+
+pytestmark = pytest.mark.gpu
+
+# factors of (q, k, v, dout, state, dstate), scale
+ENDS = {
+    'small gradient': ((1, 1, 1, 1e-3, 1, 1e-3), 0.125),
+    'smaller gradient': ((1, 1, 1, 1e-5, 1, 1e-5), 0.125),
+    'smallest gradient': ((1, 1, 1, 1e-6, 1, 0), 0.125),
+    'small values': ((1, 1, 1e-3, 1, 1e-3, 1), 0.125),
+    'smaller values': ((1, 1, 1e-5, 1, 1e-5, 1), 0.125),
+    'small queries and keys': ((1e-4, 1e-4, 100, 1, 1e-4, 1), 10.0),
+    'large state': ((1e-3, 1, 1, 1e-3, 1e6, 1), 0.01),
+    'large state gradient': ((1, 1e-3, 1e-3, 1, 1, 1e6), 0.01),
+    'large scores': ((300, 300, 1e-4, 1e-4, 1e-3, 1e-3), 0.02),
+    'large scale': ((1e-2, 1e-2, 1e-2, 100, 1e-3, 1), 1000.0),
+    'large everywhere': ((1000, 1000, 1000, 1000, 1e6, 1), 1e-9),
+}
+
+
+def _scaled(c, factors, dtype):
+    for n, f in zip(('q', 'k', 'v', 'dout', 'state', 'dstate'), factors):
+        c[n] = (c[n].float() * f).to(F32 if 'state' in n else dtype)
+    return c
+
+
+def _most(t):
+    return float(t.double().abs().max())
+
+
+def _hold(c, scale, dtype, what=''):
+    """States are float32: the bound is that of float32 operands.  Outputs: a step of the type where scores and state meet the
+    values, relative, and one for the output itself.  The last term of both: of a column (or a row of scores) whose largest
+    value is m, float16 keeps what is above 2^-39 m; T rows and two such products meet."""
+    from sam_tf_amd import ops
+    g, d = _gpu(c), _d(c)
+    a = _abs(d)
+    B, T, H, D = c['q'].shape
+    DV = c['v'].shape[3]
+    es, eo, h = _errors(F32, T, D, DV)[0], _errors(dtype, T, D, DV)[0], 1.01 * half_step(dtype)
+    q, k, v, o = (_most(c[n]) for n in ('q', 'k', 'v', 'dout'))
+    dim, low = max(D, DV), 2.0 ** -38 * (T + 64)
+    S, G = _most(c['state']) + T * k * v, _most(c['dstate']) + T * scale * q * o
+    run = lambda x: (R.linattn(x['q'], x['k'], x['v'], d['decay'], scale, x['state'], d['lengths']) +
+                     R.linattn_grad(x['q'], x['k'], x['v'], d['decay'], x['dout'], scale, x['state'], x['dstate'], d['lengths']))
+    want, size = run(d), run(a)
+    assert all(_most(want[i]) < 65504 for i in (0, 2, 3, 4)), 'the case itself is beyond float16'
+    got = (ops.linattn(g['q'], g['k'], g['v'], g['decay'], scale=scale, state=g['state'], lengths=g['lengths']) +
+           ops.linattn_grad(g['q'], g['k'], g['v'], g['decay'], g['dout'], scale=scale, state=g['state'], dstate=g['dstate'],
+                            lengths=g['lengths']))
+    rep = H // c['k'].shape[2]
+    lows = [low * x for x in (scale * q * dim * S, k * v, scale * o * dim * S, rep * v * dim * G, rep * k * dim * G, scale * q * o)]
+    for i, n in enumerate(('out', 'state', 'dq', 'dk', 'dv', 'dstate')):
+        e, r, t = (es, 0.0, 0.0) if 'state' in n else (eo + (H + 2) * U32, h, smallest(dtype))
+        within(got[i], want[i], e * size[i] + r * want[i].abs() + t + lows[i], what + ' ' + n)
+
+
+@pytest.mark.parametrize('D,DV,HK', [(64, 64, 2), (128, 128, 2), (40, 100, 1), (77, 33, 2)])
+@pytest.mark.parametrize('end', sorted(ENDS))
+def test_float16_at_the_ends_of_its_range(end, D, DV, HK):
+    f, scale = ENDS[end]
+    _hold(_scaled(_case(2, 150, 2, HK, D, DV, F16, seed=31, lengths=[150, 97]), f, F16), scale, F16)
+
+
+@pytest.mark.parametrize('end', ['smaller gradient', 'small values', 'large state', 'large scores', 'large scale'])
+def test_float16_at_the_ends_in_segments(end):
+    f, scale = ENDS[end]
+    _hold(_scaled(_case(1, 1100, 2, 2, 72, 64, F16, seed=32), f, F16), scale, F16)
+
+
+@pytest.mark.parametrize('end', ['smaller gradient', 'large state', 'large scores'])
+def test_float16_at_the_ends_of_more_heads_than_units(end):
+    f, scale = ENDS[end]
+    _hold(_scaled(_case(66, 70, 4, 4, 72, 100, F16, seed=33, lengths=[70 - b for b in range(66)]), f, F16), scale, F16)
+
+
+@pytest.mark.parametrize('dtype', [BF16, F16])
+def test_columns_of_different_size(dtype):
+    """Each column of v and dout by its own power of two, from 2^-14 to 2^8: the small ones' states as exact as the large ones'."""
+    c = _case(2, 200, 2, 2, 48, 46, dtype, seed=34)
+    p = 2.0 ** torch.linspace(-14, 8, 46).round()
+    for n in ('v', 'dout'):
+        c[n] = (c[n].float() * p).to(dtype)
+    from sam_tf_amd import ops
+    g, d = _gpu(c), _d(c)
+    a = _abs(d)
+    S = ops.linattn(g['q'], g['k'], g['v'], g['decay'], scale=0.1)[1]
+    dS = ops.linattn_grad(g['q'], g['k'], g['v'], g['decay'], g['dout'], scale=0.1)[3]
+    f = lambda x: (R.linattn(x['q'], x['k'], x['v'], d['decay'], 0.1, None, None)[1],
+                   R.linattn_grad(x['q'], x['k'], x['v'], d['decay'], x['dout'], 0.1, None, None, None)[3])
+    e = _errors(F32, 200, 48, 46)[0]
+    for x, w, m, n in zip((S, dS), f(d), f(a), ('state', 'dstate')):
+        most = m.amax((0, 1, 2))               # of a column
+        within(x, w, e * m + 2.0 ** -38 * 264 * most, n)
