@@ -99,3 +99,41 @@ def test_columns_of_different_size(dtype):
     for x, w, m, n in zip((S, dS), f(d), f(a), ('state', 'dstate')):
         most = m.amax((0, 1, 2))               # of a column
         within(x, w, e * m + 2.0 ** -38 * 264 * most, n)
+
+
+@pytest.mark.parametrize('what', ['q', 'k', 'v', 'dout'])
+@pytest.mark.parametrize('bad', [float('nan'), float('inf')])
+@pytest.mark.parametrize('dtype,D,DV', [(F32, 24, 40), (BF16, 40, 24), (F16, 64, 64), (F16, 100, 128), (BF16, 128, 128)])
+def test_rows_beside_one_that_is_not_finite(dtype, D, DV, bad, what):
+    """Row 75 of sequence 1 has a value that is not finite.  Rows that do not meet it, those of its own chunk among them, are as
+    they were: the same products in another order, each order within _errors of the sum of magnitudes, rounded once each."""
+    from sam_tf_amd import ops
+    T, H, HK, at, scale = 150, 4, 2, 75, 0.5
+    c0 = _case(2, T, H, HK, D, DV, dtype, seed=35)
+    a = _abs(_d(c0))
+    size = R.linattn(a['q'], a['k'], a['v'], a['decay'], scale, a['state'], None)[:1] + R.linattn_grad(
+        a['q'], a['k'], a['v'], a['decay'], a['dout'], scale, a['state'], a['dstate'], None)[:3]
+    error, step = _errors(dtype, T, D, DV)[0], 1.01 * half_step(dtype)
+    c = _gpu(c0)
+
+    def run():
+        o = ops.linattn(c['q'], c['k'], c['v'], c['decay'], scale, c['state'])[:1]
+        return o + ops.linattn_grad(c['q'], c['k'], c['v'], c['decay'], c['dout'], scale, c['state'], c['dstate'])[:3]
+    want = run()
+    c[what][1, at, 1 if what in ('q', 'dout') else 0, 3] = bad
+    got = run()
+    meets = [1] if what in ('q', 'dout') else [0, 1]               # query heads that meet it; their key head is 0
+    none, only, behind, upto = slice(0, 0), slice(at, at + 1), slice(at, None), slice(None, at + 1)
+    rows = {'q': (only, none, upto, upto), 'dout': (none, only, upto, upto),
+            'k': (behind, behind, none, only), 'v': (behind, behind, only, none)}[what]
+    q, k, v, o, S, dS = (_most(c0[n]) for n in ('q', 'k', 'v', 'dout', 'state', 'dstate'))
+    S, G = S + T * k * v, dS + T * scale * q * o
+    low = 2.0 ** -38 * (T + 64) * max(D, DV) * max(scale * q * S, scale * o * S, 2 * v * G, 2 * k * G)      # (as in _hold)
+    for x, w, r, m, n in zip(got, want, rows, size, ('out', 'dq', 'dk', 'dv')):
+        same = torch.ones(x.shape[:3], dtype=torch.bool)
+        same[1, r, meets if n in ('out', 'dq') else [0]] = False
+        x, w = x.cpu().double(), w.cpu().double()
+        tol = 2 * (error + (H + 2) * U32) * m + 2 * step * w.abs() + 2 * smallest(dtype) + low
+        within(x[same], w[same], tol[same], n)
+        if not bool(same.all()):
+            assert not bool(torch.isfinite(x[~same]).all(-1).any()), n
