@@ -913,7 +913,7 @@ int check(const char* who, const samx_linattn_shape* s) {
                  (long long)s->T, s->H, s->HK);
     SAMX_REQUIRE(s->D > 0 && s->D <= kMaxDim && s->DV > 0 && s->DV <= kMaxDim, "%s: head dimensions %d, %d must be in [1, %d]", who,
                  s->D, s->DV, kMaxDim);
-    SAMX_REQUIRE(s->B * s->H <= 65535, "%s: B * H %lld is more than 65535", who, (long long)(s->B * s->H));
+    SAMX_REQUIRE(s->B <= 65535 && s->B * s->H <= 65535, "%s: B %lld times H %d is more than 65535", who, (long long)s->B, s->H);
     return SAMX_OK;
 }
 
