@@ -667,7 +667,7 @@ int samx_block_norm_grad(const void* y, const void* h, const void* dh, const voi
                          float* dpost_b, float* dpre_w, float* dpre_b, void* ws, size_t ws_bytes, void* stream);
 
 /* Linear attention with a decay for each head, over B sequences of T rows with H query heads of D and HK key heads (H a
- * multiple of HK: the query heads h of key head h / (H / HK)) of D, their values of DV; D, DV at most 128, B * H at most 65535:
+ * multiple of HK: the query heads h of key head h / (H / HK)) of D, their values of DV; D, DV at most 128, B * H at most 131072:
  *   S_t = e^{decay_h} S_{t-1} + k_t v_t^T ;  out_t = scale q_t^T S_t
  * q [B, T, H, D], k [B, T, HK, D], v [B, T, HK, DV], dout [B, T, H, DV] of the element type, dense in the last dimension, other
  * strides (in elements: batch, row, head) as given; decay float32 [H], the logarithm of the factor (<= 0, -inf: no memory);

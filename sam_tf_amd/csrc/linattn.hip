@@ -43,6 +43,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kChunk = 64, kMaxDim = 128;
+constexpr int64_t kMaxHeads = 131072;   // of all sequences: three roles' workgroups of 256 threads are far fewer than 2^32 threads
 constexpr int kWaves = 4, kThreads = kWaves * 64;   // a wave for each 16 rows of a chunk
 
 // D += A B^T for 16 rows each and the kN * 4 inner values that 64 lanes' pieces hold: lane l has row l % 16, inner values
@@ -506,8 +507,8 @@ template <int DP>
 __global__ __launch_bounds__(256) void join_kernel(Args A) {
     constexpr int U = 8;
     const Role& r = A.r[blockIdx.z];
-    const int64_t bh = blockIdx.y;
-    const int e = blockIdx.x * 256 + threadIdx.x, na = r.b.dim, nc = r.c.dim, states = A.nseg - 1;
+    const int64_t bh = blockIdx.x;
+    const int e = blockIdx.y * 256 + threadIdx.x, na = r.b.dim, nc = r.c.dim, states = A.nseg - 1;
     const int b = (int)(bh / A.H), h = (int)(bh % A.H);
     int64_t L = A.T;
     if (A.lengths) L = A.lengths[b] < A.T ? A.lengths[b] : A.T;
@@ -858,7 +859,7 @@ int launch(Args& a, const int (&joined)[2], int joins, hipStream_t st) {
         if (int rc = grant.ensure((const void*)kv_kernel<T, DP, EVEN>, sizeof(LdsKv<T, DP, DP>))) return rc;
         kv_kernel<T, DP, EVEN><<<grid_of(k, a.nseg - 1), kThreads, sizeof(LdsKv<T, DP, DP>), st>>>(k);
         SAMX_LAUNCH_CHECK();
-        join_kernel<DP><<<dim3(DP * DP / 256, (unsigned)(a.B * a.H), (unsigned)joins), 256, 0, st>>>(k);
+        join_kernel<DP><<<dim3((unsigned)(a.B * a.H), DP * DP / 256, (unsigned)joins), 256, 0, st>>>(k);
         SAMX_LAUNCH_CHECK();
     }
     static samx::LdsGrant grant;
@@ -913,7 +914,8 @@ int check(const char* who, const samx_linattn_shape* s) {
                  (long long)s->T, s->H, s->HK);
     SAMX_REQUIRE(s->D > 0 && s->D <= kMaxDim && s->DV > 0 && s->DV <= kMaxDim, "%s: head dimensions %d, %d must be in [1, %d]", who,
                  s->D, s->DV, kMaxDim);
-    SAMX_REQUIRE(s->B <= 65535 && s->B * s->H <= 65535, "%s: B %lld times H %d is more than 65535", who, (long long)s->B, s->H);
+    SAMX_REQUIRE(s->B <= kMaxHeads && s->B * s->H <= kMaxHeads, "%s: B %lld times H %d is more than %lld", who, (long long)s->B, s->H,
+                 (long long)kMaxHeads);
     return SAMX_OK;
 }
 
