@@ -284,12 +284,32 @@ __global__ __launch_bounds__(1024) void wide_kernel(Args a) {
     finish<T, G, GRAD>(a, te, o, r, s[0], s[1], w, cq, cp, row, lane, true, on, shd, turnd);
 }
 
-template <typename T, int G, int NV, bool GRAD>
-int launch_row(const Args& a, hipStream_t st) {
-    constexpr int B = G < 256 ? 256 : G, R = B / G;
-    row_kernel<T, G, NV, GRAD><<<(unsigned)((a.N + R - 1) / R), B, R * row_lds(a.K), st>>>(a);
-    SAMX_LAUNCH_CHECK();
+// The rows in launches of at most 2^31 threads, G for each row.  (Beyond 2^32 a launch reports nothing and leaves rows out.)
+template <typename T, int G, typename Go>
+int in_launches(const Args& all, Go go) {
+    constexpr int64_t kMost = (int64_t(1) << 31) / G;
+    for (int64_t at = 0; at < all.N; at += kMost) {
+        Args a = all;
+        a.N = all.N - at < kMost ? all.N - at : kMost;
+        a.z = (const T*)all.z + at * all.ld;
+        a.idx = all.idx + at * all.K;
+        a.teacher = all.teacher + at * all.K;
+        if (all.lse) a.lse = all.lse + at;
+        if (all.weight) a.weight = all.weight + at;
+        a.loss = all.loss + at;
+        if (all.grad) a.grad = (T*)all.grad + at * all.ldg;
+        go(a);
+        SAMX_LAUNCH_CHECK();
+    }
     return SAMX_OK;
+}
+
+template <typename T, int G, int NV, bool GRAD>
+int launch_row(const Args& all, hipStream_t st) {
+    constexpr int B = G < 256 ? 256 : G, R = B / G;
+    return in_launches<T, G>(all, [&](const Args& a) {
+        row_kernel<T, G, NV, GRAD><<<(unsigned)((a.N + R - 1) / R), B, R * row_lds(a.K), st>>>(a);
+    });
 }
 
 template <typename T, bool GRAD>
@@ -308,9 +328,7 @@ int launch(const Args& a, hipStream_t st) {
     // bf16: loss 286 -> 226 us, gradient 550 -> 519; 4096 x 64000 float32: loss 233 -> 183, gradient 453 against 485.
     if constexpr (GRAD && sizeof(T) == 4)
         if (n <= 16384) return launch_row<T, 1024, 16, GRAD>(a, st);
-    wide_kernel<T, GRAD><<<(unsigned)a.N, 1024, row_lds(a.K), st>>>(a);
-    SAMX_LAUNCH_CHECK();
-    return SAMX_OK;
+    return in_launches<T, 1024>(a, [&](const Args& p) { wide_kernel<T, GRAD><<<(unsigned)p.N, 1024, row_lds(p.K), st>>>(p); });
 }
 
 int distill(const char* who, const void* logits, int64_t ld, int dtype, int64_t N, int64_t V, const int32_t* idx,

@@ -30,3 +30,26 @@ def test_step_of_65536_heads(dtype):
 
 def test_sequences_of_131072_heads():
     _check(_case(4096, 2, 32, 16, 4, 4, BF16, seed=42, lengths=[(b + 2) % 3 for b in range(4096)]), 0.5, BF16)
+
+
+def test_distillation_of_more_rows_than_a_launch_takes():
+    """2^26 rows and some of 64 threads each.  Exponents' arguments have two roundings relative to at most 12, sums a few more:
+    64 U32 of a probability, of a logarithm absolute."""
+    from sam_tf_amd import ops
+    N, V = 2 ** 26 + 7, 2
+    g = torch.Generator(device='cuda').manual_seed(43)
+    z = torch.randn(N, V, device='cuda', generator=g)
+    idx = torch.randint(0, V, (N, 1), device='cuda', generator=g, dtype=torch.int32)
+    teacher = torch.zeros(N, 1, device='cuda')
+    weight = torch.rand(N, device='cuda', generator=g)
+    loss, grad = ops.distill_grad(z, idx, teacher, weight=weight, scale=0.5)
+    alone = ops.distill_loss(z, idx, teacher, weight=weight)
+    for a in range(0, N, 2 ** 24):
+        s = slice(a, a + 2 ** 24)
+        q = torch.log_softmax(z[s].double(), 1)
+        w, i = weight[s].double(), idx[s].long()
+        want = -w * q.gather(1, i)[:, 0]
+        for x in (loss, alone):
+            assert float(((x[s].double() - want).abs() / (w * (1 + want.abs()) + 1e-30)).max()) < 64 * U32
+        dense = q.exp().scatter_add(1, i, -torch.ones_like(q[:, :1]))
+        assert float((grad[s].double() - 0.5 * w[:, None] * dense).abs().max()) < 64 * U32
