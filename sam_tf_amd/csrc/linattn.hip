@@ -772,13 +772,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
 // sums of the query heads that share a key head: float32 [rows, HK, grp, dim] -> [rows, HK, dim] of the type
 template <typename T>
 __global__ __launch_bounds__(256) void group_kernel(const float* __restrict__ in, T* __restrict__ out, int64_t n, int grp, int dim) {
-    const int64_t e = blockIdx.x * (int64_t)256 + threadIdx.x;
-    if (e >= n) return;
-    const int64_t row = e / dim, d = e % dim;
-    const float* p = in + row * grp * dim + d;
-    float v = 0.f;
-    for (int k = 0; k < grp; ++k) v += p[(int64_t)k * dim];
-    out[e] = from_float<T>(v);
+    for (int64_t e = blockIdx.x * (int64_t)256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256) {
+        const int64_t row = e / dim, d = e % dim;
+        const float* p = in + row * grp * dim + d;
+        float v = 0.f;
+        for (int k = 0; k < grp; ++k) v += p[(int64_t)k * dim];
+        out[e] = from_float<T>(v);
+    }
 }
 
 // One row: S <- l S + k v^T, out = c q^T S, in place.  A workgroup has a head's state (four columns for each of cols / 4
@@ -1017,7 +1017,8 @@ int samx_linattn_grad(const samx_linattn_shape* s, const void* q, const void* k,
             const int64_t n = rows * s->HK * dim;
             const float* in = i ? dv_h : dk_h;
             void* out = i ? dv : dk;
-            const unsigned g = (unsigned)((n + 255) / 256);
+            const int64_t want = (n + 255) / 256, most = int64_t(1) << 23;      // (a launch of 2^32 threads leaves some out)
+            const unsigned g = (unsigned)(want < most ? want : most);
             if (s->dtype == kF32) group_kernel<float><<<g, 256, 0, st>>>(in, (float*)out, n, rep, dim);
             else if (s->dtype == kBF16) group_kernel<bf16><<<g, 256, 0, st>>>(in, (bf16*)out, n, rep, dim);
             else group_kernel<f16><<<g, 256, 0, st>>>(in, (f16*)out, n, rep, dim);

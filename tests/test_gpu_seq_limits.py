@@ -53,3 +53,29 @@ def test_distillation_of_more_rows_than_a_launch_takes():
             assert float(((x[s].double() - want).abs() / (w * (1 + want.abs()) + 1e-30)).max()) < 64 * U32
         dense = q.exp().scatter_add(1, i, -torch.ones_like(q[:, :1]))
         assert float((grad[s].double() - 0.5 * w[:, None] * dense).abs().max()) < 64 * U32
+
+
+def test_shared_heads_gradient_of_more_elements_than_a_launch_takes():
+    """2^32 elements and some of dk.  All rows alike (one row, stride 0): the gradient's state is a geometric sum, and both
+    gradients are known."""
+    from sam_tf_amd import ops
+    H, D, DV, T, scale = 2, 128, 8, 2 ** 25 + 3, 0.25
+    c = _case(1, 1, H, 1, D, DV, BF16, seed=44, state=False, decay=[-1.0, -2.0])
+    row = {n: c[n].double()[0, 0] for n in ('q', 'k', 'v', 'dout')}
+    g = _gpu(c)
+    q, k, v, o = (g[n].expand(1, T, -1, -1) for n in ('q', 'k', 'v', 'dout'))
+    got = ops.linattn_grad(q, k, v, g['decay'], o, scale=scale)
+    left = T - torch.arange(T - 64, T, dtype=torch.float64)                # rows from each of the last 64 on to the end
+    lam = torch.exp(c['decay'].double())
+    many = scale * (1 - lam ** left[:, None]) / (1 - lam)                  # [64, H]
+    b = lambda t: t.abs()
+    f = lambda q, o, k, v: (((o * v).sum(-1)[:, None] * q * many[..., None]).sum(1), ((q * k).sum(-1)[:, None] * o * many[..., None]).sum(1))
+    want, size = f(row['q'], row['dout'], row['k'], row['v']), f(b(row['q']), b(row['dout']), b(row['k']), b(row['v']))
+    h = half_step(BF16)
+    for x, w, m in zip(got[1:3], want, size):
+        x = x[0, :, 0]
+        tol = (3.2 * h + 300 * U32) * m
+        within(x[-64:], w, tol)
+        far, most = w[0].cuda(), tol[0].cuda()
+        for a in range(0, T - 64, 2 ** 22):
+            assert bool(((x[a:min(T - 64, a + 2 ** 22)].double() - far).abs() <= most).all()), a
