@@ -702,7 +702,7 @@ int samx_linattn_step(const samx_linattn_shape* s, const void* q, const void* k,
  *   p_k = e^{t_k / tau - lse}   (lse float32 [N]: the teacher's own log-normaliser at tau; NULL: over the K entries)
  *   loss = w sum_k p_k (log p_k - log softmax(z / tau)[idx_k])          float32 [N]; w = weight[row], NULL: 1
  * samx_distill_grad also writes the gradient of scale * sum(loss) to grad (element type, rows ld_grad apart; columns behind
- * V stay as they were; grad may be the logits' own buffer with their stride).
+ * V stay as they were; grad may be the logits' own buffer with their stride; no output overlaps another input).
  * Entries with an index outside [0, V) do not count (a row may know fewer than K); an index that stands twice counts twice.
  * A row of weight 0 has loss 0 and gradient 0 whatever its logits hold.  Logits of -inf have probability 0; a row of nothing
  * else has q = 0 (loss +inf where the teacher has any mass). */

@@ -1152,18 +1152,21 @@ def _distill_args(logits, idx, teacher, lse, weight, loss):
     if not (isinstance(idx, torch.Tensor) and idx.dim() == 2):
         raise ValueError('idx must be [rows, K]')
     K = idx.shape[1]
-    if loss is None:
+    given = loss is not None
+    if not given:
         loss = torch.empty(N, dtype=F32, device=dev)
-    return (dev, ld, N, V, K, loss, (logits.data_ptr(), ld, code, N, V, _on(idx, dev, I32, (N, K), 'idx'),
-                                     _on(teacher, dev, F32, (N, K), 'teacher'), K),
+    args = ((logits.data_ptr(), ld, code, N, V, _on(idx, dev, I32, (N, K), 'idx'), _on(teacher, dev, F32, (N, K), 'teacher'), K),
             _opt_on(lse, dev, F32, (N,), 'lse'), _opt_on(weight, dev, F32, (N,), 'weight'), _on(loss, dev, F32, (N,), 'loss'))
+    if given:
+        _clear(loss, 'loss', (), (('logits', logits), ('idx', idx), ('teacher', teacher), ('lse', lse), ('weight', weight)))
+    return (dev, ld, N, V, K, loss) + args
 
 
 def distill_loss(logits, idx, teacher, tau=1.0, lse=None, weight=None, loss=None):
     """Imitation of a teacher's top logits: loss float32 [rows], weight * sum_k p_k (log p_k - log softmax(logits /
     tau)[idx_k]) with p_k = exp(teacher_k / tau - lse) (lse None: normalised over the K entries).  logits [rows, V] in
     float32, bfloat16 or float16, rows may be apart; idx int32 [rows, K] (entries outside [0, V) do not count), teacher
-    float32 [rows, K]; lse, weight float32 [rows] (samx_distill_loss)."""
+    float32 [rows, K]; lse, weight float32 [rows].  A loss that is given overlaps no input (samx_distill_loss)."""
     dev, _, _, _, _, loss, a, pn, pw, pl = _distill_args(logits, idx, teacher, lse, weight, loss)
     check(_L().samx_distill_loss(*a, tau, pn, pw, pl, _raw_stream(dev.index)))
     return loss
@@ -1171,8 +1174,8 @@ def distill_loss(logits, idx, teacher, tau=1.0, lse=None, weight=None, loss=None
 
 def distill_grad(logits, idx, teacher, tau=1.0, lse=None, weight=None, scale=1.0, loss=None, grad=None):
     """distill_loss and the gradient of scale * its sum: (loss, grad).  grad has the logits' type and shape (and a row
-    stride up to 255 columns wider than V); it may be given, the logits themselves among them; columns behind V stay as
-    they were (samx_distill_grad)."""
+    stride up to 255 columns wider than V); it may be given, the logits themselves among them (it overlaps nothing
+    else); columns behind V stay as they were (samx_distill_grad)."""
     dev, ld, N, V, K, loss, a, pn, pw, pl = _distill_args(logits, idx, teacher, lse, weight, loss)
     if grad is None:
         ldg = ld if V <= ld < V + 256 else V
@@ -1184,5 +1187,6 @@ def distill_grad(logits, idx, teacher, tau=1.0, lse=None, weight=None, scale=1.0
         x, y, e = logits.data_ptr(), grad.data_ptr(), logits.element_size()
         if x != y and N and x < y + ((N - 1) * ldg + V) * e and y < x + ((N - 1) * ld + V) * e:
             raise ValueError('grad overlaps the logits without being them')
+        _clear(grad, 'grad', (), (('idx', idx), ('teacher', teacher), ('lse', lse), ('weight', weight), ('loss', loss)))
     check(_L().samx_distill_grad(*a, tau, pn, pw, scale, pl, grad.data_ptr(), ldg, _raw_stream(dev.index)))
     return loss, grad
