@@ -119,8 +119,8 @@ int samx_per_leaves_from_td(const float* td, const int64_t* idxs, int64_t n, int
  * comes out of memory that the first eager call of any of them sets aside: make one before the first capture.
  * samx_pow_device_f32_range / samx_pow_host_f32_range: the same for the n float32 values whose bit patterns
  * start at first_bits, widened to double, + bonus (device result in HBM / libm result in host memory).
- * samx_pow_selfcheck(n): HOST — the number of n pseudo-random cases in which that host function differs from this
- * machine's pow (0). */
+ * samx_pow_host(x, y, n, out): HOST — that host function itself.  samx_pow_selfcheck(n): HOST — the number of n
+ * pseudo-random cases in which it is more than a step of the last place from the long double pow (0). */
 int samx_pow_device(const double* x, double y, int64_t n, double* out, void* stream);
 int samx_pow_device_f32_range(uint32_t first_bits, int64_t n, double bonus, double y, double* out, void* stream);
 int samx_pow_host_f32_range(uint32_t first_bits, int64_t n, double bonus, double y, double* out_host);

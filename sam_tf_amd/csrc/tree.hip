@@ -426,13 +426,14 @@ int samx_pow_host_f32_range(uint32_t first_bits, int64_t n, double bonus, double
 
 int samx_pow_host(const double* x_host, double y, int64_t n, double* out_host) {
     SAMX_REQUIRE(x_host && out_host && n > 0, "samx_pow_host: bad arguments");
-    for (int64_t i = 0; i < n; ++i) out_host[i] = pow(x_host[i], y);
+    memmove(out_host, x_host, (size_t)n * sizeof(double));
+    samx::host_pow_values(out_host, n, y);
     return SAMX_OK;
 }
 
 int64_t samx_pow_selfcheck(int64_t n) {
-    // the host function that the device entry points put on the stream against pow called here, on n pseudo-random
-    // bases and the usual exponents
+    // the host function that the device entry points put on the stream against the long double pow, on n pseudo-random
+    // bases and the usual exponents: off by more than a step of the last place where this process has no sound pow
     uint64_t s = 0x9E3779B97F4A7C15ull;
     int64_t bad = 0;
     const double ys[4] = {0.3, 0.6, -0.4, -1.0};
@@ -444,8 +445,8 @@ int64_t samx_pow_selfcheck(int64_t n) {
         memcpy(&x, &u, 8);
         a = x;
         samx::host_pow_values(&a, 1, ys[i & 3]);
-        const double b = pow(x, ys[i & 3]);
-        if (memcmp(&a, &b, 8) != 0) ++bad;
+        const long double want = powl((long double)x, (long double)ys[i & 3]);
+        if (!(fabsl((long double)a - want) <= (long double)(nextafter(a, INFINITY) - a))) ++bad;
     }
     return bad;
 }

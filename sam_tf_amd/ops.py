@@ -120,11 +120,21 @@ _POW_OK = None
 
 
 def pow_matches_host(n=200000):
-    """True when the host function that the library puts on a stream gives THIS machine's libm pow on n cases
-    (samx_pow_selfcheck)."""
+    """True when the function that the library puts on a stream is this machine's pow: sound at all (samx_pow_selfcheck), and
+    bit for bit the interpreter's `**` on n cases, which is what the reference computes with (a library can have been bound to
+    another libm than the interpreter's)."""
     global _POW_OK
     if _POW_OK is None:
-        _POW_OK = int(_L().samx_pow_selfcheck(int(n))) == 0
+        L, n = _L(), int(n)
+        rs = np.random.RandomState(1)
+        ok = int(L.samx_pow_selfcheck(n)) == 0
+        for y in (0.3, 0.6, -0.4, -1.0):      # priority ** alpha, weights of -beta
+            x = np.ldexp(rs.uniform(1.0, 2.0, n // 4), rs.randint(-30, 31, n // 4))
+            got = np.empty_like(x)
+            check(L.samx_pow_host(x.ctypes.data, y, x.size, got.ctypes.data))
+            want = np.array([v ** y for v in x.tolist()])
+            ok = ok and bool((got.view(np.uint64) == want.view(np.uint64)).all())
+        _POW_OK = ok
     return _POW_OK
 
 
