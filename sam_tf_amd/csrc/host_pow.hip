@@ -48,8 +48,11 @@ int capturing(hipStream_t st, bool* yes) {
     return SAMX_OK;
 }
 
+// (*x stays as it was where there is no memory: what is left of a chunk goes on being given out)
 int pinned(int64_t n, double** x) {
-    SAMX_CHECK_HIP(hipHostMalloc((void**)x, (size_t)n * sizeof(double), hipHostMallocPortable));
+    void* got = nullptr;
+    SAMX_CHECK_HIP(hipHostMalloc(&got, (size_t)n * sizeof(double), hipHostMallocPortable));
+    *x = (double*)got;
     return SAMX_OK;
 }
 
