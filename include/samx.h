@@ -673,10 +673,10 @@ int samx_block_norm_grad(const void* y, const void* h, const void* dh, const voi
  * strides (in elements: batch, row, head) as given; decay float32 [H], the logarithm of the factor (<= 0, -inf: no memory);
  * state float32 [B, H, D, DV] dense, state_in NULL: zero.  lengths int32 [B] (NULL: T): rows of each sequence that are there
  * (taken into [0, T]); rows behind them are not read, their outputs are zeros, the state behind a sequence is that of its
- * last row.  out, dq, dk, dv are dense; no output overlaps an input.  Scores and the state are float32; products of 16-bit
- * types take the scores and, for out, a copy of the state rounded to their own type, half a step each beside the output's own
- * (float16: as fractions of a power of two, so that neither has to be within its range).  An infinity or a NaN of a row
- * reaches what the recurrence takes it to and nothing else; behind it an infinity may have become a NaN. */
+ * last row.  out, dq, dk, dv are dense; no output overlaps an input.  Scores and the state are float32 whatever the type
+ * (products of 16-bit types take each as two numbers of the type, of float16 as fractions of a power of two, so that none has
+ * to be within its range); an output is rounded once.  An infinity or a NaN of a row reaches what the recurrence takes it to
+ * and nothing else; behind it an infinity may have become a NaN. */
 typedef struct samx_linattn_shape {
     int32_t dtype, H, HK, D, DV, pad;
     int64_t B, T;

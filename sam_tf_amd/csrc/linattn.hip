@@ -15,21 +15,22 @@
 //
 // A chunk of 64 positions at a time, on the matrix cores: scores P = a b^T masked with l^{p-s}, out = P c + l^p a X,
 // X <- l^64 X + sum_s l^{64-s} b_s c_s^T.  X stays in the registers of the workgroup (float32; each wave owns whole
-// columns).  Operands of 16 bits enter the matrix cores as they are; P and the copy of X that meets a are rounded to
-// their type (an output of that type is rounded again), but l^{64-s} c_s is split into numbers of the type whose sum it is,
-// so that the state, a float32 output, is one.  float16, which has too few exponents for any of these, takes each as a
-// fraction of a power of two (Scale).  float32 operands use the float32 matrix instructions throughout.
+// columns, and their part of out: the tiles it holds are operands of the product with a as they stand).  Operands of 16 bits
+// enter the matrix cores as they are; P and X enter as two numbers of their type each, so that an output of 16 bits is rounded
+// by half a step once (as one number each its error was 1.4 times that), and l^{64-s} c_s as the numbers of the type whose sum
+// it is, so that the state, a float32 output, is one.  float16, which has too few exponents for any of these, takes each as
+// fractions of a power of two (Scale).  float32 operands use the float32 matrix instructions throughout.
 //
 // Where batch times heads is less than the device holds, time is cut into segments: kv_kernel makes each segment's own
 // contribution to the state behind it, join_kernel runs the recurrence over the segments, mix_kernel does the rest with
 // a known state at each segment's start.
 //
-// Measured, 16 heads of 128, bf16.  32 x 1024 rows (two workgroups for each compute unit, no segments): 155 us, 3900 GB/s of
-// 4750 that a large copy reaches.  2 x 4096 rows: 81 us in 8 segments (kv 23, join 9, mix 45), the keys and values read
-// twice.  Gradient of 4 x 2048 ragged rows: 111 us, two workgroups for each head's columns (of one for all of them a chunk
-// took 4.6 us: the state's update 1.2, the stores 0.7, waiting for loads 0.6, the other products' chain the rest).
+// Measured, 16 heads of 128, bf16.  32 x 1024 rows (two workgroups for each compute unit, no segments): 165 us, 3650 GB/s of
+// 4750 that a large copy reaches.  2 x 4096 rows: 84 us in 8 segments (alone: kv 24, join 8, mix 54), the keys and values read
+// twice.  Gradient of 4 x 2048 ragged rows: 131 us, two workgroups for each head's columns.  (P and X as one number each: 150,
+// 78 and 111 us; X passed on through LDS as two: 190, 82 and 128, gradient of 32 x 1024 rows 519 against 432.)
 // float32: its matrix instructions have a sixteenth of the rate, and its tiles leave LDS for one workgroup a unit
-// (2 x 4096 rows 205 us).
+// (2 x 4096 rows 210 us).
 #include "seq_dev.h"
 #include "../../include/samx.h"
 #include <type_traits>
@@ -142,15 +143,6 @@ struct Rows {
         p = (const SAMX_GLOBAL char*)m.p + (int64_t)sizeof(T) * (q.b * m.sb + (int64_t)(q.h / m.grp) * m.sh + from + (rev ? (q.L - 1) * m.st : 0));
         step = (int64_t)sizeof(T) * (rev ? -m.st : m.st);
     }
-    __device__ __forceinline__ float value(int64_t pos, int i) const {
-        T v;
-        if constexpr (sizeof(T) == 4) v = *(const SAMX_GLOBAL float*)(p + pos * step + i * 4);
-        else {
-            const uint16_t u = *(const SAMX_GLOBAL uint16_t*)(p + pos * step + i * 2);
-            __builtin_memcpy(&v, &u, 2);
-        }
-        return to_float(v);
-    }
     // elements [at, at + kN) of position base + pos.  What lies behind the chunk's n positions or behind the row's end is
     // not what comes here: the caller does not use it.
     __device__ __forceinline__ Piece<T> piece(int64_t base, int pos, int at, int n) const {
@@ -199,10 +191,17 @@ __device__ __forceinline__ void lds_put(T* p, const Piece<T>& r) {
     __builtin_memcpy(&v, &r, 16);
     *reinterpret_cast<u32x4*>(p) = v;
 }
-__device__ __forceinline__ void lds_put4(float* p, const float (&v)[4]) { *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]}; }
+// 4 values, rounded; v: what of them that leaves
+__device__ __forceinline__ void put_part(float* p, float (&v)[4]) { *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]}; }
 template <typename T>
-__device__ __forceinline__ void lds_put4(T* p, const float (&v)[4]) {
-    *reinterpret_cast<u32x2*>(p) = u32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+__device__ __forceinline__ void put_part(T* p, float (&v)[4]) {
+    const u32x2 x = {pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+    *reinterpret_cast<u32x2*>(p) = x;
+    Piece<T> r;
+    r.w[0] = x[0];
+    r.w[1] = x[1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] -= r.f(e);
 }
 // A piece down a column: elements [0, kN) are rows[e][lane % 16].  16 bits: two transposing reads, in each of which 16
 // lanes read 4 rows of 16 values and get a column each; with 4-byte values a read for each row.
@@ -223,18 +222,12 @@ __device__ __forceinline__ Piece<T> lds_column(const T* rows, int stride) {
     }
     return r;
 }
-// what the lanes of a wave have written to LDS is there for the others of the wave
-__device__ __forceinline__ void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
 
 // float16: values that are to be rounded to it, or split into parts of it, are first taken to a power of two's fractions, so
 // that the largest of those that share it stands in [2^14, 2^15): none overflows, and what is below 2^-39 of the largest is all
 // that is lost.  One power for each column of c and of X and one for each row of P: lanes of one l % 16.  (Without it a value
 // of the state beyond 65504 was an infinity to its rows, and the state of values around 1e-5 had a few per cent of error.)
-// It costs: 32 x 1024 rows, 16 heads of 128, 180 us where bfloat16 takes 146; the gradient of 4 x 2048 rows 161, not 134.
+// It costs: 32 x 1024 rows, 16 heads of 128, 204 us where bfloat16 takes 163; the gradient of 4 x 2048 rows 188, not 167.
 template <typename T> constexpr bool kScaled = std::is_same<T, f16>::value;
 struct Scale { float up, down; };              // the power and one over it
 // of values whose magnitudes are at most `most` (in this lane); none below 2^(least - 127 - 14)
@@ -249,6 +242,9 @@ __device__ __forceinline__ Scale scale_of(float most, uint32_t least = 15) {
     return {__uint_as_float((e - 14u) << 23), __uint_as_float((268u - e) << 23)};
 }
 
+// numbers that a score and a value of X are as they enter a product: two of 16 bits, the second what the first has left
+template <typename T> constexpr int kHalves = sizeof(T) == 2 ? 2 : 1;
+
 // LDS rows are 16 bytes longer than their contents: 16 lanes that read 16 rows at one column use all banks
 template <typename T, int DP, int DC>
 struct LdsKv {
@@ -261,9 +257,9 @@ template <typename T, int DP, int DC>
 struct Lds : LdsKv<T, DP, DC> {
     static constexpr int kTok = kChunk + Piece<T>::kN;
     static_assert(sizeof(LdsKv<T, DP, DC>) % 16 == 0, "pieces are read whole");
-    T p[4][16][kTok];                                    // each wave's 16 rows of scores
-    T x[DC][LdsKv<T, DP, DC>::kRow];                     // X, a row for each column
-    float xs[kScaled<T> ? DC : 4];                       // the power of two of each of these rows
+    T a[kChunk][LdsKv<T, DP, DC>::kRow];
+    T p[kHalves<T>][kChunk][kTok];                       // scores
+    float ps[kScaled<T> ? kChunk : 4], xs[kScaled<T> ? DC : 4];   // the powers of two of P's rows and X's columns
 };
 
 // N groups of products, group g's operands read (into buf[g % (AHEAD + 1)]) AHEAD groups before they are used; nothing is
@@ -292,23 +288,36 @@ __device__ __forceinline__ uint32_t odd_bits(uint32_t w) {
     return ((w & e) + one) & (sizeof(T) == 4 ? 0x80000000u : 0x80008000u);
 }
 
-// A chunk's rows of b and c on their way to LDS
-template <typename T, int DP, int DC>
+// A chunk's rows of b and c, and of a as A says, on their way to LDS.  kByRow: each lane has pieces of one row of a, so that a row
+// that is not whole pieces costs a lane one piece that waits for its elements, not four (100 of 128 dimensions, bfloat16,
+// gradient of 4 x 2048 rows, 4 key heads: 350 us against 398); whole pieces do better side by side (4 x 2048 rows of 128: 167
+// against 171; float32 519 against 568).
+enum StageA { kNoA, kSideBySide, kByRow };
+template <typename T, int DP, int DC, StageA A>
 struct Staged {
     static constexpr int kN = Piece<T>::kN;
     static constexpr int kAcross = DP / kN, kDown = kThreads / kAcross, kPer = kChunk / kDown;
     static constexpr int kAcrossC = DC / kN, kDownC = kThreads / kAcrossC, kPerC = kChunk / kDownC;
-    Piece<T> b[kPer], c[kPerC];
+    Piece<T> a[A == kNoA ? 1 : kPer], b[kPer], c[kPerC];
+    static __device__ __forceinline__ int a_row(int u) {
+        return A == kByRow ? threadIdx.x / 64 * 16 + threadIdx.x % 16 : threadIdx.x / kAcross + u * kDown;
+    }
+    static __device__ __forceinline__ int a_col(int u) {
+        return (A == kByRow ? u * 4 + threadIdx.x % 64 / 16 : threadIdx.x % kAcross) * kN;
+    }
     template <bool EVEN>
-    __device__ __forceinline__ void load(const Rows<T, EVEN>& mb, const Rows<T, EVEN>& mc, int64_t base, int n) {
+    __device__ __forceinline__ void load(const Rows<T, EVEN>& ma, const Rows<T, EVEN>& mb, const Rows<T, EVEN>& mc, int64_t base, int n) {
         const int t = threadIdx.x / kAcross, d = threadIdx.x % kAcross * kN;
         const int tc = threadIdx.x / kAcrossC, e = threadIdx.x % kAcrossC * kN;
+        if constexpr (A != kNoA)
+#pragma unroll
+            for (int u = 0; u < kPer; ++u) a[u] = ma.piece(base, a_row(u), a_col(u), n);
 #pragma unroll
         for (int u = 0; u < kPer; ++u) b[u] = mb.piece(base, t + u * kDown, d, n);
 #pragma unroll
         for (int u = 0; u < kPerC; ++u) c[u] = mc.piece(base, tc + u * kDownC, e, n);
     }
-    // zeros behind the rows' ends and behind the n positions
+    // zeros behind the rows' ends and behind the n positions (a and b are as wide)
     template <typename L>
     __device__ __forceinline__ uint32_t store(L& l, int db, int dc, int n) const {
         const int t = threadIdx.x / kAcross, d = threadIdx.x % kAcross * kN;
@@ -316,13 +325,16 @@ struct Staged {
         uint32_t odd = 0;                 // whether c has something that is not finite
 #pragma unroll
         for (int u = 0; u < kPer; ++u) {
+            const uint32_t ka = a_col(u) < db && a_row(u) < n ? ~0u : 0u;
             const uint32_t kb = d < db && t + u * kDown < n ? ~0u : 0u, kc = e < dc && tc + u * kDownC < n ? ~0u : 0u;
-            Piece<T> x, y;
+            Piece<T> w, x, y;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
+                if constexpr (A != kNoA) w.w[j] = a[u].w[j] & ka;
                 x.w[j] = b[u].w[j] & kb;
                 if (u < kPerC) { y.w[j] = c[u].w[j] & kc; odd |= odd_bits<T>(y.w[j]); }
             }
+            if constexpr (A != kNoA) lds_put(&l.a[a_row(u)][a_col(u)], w);
             lds_put(&l.b[t + u * kDown][d], x);
             if (u < kPerC) lds_put(&l.c[tc + u * kDownC][e], y);
         }
@@ -343,6 +355,34 @@ struct State {
             for (int i = 0; i < kI; ++i) x[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 };
+
+// Tile column j of X as it enters a product with a, inner values of mma m: the lane's own registers.  16 bits: the tiles 2m and
+// 2m + 1, an order of the inner values that a_piece has too, rounded (X half 0) and what of it that leaves (half 1).
+template <typename T, int DP, int DC>
+__device__ __forceinline__ void x_pieces(const State<DP, DC>& S, int j, int m, float down, Piece<T> (&x)[kHalves<T>]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[0].w[e] = __float_as_uint(S.x[j][m][e]);
+    } else {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = kScaled<T> ? S.x[j][2 * m + e / 4][e % 4] * down : S.x[j][2 * m + e / 4][e % 4];
+        x[0] = pack<T>(v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] -= x[0].f(e);
+        x[1] = pack<T>(v);
+    }
+}
+template <typename T>
+__device__ __forceinline__ Piece<T> a_piece(const T* row, int m, int q) {
+    if constexpr (sizeof(T) == 4) return lds_piece(row + m * 16 + q * 4);
+    else {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(row + m * 32 + q * 4), y = *reinterpret_cast<const u32x2*>(row + m * 32 + 16 + q * 4);
+        Piece<T> r;
+        r.w[0] = x[0]; r.w[1] = x[1]; r.w[2] = y[0]; r.w[3] = y[1];
+        return r;
+    }
+}
 
 // numbers of the type whose sum a float32 is
 template <typename T> constexpr int kParts = 1;
@@ -490,13 +530,13 @@ __global__ __launch_bounds__(kThreads, 2) void kv_kernel(Args A) {
     if (threadIdx.x <= 2 * kChunk) l.lam[threadIdx.x] = threadIdx.x < kChunk ? 0.f : power(p.g, threadIdx.x - kChunk);
     State<DP, DP> S;
     S.zero();
-    Staged<T, DP, DP> st;
-    st.load(b, c, at, kChunk);
+    Staged<T, DP, DP, kNoA> st;
+    st.load(b, b, c, at, kChunk);
     for (int64_t k = 0; k < A.seg_len; k += kChunk) {
         __syncthreads();
         st.store(l, r.b.dim, r.c.dim, kChunk);
         __syncthreads();
-        if (k + kChunk < A.seg_len) st.load(b, c, at + k + kChunk, kChunk);
+        if (k + kChunk < A.seg_len) st.load(b, b, c, at + k + kChunk, kChunk);
         update<T, DP, DP>(S, l, kChunk, r.kv);
     }
     seg_store<DP, DP>(S, (SAMX_GLOBAL float*)r.seg + ((int64_t)(p.b * A.H + p.h) * (A.nseg - 1) + p.seg) * A.seg_size);
@@ -542,9 +582,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
     if (!place_of(A, A.nseg, p)) return;
     // (by value: a reference into the arguments makes the compiler keep a copy of all of them in scratch memory)
     const Role r = A.r[p.role];
-    // wave w: columns of a state; of a chunk, rows 16 w + [0, 16) of out
+    // wave w: tiles w, w + kWaves of the columns, of the state and of out; of a chunk's scores, rows 16 w + [0, 16)
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, q = lane >> 4;
-    constexpr int kTiles = DC / 16;
     const int64_t at = (int64_t)p.seg * A.seg_len, bh = (int64_t)p.b * A.H + p.h;
     const int64_t to = at + A.seg_len < p.L ? at + A.seg_len : p.L;         // this segment's positions
     constexpr bool kShare = DC < DP;       // a workgroup has DC of the columns
@@ -554,16 +593,16 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
     const int64_t out_row = (int64_t)A.H * all;
     const int64_t out_at = ((int64_t)p.b * A.T * A.H + p.h) * all + c0;
     SAMX_GLOBAL char* const outp = (SAMX_GLOBAL char*)r.out + out_at * (r.out_f32 ? 4 : (int)sizeof(T));
-    // four of a row's outputs from d on, those that exist
-    auto put4 = [=](auto f32, int64_t row, int d, f32x4 v) {
+    // four of a row's outputs from d on, those that exist; el: elements from the first row to it
+    auto put4 = [=](auto f32, int64_t el, int d, f32x4 v) {
         if constexpr (decltype(f32)::value) {
-            SAMX_GLOBAL float* o = (SAMX_GLOBAL float*)outp + row * out_row + d;
+            SAMX_GLOBAL float* o = (SAMX_GLOBAL float*)outp + el + d;
             if (EVEN) { if (d < dc) *(SAMX_GLOBAL f32x4_any*)o = v; return; }
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (d + e < dc) o[e] = v[e];
         } else if constexpr (sizeof(T) == 2) {
-            SAMX_GLOBAL uint16_t* o = (SAMX_GLOBAL uint16_t*)outp + row * out_row + d;
+            SAMX_GLOBAL uint16_t* o = (SAMX_GLOBAL uint16_t*)outp + el + d;
             const uint32_t lo = pack2<T>(v[0], v[1]), hi = pack2<T>(v[2], v[3]);
             if (EVEN) { if (d < dc) *(SAMX_GLOBAL u32x2_any*)o = u32x2{lo, hi}; return; }
             if (d < dc) o[0] = (uint16_t)lo;
@@ -577,8 +616,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
         const int64_t z0 = at > p.L ? at : p.L, z1 = at + A.seg_len < A.T ? at + A.seg_len : A.T;
         for (int64_t t = z0 + w; t < z1; t += kWaves)
             for (int d = lane * 4; d < dc; d += 256) {
-                if (wide) put4(std::true_type(), t, d, f32x4{0.f, 0.f, 0.f, 0.f});
-                else put4(std::false_type(), t, d, f32x4{0.f, 0.f, 0.f, 0.f});
+                if (wide) put4(std::true_type(), t * out_row, d, f32x4{0.f, 0.f, 0.f, 0.f});
+                else put4(std::false_type(), t * out_row, d, f32x4{0.f, 0.f, 0.f, 0.f});
             }
     }
     State<DP, DC> S;
@@ -594,18 +633,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
     }
     if (at >= to) return;
     const Rows<T, EVEN> a(r.a, p, r.rev), b(r.b, p, r.rev), c(r.c, p, r.rev, c0);
-    const int row = w * 16 + r16;          // of a chunk: this lane's
-    Staged<T, DP, DC> st;
-    // a's rows of this wave, whole; behind their ends there is something of the row, which only meets zeros of b and X, and
-    // a row that the chunk does not have is another one, whose outputs are not written
-    Piece<T> af[kK];
+    const int row = w * 16 + r16;          // of a chunk: the one whose scores this lane makes
+    Staged<T, DP, DC, EVEN || sizeof(T) == 4 ? kSideBySide : kByRow> st;
     auto rows_at = [&](int64_t base) { return (int)(to - base < kChunk ? to - base : kChunk); };
-    auto fetch_a = [&](int64_t base) {
-#pragma unroll
-        for (int k = 0; k < kK; ++k) af[k] = a.piece(base, row, k * kInner + q * kN, rows_at(base));
-    };
-    st.load(b, c, at, rows_at(at));
-    fetch_a(at);
+    st.load(a, b, c, at, rows_at(at));
     const bool last = to == p.L;           // this segment makes the state behind the last position
     if (p.seg > 0) seg_load<DP, DC>(S, (const SAMX_GLOBAL float*)r.seg + (bh * (A.nseg - 1) + p.seg - 1) * A.seg_size +
                                            (r.turned ? c0 : c0 * DP), r.turned);
@@ -614,14 +645,60 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
     if (threadIdx.x <= 2 * kChunk) l.lam[threadIdx.x] = threadIdx.x < kChunk ? 0.f : power(p.g, threadIdx.x - kChunk);
     if (threadIdx.x == 0) l.odd = 0u;
     __syncthreads();
+    constexpr int kJ = State<DP, DC>::kJ, kU = kHalves<T>;
     for (int64_t base = at; base < to; base += kChunk) {
         const int n = (int)(to - base < kChunk ? to - base : kChunk);
         const bool more = base + kChunk < to;
         const uint32_t chunk = (uint32_t)((base - at) / kChunk) + 1u;
         if (st.store(l, da, dc, n)) l.odd = chunk;
+        __syncthreads();
+        if (more) st.load(a, b, c, base + kChunk, rows_at(base + kChunk));
+        // scores, transposed: column = this lane's row, rows = positions s.  (Nothing here branches on the wave: no read
+        // would be ahead of its use across a branch.)
+        f32x4 sc[4];
 #pragma unroll
-        for (int j = 0; j < State<DP, DC>::kJ; ++j) {        // X's copy for the products with a
-            float down = 1.f;
+        for (int t = 0; t < 4; ++t) sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        {
+            Piece<T> f[3][5];
+            in_groups<kK, 2>(
+                [&](int k, int at) {
+                    f[at][4] = lds_piece(&l.a[row][k * kInner + q * kN]);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) f[at][t] = lds_piece(&l.b[t * 16 + r16][k * kInner + q * kN]);
+                },
+                [&](int k, int at) {
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) sc[t] = mma(f[at][t], f[at][4], sc[t]);
+                });
+        }
+        {
+            float v[4][4], most = 0.f;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {   // (l^d is 0 behind the row, but 0 times a NaN is none)
+                    const float x = r.ps * l.lam[kChunk + row - (t * 16 + q * 4 + e)] * sc[t][e];
+                    v[t][e] = row >= t * 16 + q * 4 + e ? x : 0.f;
+                    if constexpr (kScaled<T>) most = fmaxf(most, fabsf(v[t][e]));
+                }
+            if constexpr (kScaled<T>) {
+                // (not below 2^-54: a X is divided by it, and such scores add nothing to an output of this type)
+                const Scale s = scale_of(most, 127 - 40);
+                if (q == 0) l.ps[row] = s.up;
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[t][e] *= s.down;
+            }
+#pragma unroll
+            for (int u = 0; u < kU; ++u)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) put_part(&l.p[u][row][t * 16 + q * 4], v[t]);
+        }
+        float down[kJ];
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) {
+            down[j] = 1.f;
             if constexpr (kScaled<T>) {
                 float most = 0.f;
 #pragma unroll
@@ -629,135 +706,120 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
 #pragma unroll
                     for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(S.x[j][i][e]));
                 const Scale s = scale_of(most);
-                down = s.down;
+                down[j] = s.down;
                 if (q == 0) l.xs[(w + kWaves * j) * 16 + r16] = s.up;
             }
-#pragma unroll
-            for (int i = 0; i < State<DP, DC>::kI; ++i) {
-                float v[4] = {S.x[j][i][0], S.x[j][i][1], S.x[j][i][2], S.x[j][i][3]};
-                if constexpr (kScaled<T>)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] *= down;
-                lds_put4(&l.x[(w + kWaves * j) * 16 + r16][i * 16 + q * 4], v);
-            }
         }
-        __syncthreads();
-        if (more) st.load(b, c, base + kChunk, rows_at(base + kChunk));
-        // scores, transposed: column = this wave's row, rows = positions s.  (Nothing here branches on the wave: no read
-        // would be ahead of its use across a branch.)
-        f32x4 sc[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        // out, transposed: column = this wave's row, rows = columns of c
-        f32x4 o[kTiles];
-#pragma unroll
-        for (int j = 0; j < kTiles; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        constexpr int kFour = kTiles / 4;
-        Piece<T> f[3][4];
-        in_groups<kK * (1 + kFour), 2>(
-            [&](int g, int at) {
-                const int k = g % kK, j = (g / kK - 1) * 4;
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-                    f[at][t] = g < kK ? lds_piece(&l.b[t * 16 + r16][k * kInner + q * kN])
-                                      : lds_piece(&l.x[(j + t) * 16 + r16][k * kInner + q * kN]);
-            },
-            [&](int g, int at) {
-                const int k = g % kK, j = (g / kK - 1) * 4;
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    if (g < kK) sc[t] = mma(f[at][t], af[k], sc[t]);
-                    else o[j + t] = mma(f[at][t], af[k], o[j + t]);
-                }
-            });
-        if (more) fetch_a(base + kChunk);
-        const float decayed = r.so * l.lam[kChunk + row];
-        float lam[4][4];
+        // out, transposed, of this wave's columns: column = position t * 16 + lane % 16, rows = columns of c
+        f32x4 o[4][kJ];
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) lam[t][e] = l.lam[kChunk + row - (t * 16 + q * 4 + e)];
-        __builtin_amdgcn_sched_barrier(0);
-        if constexpr (!kScaled<T>)
+            for (int j = 0; j < kJ; ++j) o[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        {
+            Piece<T> f[2][4];
+            in_groups<kK, 1>(
+                [&](int m, int at) {
 #pragma unroll
-            for (int j = 0; j < kTiles; ++j) o[j] *= decayed;
-        Scale ps{1.f, 1.f};
-        if constexpr (kScaled<T>) {
-            float most = 0.f;
+                    for (int t = 0; t < 4; ++t) f[at][t] = a_piece(&l.a[t * 16 + r16][0], m, q);
+                },
+                [&](int m, int at) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+                    for (int j = 0; j < kJ; ++j) {
+                        Piece<T> x[kU];
+                        x_pieces<T, DP, DC>(S, j, m, down[j], x);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) most = fmaxf(most, row >= t * 16 + q * 4 + e ? fabsf(r.ps * lam[t][e] * sc[t][e]) : 0.f);
-            // (not below 2^-54: a X is divided by it, and such scores add nothing to an output of this type)
-            ps = scale_of(most, 127 - 40);
+                        for (int u = 0; u < kU; ++u)
 #pragma unroll
-            for (int j = 0; j < kTiles; ++j) {
-                const f32x4 s = *reinterpret_cast<const f32x4*>(&l.xs[j * 16 + q * 4]);
-                o[j] *= s * (decayed * ps.down);
-            }
+                            for (int t = 0; t < 4; ++t) o[t][j] = mma(x[u], f[at][t], o[t][j]);
+                    }
+                });
         }
+        __syncthreads();                   // everybody's scores are there
+        // of position t * 16 + lane % 16: a X's factor, and the power of two that the scores' row has been divided by
+        const auto factors = [&](int t, float& d, float& up) {
+            d = r.so * l.lam[kChunk + t * 16 + r16];
+            up = 1.f;
+            if constexpr (kScaled<T>) {
+                up = l.ps[t * 16 + r16];
+                d *= __uint_as_float((254u << 23) - __float_as_uint(up));        // one over a power of two
+            }
+        };
+        const auto decayed = [&](int j, float d, f32x4 v) {
+            if constexpr (kScaled<T>) return v * (*reinterpret_cast<const f32x4*>(&l.xs[(w + kWaves * j) * 16 + q * 4]) * d);
+            else return v * d;
+        };
+        float up[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            float v[4];
+            float d;
+            factors(t, d, up[t]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {   // (l^d is 0 behind the row, but 0 times a NaN is none)
-                const float x = r.ps * lam[t][e] * sc[t][e];
-                v[e] = row >= t * 16 + q * 4 + e ? x : 0.f;
-                if constexpr (kScaled<T>) v[e] *= ps.down;
-            }
-            lds_put4(&l.p[w][r16][t * 16 + q * 4], v);
+            for (int j = 0; j < kJ; ++j) o[t][j] = decayed(j, d, o[t][j]);
         }
-        wave_sync();
-        Piece<T> pk[kChunk / kInner];
+        {
+            Piece<T> fc[2][kJ], fp[2][4];
+            in_groups<kChunk / kInner * kU, 1>(
+                [&](int g, int at) {
+                    const int k = g / kU, u = g % kU;
+                    if (u == 0)
 #pragma unroll
-        for (int k = 0; k < kChunk / kInner; ++k) pk[k] = lds_piece(&l.p[w][r16][k * kInner + q * kN]);
-        in_groups<kChunk / kInner * kFour, 2>(
-            [&](int g, int at) {
+                        for (int j = 0; j < kJ; ++j) fc[k % 2][j] = lds_column(&l.c[k * kInner + q * kN][(w + kWaves * j) * 16], kRowC);
 #pragma unroll
-                for (int t = 0; t < 4; ++t)
-                    f[at][t] = lds_column(&l.c[g / kFour * kInner + q * kN][(g % kFour * 4 + t) * 16], kRowC);
-            },
-            [&](int g, int at) {
+                    for (int t = 0; t < 4; ++t)
+                        if (k * kInner < (t + 1) * 16) fp[at][t] = lds_piece(&l.p[u][t * 16 + r16][k * kInner + q * kN]);
+                },
+                [&](int g, int at) {
+                    const int k = g / kU;
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    f32x4& d = o[g % kFour * 4 + t];
-                    d = mma(f[at][t], pk[g / kFour], d);
-                }
-            });
-        if constexpr (kScaled<T>)
+                    for (int j = 0; j < kJ; ++j)
 #pragma unroll
-            for (int j = 0; j < kTiles; ++j) o[j] *= ps.up;
-        if (row < n) {
-            const int64_t tok = r.rev ? p.L - 1 - (base + row) : base + row;
-            if (wide) {
-#pragma unroll
-                for (int j = 0; j < kTiles; ++j) put4(std::true_type(), tok, j * 16 + q * 4, o[j]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < kTiles; ++j) put4(std::false_type(), tok, j * 16 + q * 4, o[j]);
-            }
+                        for (int t = 0; t < 4; ++t)
+                            if (k * kInner < (t + 1) * 16) o[t][j] = mma(fc[k % 2][j], fp[at][t], o[t][j]);
+                });
         }
-        if (__builtin_amdgcn_readfirstlane(l.odd) == chunk && row < n) {
+        // (elements from the first row of out to position `base`'s, and on from one position to the next)
+        const int64_t o_base = (r.rev ? p.L - 1 - base : base) * out_row, o_step = r.rev ? -out_row : out_row;
+        const int64_t o_lane = r16 * o_step;
+        const auto put = [&](int t, int j, f32x4 v) {
+            if (t * 16 + r16 >= n) return;
+            const int64_t el = o_base + t * 16 * o_step + o_lane;
+            if (wide) put4(std::true_type(), el, (w + kWaves * j) * 16 + q * 4, v);
+            else put4(std::false_type(), el, (w + kWaves * j) * 16 + q * 4, v);
+        };
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < kJ; ++j) put(t, j, kScaled<T> ? o[t][j] * up[t] : o[t][j]);
+        if (__builtin_amdgcn_readfirstlane(l.odd) == chunk) {
             // Zeros behind a row's own position times an infinity or a NaN there were NaN in what has just been written: once
-            // more, one product after the other, up to the row.  (Kept out of the way of the products above: as their other
-            // branch it cost them their reads ahead, 146 -> 183 us for the gradient of 4 x 2048 rows.)
-            const int64_t tok = r.rev ? p.L - 1 - (base + row) : base + row;
-            for (int d = q * 4; d < dc; d += 16) {
-                f32x4 v = {0.f, 0.f, 0.f, 0.f};
-                for (int i = 0; i < da; ++i) {
-                    const float x = a.value(base + row, i);
+            // more, with the scores' products one after the other, up to the row.  (Kept out of the way of the products above: as
+            // their other branch it cost them their reads ahead, a quarter more time for the gradient of 4 x 2048 rows.)
+#pragma unroll 1
+            for (int t = 0; t < 4; ++t) {
+                float d, up;
+                factors(t, d, up);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] += x * to_float(l.x[d + e][i]);
-                }
-                v *= decayed;
-                if constexpr (kScaled<T>) v *= *reinterpret_cast<const f32x4*>(&l.xs[d]);
-                for (int t = 0; t <= row; ++t) {
-                    const float x = to_float(l.p[w][r16][t]) * ps.up;
+                for (int j = 0; j < kJ; ++j) {
+                    f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] += x * to_float(l.c[t][d + e]);
+                    for (int m = 0; m < kK; ++m) {
+                        Piece<T> x[kU];
+                        x_pieces<T, DP, DC>(S, j, m, down[j], x);
+                        const Piece<T> f = a_piece(&l.a[t * 16 + r16][0], m, q);
+#pragma unroll
+                        for (int u = 0; u < kU; ++u) v = mma(x[u], f, v);
+                    }
+                    v = decayed(j, d, v);
+                    for (int i = 0; i <= t * 16 + r16; ++i) {
+                        float x = 0.f;
+#pragma unroll
+                        for (int u = 0; u < kU; ++u) x += to_float(l.p[u][t * 16 + r16][i]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] += x * to_float(l.c[i][(w + kWaves * j) * 16 + q * 4 + e]);
+                    }
+                    put(t, j, v * up);
                 }
-                if (wide) put4(std::true_type(), tok, d, v);
-                else put4(std::false_type(), tok, d, v);
             }
         }
         if (more || (last && s_out)) {
@@ -827,11 +889,12 @@ __global__ __launch_bounds__(256) void step_kernel(Mat Q, Mat K, Mat V, const fl
 
 // ---------------------------------------------------------------- host
 
-// How many segments time is cut into.  In the time that a workgroup takes for a chunk (4 us at 128 dimensions of 16 bits):
+// How many segments time is cut into.  In the time that a workgroup takes for a chunk (about 4 us at 128 dimensions of 16 bits):
 // a sequence of c chunks takes c; in n segments it takes c / n, and half as much again for kv_kernel, 6 for the other two
 // launches and the states' way through memory, times the rounds in which the device takes all the workgroups, one for each
 // of its units (two at once take twice as long: they are bound by memory).  Measured (us), 2 x 4096 rows, 16 heads of 128,
-// bfloat16: n = 4 97, 8 80, 16 89; gradient of 4 x 2048 ragged rows: n = 1 111, 2 157.
+// bfloat16: n = 4 109, 6 99, 8 85, 11 92, 16 85; gradient of 4 x 2048 ragged rows: n = 1 131, 2 163, 4 159 (n = 1 with two
+// workgroups for a head's columns, 172 with one); float32, 3 x 1531 ragged rows of 6 heads: n = 4 104, 14 65.
 void cut(Args& a) {
     const int64_t c = (a.T + kChunk - 1) / kChunk, units = (int64_t)a.B * a.H * a.roles, cu = cu_count();
     double best = 0.0;
@@ -865,9 +928,10 @@ int launch(Args& a, const int (&joined)[2], int joins, hipStream_t st) {
     static samx::LdsGrant grant;
     // As long as the device has a unit for every workgroup two of them share a head's columns, each with all the scores: two
     // on a unit hide each other's waits.  Where it holds more anyway the scores made twice cost more.  One against two,
-    // bf16, 16 heads of 128: 8 x 512 rows 46 and 34 us, 16 x 1024 93 and 91, 32 x 1024 155 and 171; gradient of 4 x 2048
-    // ragged rows 151 and 111, of 16 x 1024 209 and 230.  float32's tiles leave LDS for one on a unit: there as long as both
-    // halves have a unit of their own (8 x 512 rows 155 and 95; gradient of 4 x 512 rows, 8 heads of 72 and 88, 132 and 84).
+    // bf16, 16 heads of 128: 8 x 512 rows 53 and 40 us, 16 x 1024 108 and 105, 32 x 1024 165 and 205; gradient of 4 x 2048
+    // ragged rows 172 and 131, of 16 x 1024 233 and 277.  float32's tiles leave LDS for one on a unit: there as long as both
+    // halves have a unit of their own (8 x 512 rows 145 and 91, 16 x 1024 289 and 337; gradient of 4 x 512 rows, 8 heads of 72
+    // and 88, 129 and 82).
     if constexpr (DP == 128) {
         if ((int64_t)a.B * a.H * a.roles * a.nseg * (sizeof(T) == 4 ? 2 : 1) <= cu_count()) {
             a.parts = 2;

@@ -1100,7 +1100,8 @@ def linattn(q, k, v, decay, scale=1.0, state=None, lengths=None, out=None, state
     """Linear attention with a decay for each head, S_t = exp(decay) S_{t-1} + k_t v_t^T, out_t = scale q_t^T S_t, over
     whole sequences: q [B, T, H, D], k [B, T, HK, D], v [B, T, HK, DV] in float32, bfloat16 or float16 (views of a joint
     projection may be given), decay float32 [H], state float32 [B, H, D, DV] before the first row (None: zero), lengths
-    int32 [B] (None: T).  Returns (out [B, T, H, DV], the state behind the last row) (samx_linattn)."""
+    int32 [B] (None: T).  Returns (out [B, T, H, DV], the state behind the last row).  Scores and the state are float32 whatever
+    the type, an output is rounded once; float16 has no narrower range than bfloat16 but for its outputs (samx_linattn)."""
     s, dev, lead, pq, pk, pv, pd = _linattn_args(q, k, v, decay, 4)
     shape = (s.B, s.H, s.D, s.DV)
     ps, pl = _opt_on(state, dev, F32, shape, 'state'), _opt_on(lengths, dev, I32, (s.B,), 'lengths')

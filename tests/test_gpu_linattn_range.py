@@ -137,3 +137,27 @@ def test_rows_beside_one_that_is_not_finite(dtype, D, DV, bad, what):
         within(x[same], w[same], tol[same], n)
         if not bool(same.all()):
             assert not bool(torch.isfinite(x[~same]).all(-1).any()), n
+
+
+@pytest.mark.parametrize('dtype', [BF16, F16])
+@pytest.mark.parametrize('B,T,H,HK,D,DV,lengths', [(2, 200, 2, 2, 64, 64, None), (3, 150, 4, 2, 128, 128, [150, 64, 97]), (2, 130, 2, 1, 45, 100, None),
+                                                   (1, 1100, 2, 2, 128, 72, None), (66, 70, 4, 4, 96, 128, [70 - b for b in range(66)])])
+def test_outputs_of_16_bits_are_rounded_once(B, T, H, HK, D, DV, lengths, dtype):
+    """Scores and the state's copy meet the values as two numbers each, so half a step squared is lost there (twice, and once
+    more where the state's terms are split); the output's own rounding is the only one of half a step."""
+    from sam_tf_amd import ops
+    scale = D ** -0.5
+    c = _case(B, T, H, HK, D, DV, dtype, seed=36, lengths=lengths)
+    g, d = _gpu(c), _d(c)
+    a = _abs(d)
+    step, f = half_step(dtype), _errors(F32, T, D, DV)[0]
+    run = lambda x: (R.linattn(x['q'], x['k'], x['v'], d['decay'], scale, x['state'], d['lengths'])[:1] +
+                     R.linattn_grad(x['q'], x['k'], x['v'], d['decay'], x['dout'], scale, x['state'], x['dstate'], d['lengths'])[:3])
+    kw = dict(scale=scale, state=g['state'], lengths=g['lengths'])
+    got = ops.linattn(g['q'], g['k'], g['v'], g['decay'], **kw)[:1] + \
+        ops.linattn_grad(g['q'], g['k'], g['v'], g['decay'], g['dout'], dstate=g['dstate'], **kw)[:3]
+    q, k, v, o, S, dS = (_most(c[n]) for n in ('q', 'k', 'v', 'dout', 'state', 'dstate'))
+    S, G = S + T * k * v, dS + T * scale * q * o
+    low = 0.0 if dtype == BF16 else 2.0 ** -38 * (T + 64) * max(D, DV) * max(scale * q * S, scale * o * S, 2 * v * G, 2 * k * G)  # (as in _hold)
+    for x, w, m, n in zip(got, run(d), run(a), ('out', 'dq', 'dk', 'dv')):
+        within(x, w, (f + (H + 2) * U32 + 3.3 * step * step) * m + step * (1 + step) * w.abs() + smallest(dtype) + low, n)
