@@ -161,3 +161,52 @@ def test_outputs_of_16_bits_are_rounded_once(B, T, H, HK, D, DV, lengths, dtype)
     low = 0.0 if dtype == BF16 else 2.0 ** -38 * (T + 64) * max(D, DV) * max(scale * q * S, scale * o * S, 2 * v * G, 2 * k * G)  # (as in _hold)
     for x, w, m, n in zip(got, run(d), run(a), ('out', 'dq', 'dk', 'dv')):
         within(x, w, (f + (H + 2) * U32 + 3.3 * step * step) * m + step * (1 + step) * w.abs() + smallest(dtype) + low, n)
+
+
+@pytest.mark.parametrize('bad', [float('inf'), float('nan')])
+@pytest.mark.parametrize('dtype,D,DV', [(F32, 24, 40), (BF16, 40, 24), (F16, 64, 64), (F16, 100, 128), (BF16, 128, 128)])
+def test_a_state_that_is_not_finite_in_one_place(dtype, D, DV, bad):
+    """Element (3, 5) of one head's state meets column 5 of out and element 3 of dq; of its gradient, element 3 of dk and
+    column 5 of dv.  Everything else has the same bits."""
+    from sam_tf_amd import ops
+    c = _gpu(_case(2, 150, 2, 2, D, DV, dtype, seed=37))
+
+    def run(state, dstate):
+        return (ops.linattn(c['q'], c['k'], c['v'], c['decay'], 0.2, state) +
+                ops.linattn_grad(c['q'], c['k'], c['v'], c['decay'], c['dout'], 0.2, state, dstate))
+    want = run(c['state'], c['dstate'])
+    s, d = c['state'].clone(), c['dstate'].clone()
+    s[1, 1, 3, 5] = bad
+    d[1, 0, 3, 5] = bad
+    got = run(s, d)
+    meets = [torch.zeros(w.shape, dtype=torch.bool, device='cuda') for w in want]
+    out, state, dq, dk, dv, dstate = meets
+    out[1, :, 1, 5] = state[1, 1, 3, 5] = dq[1, :, 1, 3] = dk[1, :, 0, 3] = dv[1, :, 0, 5] = dstate[1, 0, 3, 5] = True
+    for x, w, m, n in zip(got, want, meets, ('out', 'state', 'dq', 'dk', 'dv', 'dstate')):
+        assert torch.equal(x[~m], w[~m]), n
+        assert not bool(torch.isfinite(x[m]).any()), n
+
+
+def test_float16_captured_and_replayed():
+    from sam_tf_amd import ops
+    g = _gpu(_case(3, 700, 2, 1, 128, 72, F16, seed=38, lengths=[700, 333, 64]))
+
+    def step():
+        return (ops.linattn(g['q'], g['k'], g['v'], g['decay'], 0.1, g['state'], g['lengths']) +
+                ops.linattn_grad(g['q'], g['k'], g['v'], g['decay'], g['dout'], 0.1, g['state'], g['dstate'], g['lengths']))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        for n in ('q', 'k', 'v', 'dout'):
+            g[n].copy_(torch.randn(g[n].shape, generator=torch.Generator().manual_seed(9 * i + len(n))) * 10.0 ** (1 - i))
+        g['lengths'].copy_(torch.tensor([700 - 150 * i, 90 * i, 64 + i], dtype=torch.int32))
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
