@@ -746,7 +746,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
             }
         };
         const auto decayed = [&](int j, float d, f32x4 v) {
-            if constexpr (kScaled<T>) return v * (*reinterpret_cast<const f32x4*>(&l.xs[(w + kWaves * j) * 16 + q * 4]) * d);
+            // (one factor after the other: their product can be an infinity where v is 0)
+            if constexpr (kScaled<T>) return (v * *reinterpret_cast<const f32x4*>(&l.xs[(w + kWaves * j) * 16 + q * 4])) * d;
             else return v * d;
         };
         float up[4];

@@ -210,3 +210,19 @@ def test_float16_captured_and_replayed():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+def test_rows_of_zeros_meet_a_huge_state(dtype):
+    """0 times a state of 1e30 is 0, also where the row's scores are zeros."""
+    from sam_tf_amd import ops
+    c = _case(2, 100, 2, 2, 72, 80, dtype, seed=39)
+    c['state'] *= 1e30
+    c['dstate'] *= 1e30
+    for n in ('q', 'k', 'v', 'dout'):
+        c[n][:, 30:71] = 0
+    g = _gpu(c)
+    out = ops.linattn(g['q'], g['k'], g['v'], g['decay'], scale=0.5, state=g['state'])[0]
+    got = ops.linattn_grad(g['q'], g['k'], g['v'], g['decay'], g['dout'], scale=0.5, state=g['state'], dstate=g['dstate'])[:3]
+    for x in (out,) + got:
+        assert bool((x[:, 30:71] == 0).all())
