@@ -932,7 +932,7 @@ SEQ_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # SAMX_F3
 _NORM = {'rms': 0, 'layer': 1}
 
 
-# a device's current stream, and the current device: torch's own calls below the public ones (half a microsecond each less),
+# a device's current stream, and the current device: torch's own calls below the public ones (0.1 us each, not 1.1 and 0.2),
 # where this torch has them
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 _current_device = getattr(torch._C, '_cuda_getDevice', None) or torch.cuda.current_device
